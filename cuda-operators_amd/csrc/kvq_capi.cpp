@@ -16,21 +16,20 @@
 #include <vector>
 
 #include "../../include/kvq.h"
+#include "kvq_call.hpp"
 #include "kvq_internal.hpp"
 
 namespace {
 
+using kvq::checked_call;
+using kvq::debug_sync;
 using kvq::DecodeArgs;
 using kvq::DecodePlan;
+using kvq::env_on;
+using kvq::kCounterBytes;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr size_t kAlign = 256;
-// Arrival counters live in a fixed-size prefix of every workspace, so a
-// workspace zero-filled once stays valid for any later problem shape: the
-// counters are only ever written as counters (and left at zero), partial
-// records always start after the prefix.  Problems with more sequence groups
-// than counters use the separate merge kernel instead.
-constexpr size_t kCounterBytes = 256 * 1024;
 constexpr long kMaxCounters = static_cast<long>(kCounterBytes / sizeof(int));
 // Workgroups a decode launch aims for when it picks the split count itself
 // (MI355X: 256 CUs).  An 8-wave VALU workgroup fills a CU's issue slots on its
@@ -89,20 +88,6 @@ size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 // * KVQ_PREFILL_MAX_GROUPS: a positive integer caps the prefill quantiser's
 //   workgroups per plane (default and maximum 2^20), so tests can run its
 //   grid-stride loop on small inputs.
-bool env_on(const char* name) {
-    const char* s = getenv(name);
-    if (!s) return false;
-    static const char* const kOn[] = {"1", "true", "yes", "on", "TRUE", "YES", "ON", "True", "Yes", "On"};
-    for (const char* o : kOn)
-        if (strcmp(s, o) == 0) return true;
-    return false;
-}
-
-bool debug_sync() {
-    static const bool on = env_on("KVQ_DEBUG_SYNC");
-    return on;
-}
-
 enum ForcedKernel { kForceNone = 0, kForceValu = 1, kForceGeneric = 2 };
 
 // KVQ_FLAT_PLAN=0 keeps ragged matrix-core batches on the per-sequence item
@@ -142,54 +127,6 @@ int forced_kernel() {
         return static_cast<int>(kForceNone);
     }();
     return k;
-}
-
-// The library's code objects are built for gfx950 only.  Checked once per
-// device before its first launch, as the reference warns once about an
-// untuned architecture (kv_cache/KV_int8_split_optimized.cu:57-65); here
-// another architecture cannot run the kernels at all, so the call fails with
-// hipErrorInvalidDevice after one stderr line.
-std::mutex g_arch_mutex;
-signed char g_arch_state[64];  // 0 unknown, 1 gfx950, -1 other
-
-hipError_t arch_check() {
-    int dev = 0;
-    hipError_t err = hipGetDevice(&dev);
-    if (err != hipSuccess) return err;
-    if (dev < 0 || dev >= 64) return hipErrorInvalidDevice;
-    std::lock_guard<std::mutex> lock(g_arch_mutex);
-    if (g_arch_state[dev] == 0) {
-        hipDeviceProp_t prop;
-        err = hipGetDeviceProperties(&prop, dev);
-        if (err != hipSuccess) return err;
-        const bool ok = strncmp(prop.gcnArchName, "gfx950", 6) == 0 &&
-                        (prop.gcnArchName[6] == '\0' || prop.gcnArchName[6] == ':');
-        g_arch_state[dev] = ok ? 1 : -1;
-        if (!ok)
-            fprintf(stderr, "[kvq] device %d is %s; libkvq is built for gfx950 (MI355X) only\n", dev,
-                    prop.gcnArchName);
-    }
-    return g_arch_state[dev] > 0 ? hipSuccess : hipErrorInvalidDevice;
-}
-
-// Every launching entry point returns through here: the device check, the
-// launches, then (KVQ_DEBUG_SYNC) the stream's completion status.
-hipError_t finish_call(hipError_t err, hipStream_t stream);
-template <class Launch>
-hipError_t checked_call(hipStream_t stream, Launch&& launch) {
-    const hipError_t err = arch_check();
-    if (err != hipSuccess) return err;
-    return finish_call(launch(), stream);
-}
-
-hipError_t finish_call(hipError_t err, hipStream_t stream) {
-    if (err != hipSuccess || !debug_sync()) return err;
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    err = hipStreamIsCapturing(stream, &st);
-    if (err != hipSuccess || st != hipStreamCaptureStatusNone) return err;
-    // The launchers already returned their launch status; the caller's own
-    // pending error (hipGetLastError) is left for the caller.
-    return hipStreamSynchronize(stream);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -174,6 +174,11 @@ __device__ __forceinline__ int buffer_load4(buf_rsrc r, int voff, int soff) {
 // v_exp_f32: 2^x, exp2(-inf) == 0.
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// fp32 to bf16, to nearest even (v_cvt_pk_bf16_f32).
+__device__ __forceinline__ uint16_t bf16_of(float x) {
+    return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
+}
+
 // ---------------------------------------------------------------------------
 // Per-token symmetric int8 quantiser.  scale = amax / 127.0f with IEEE division
 // (HIP's default correctly rounded fp32 divide), q = clamp(rintf(x / scale),

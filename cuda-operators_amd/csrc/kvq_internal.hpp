@@ -115,6 +115,13 @@ enum class Kernel {
     Mfma,     // decode_mfma: d a multiple of 16 from 48 to 128, up to 8 query heads per kv head group
 };
 
+// Arrival counters live in a fixed-size prefix of every workspace, so a
+// workspace zero-filled once stays valid for any later problem shape: the
+// counters are only ever written as counters (and left at zero), partial
+// records always start after the prefix.  Problems with more sequence groups
+// than counters use the separate merge kernel instead.
+constexpr size_t kCounterBytes = 256 * 1024;
+
 // Launch plan chosen on the host.
 struct DecodePlan {
     Kernel kernel;

@@ -1,0 +1,351 @@
+// kvq_pages.hip -- gfx950 kernels around a paged cache: page maps, packed cache
+// writes and reads, key bounds of pages.
+#include <limits.h>
+#include <math.h>
+
+#include "kvq_bounds.hpp"
+#include "kvq_device.hpp"
+#include "kvq_pages.hpp"
+
+namespace kvq {
+namespace {
+
+// ---------------------------------------------------------------------------
+// Page map: block tables, free pages and slots from request lengths.
+// ---------------------------------------------------------------------------
+// With old_b and new_b a sequence's lengths and P(x) = ceil(x / page size), it
+// needs max(P(new) - P(old), 0) pages or gives up max(P(old) - P(new), 0).  Two
+// prefix sums over the batch say everything else: that of the packed rows which
+// row is whose, those of the pages which place of the stack
+//   S = free_pages[0, F) ++ pages given up, in order (R of them)
+// is whose: growing sequences take S[F + R - 1], S[F + R - 2], .. in order, so
+// where the prefix sum is beyond F + R the request is refused (sums only grow,
+// so the granted ones' sum is their own prefix).  The A pages taken leave
+// S[0, F + R - A); of these the places from F on are written back.  Places read
+// to hand out, [F + R - A, F) and pages given up, are never written, so the
+// workgroups need no order among them; only lengths and the free count, which
+// may be updated in place, are written by the last workgroup to arrive.
+// Bound by latency: the loads of the lengths, two scans, a dependent load of a
+// page id, the stores.
+constexpr int kMapThreads = 1024;
+constexpr int kMapWaves = kMapThreads / kWave;
+
+__device__ __forceinline__ unsigned long long wave_inclusive_scan64(unsigned long long v, int lane) {
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) {
+        const unsigned long long x = __shfl_up(v, off);
+        if (lane >= off) v += x;
+    }
+    return v;
+}
+
+// Inclusive scan of one value a thread over the workgroup; part: one entry a
+// wave, used by this scan alone.
+__device__ __forceinline__ unsigned long long group_inclusive_scan(unsigned long long v, unsigned long long* part) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = threadIdx.x / kWave;
+    v = wave_inclusive_scan64(v, lane);
+    if (lane == kWave - 1) part[wave] = v;
+    __syncthreads();
+    for (int w = 0; w < wave; w++) v += part[w];
+    return v;
+}
+
+__device__ __forceinline__ int pages_of(int tokens, const FastDiv& page) {
+    return static_cast<int>(fastdiv(static_cast<uint32_t>(tokens) + page.d - 1, page));
+}
+
+// What sequence b asks for.  off: its first packed row, saturated at a.T.
+struct Request {
+    int old, want;  // tokens held, and if its pages are granted
+    int rows, need, gives;
+};
+__device__ __forceinline__ Request request_of(const PageMapArgs& a, int b, long long off) {
+    Request r;
+    const int n = a.new_tokens[b];
+    r.old = min(max(a.lengths[b], 0), a.cap);
+    r.rows = max(n, 0);
+    if (n < 0) r.want = max(r.old + n, 0);
+    else r.want = n <= a.cap - r.old && off + n <= a.T ? r.old + n : r.old;
+    const int p0 = pages_of(r.old, a.page), p1 = pages_of(r.want, a.page);
+    r.need = max(p1 - p0, 0);
+    r.gives = max(p0 - p1, 0);
+    return r;
+}
+
+// The last i in [0, n) with v[i] <= x, for ascending v with v[0] <= x.
+__device__ __forceinline__ int last_not_above(const int* v, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (v[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__global__ __launch_bounds__(kMapThreads) void page_map_kernel(const PageMapArgs a) {
+    extern __shared__ int s_map[];  // B + 1 row offsets, B needs, B gives (exclusive prefix sums)
+    __shared__ unsigned long long s_part[2][kMapWaves];
+    __shared__ int s_taken[kMapWaves];
+    __shared__ int s_last;
+    int* s_off = s_map;
+    int* s_need = s_map + a.B + 1;
+    int* s_gives = s_need + a.B;
+    const int t = threadIdx.x;
+    const int lane = t & (kWave - 1);
+    const int wave = t / kWave;
+    const int per = (a.B + kMapThreads - 1) / kMapThreads;
+    const int b0 = min(t * per, a.B), b1 = min(b0 + per, a.B);
+
+    unsigned long long rows = 0;
+    for (int b = b0; b < b1; b++) rows += static_cast<unsigned>(max(a.new_tokens[b], 0));
+    unsigned long long at = group_inclusive_scan(rows, s_part[0]) - rows;
+    for (int b = b0; b < b1; b++) {
+        s_off[b] = static_cast<int>(min(at, static_cast<unsigned long long>(a.T)));
+        at += static_cast<unsigned>(max(a.new_tokens[b], 0));
+    }
+    if (b1 == a.B) s_off[a.B] = static_cast<int>(min(at, static_cast<unsigned long long>(a.T)));  // every such thread alike
+
+    // Pages: needs in the low half, gives in the high half (both below 2^31:
+    // B * max_pages is).
+    unsigned long long sum = 0;
+    for (int b = b0; b < b1; b++) {
+        const Request r = request_of(a, b, s_off[b]);
+        sum += (static_cast<unsigned long long>(static_cast<unsigned>(r.gives)) << 32) | static_cast<unsigned>(r.need);
+    }
+    at = group_inclusive_scan(sum, s_part[1]) - sum;
+    unsigned long long total = 0;
+    for (int w = 0; w < kMapWaves; w++) total += s_part[1][w];
+    const int F = min(max(*a.free_count, 0), a.num_pages);
+    const long long have = static_cast<long long>(F) + static_cast<long long>(total >> 32);  // F + R
+    int taken = 0;
+    for (int b = b0; b < b1; b++) {
+        const Request r = request_of(a, b, s_off[b]);
+        s_need[b] = static_cast<int>(at & 0xffffffffu);
+        s_gives[b] = static_cast<int>(at >> 32);
+        at += (static_cast<unsigned long long>(static_cast<unsigned>(r.gives)) << 32) | static_cast<unsigned>(r.need);
+        const int incl = s_need[b] + r.need;
+        if (incl <= have) taken = max(taken, incl);
+    }
+#pragma unroll
+    for (int off = kWave / 2; off > 0; off >>= 1) taken = max(taken, __shfl_xor(taken, off));
+    if (lane == 0) s_taken[wave] = taken;
+    __syncthreads();
+    int A = 0;
+    for (int w = 0; w < kMapWaves; w++) A = max(A, s_taken[w]);
+    const long long left = have - A;  // entries of the stack afterwards
+
+    auto granted = [&](int b, const Request& r) { return r.need == 0 || s_need[b] + r.need <= have; };
+    auto given_up = [&](int g) {  // the g-th page given up
+        const int c = last_not_above(s_gives, a.B, g);
+        const Request r = request_of(a, c, s_off[c]);
+        return a.table[static_cast<size_t>(c) * a.max_pages + pages_of(r.want, a.page) + (g - s_gives[c])];
+    };
+    auto stack_at = [&](long long i) { return i < F ? a.free_pages[i] : given_up(static_cast<int>(i - F)); };
+
+    // Pages: a wave a sequence.
+    const int waves = gridDim.x * kMapWaves;
+    for (int b = blockIdx.x * kMapWaves + wave; b < a.B; b += waves) {
+        const Request r = request_of(a, b, s_off[b]);
+        int32_t* row = a.table + static_cast<size_t>(b) * a.max_pages;
+        if (r.need > 0 && granted(b, r)) {
+            const int p0 = pages_of(r.old, a.page);
+            for (int i = lane; i < r.need; i += kWave) row[p0 + i] = stack_at(have - 1 - (s_need[b] + i));
+        }
+        const int p1 = pages_of(r.want, a.page);
+        for (int i = lane; i < r.gives; i += kWave) {
+            const long long to = static_cast<long long>(F) + s_gives[b] + i;
+            if (to < left && to < a.num_pages) a.free_pages[to] = row[p1 + i];
+        }
+    }
+
+    // Packed rows.  A new page's id is taken from the stack again rather than
+    // from the table, which another wave may not have written yet.
+    if (a.slot_map || a.token_seq || a.token_pos) {
+        const long long step = static_cast<long long>(gridDim.x) * kMapThreads;
+        for (long long i = static_cast<long long>(blockIdx.x) * kMapThreads + t; i < a.T; i += step) {
+            int slot = -1, seq = -1, pos = -1;
+            const int row = static_cast<int>(i);
+            if (row < s_off[a.B]) {
+                seq = last_not_above(s_off, a.B, row);
+                const Request r = request_of(a, seq, s_off[seq]);
+                const int k = row - s_off[seq];
+                pos = static_cast<int>(min(static_cast<long long>(r.old) + k, static_cast<long long>(INT_MAX)));
+                if (k < r.want - r.old && granted(seq, r)) {
+                    const int pi = static_cast<int>(fastdiv(static_cast<uint32_t>(pos), a.page));
+                    const int p0 = pages_of(r.old, a.page);
+                    const int id = pi < p0 ? a.table[static_cast<size_t>(seq) * a.max_pages + pi]
+                                           : stack_at(have - 1 - (s_need[seq] + pi - p0));
+                    const int size = static_cast<int>(a.page.d);
+                    if (id >= 0 && id < a.num_pages) slot = id * size + (pos - pi * size);
+                }
+            }
+            if (a.slot_map) a.slot_map[i] = slot;
+            if (a.token_seq) a.token_seq[i] = seq;
+            if (a.token_pos) a.token_pos[i] = pos;
+        }
+    }
+
+    // The last workgroup writes what the others read.
+    __syncthreads();
+    if (a.arrivals) {
+        if (t == 0)
+            s_last = __hip_atomic_fetch_add(a.arrivals, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                     static_cast<int>(gridDim.x) - 1;
+        __syncthreads();
+        if (!s_last) return;
+        if (t == 0) __hip_atomic_store(a.arrivals, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    for (int b = b0; b < b1; b++) {
+        const Request r = request_of(a, b, s_off[b]);
+        const int now = granted(b, r) ? r.want : r.old;
+        a.new_lengths[b] = now;
+        a.granted[b] = now - r.old;
+        a.offsets[b] = s_off[b];
+    }
+    if (t == 0) {
+        a.offsets[a.B] = s_off[a.B];
+        *a.new_free_count = static_cast<int>(min(left, static_cast<long long>(a.num_pages)));
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Packed rows into and out of their slots.
+// ---------------------------------------------------------------------------
+constexpr int kSlotWaves = 4;
+
+// Pool row of token t's row for kv head h; -1: the slot lies outside the pool.
+__device__ __forceinline__ long long slot_row(const SlotArgs& a, int t, int h) {
+    const int s = a.slots[t];
+    if (s < 0 || s >= a.slots_in_pool) return -1;
+    const int page = static_cast<int>(fastdiv(static_cast<uint32_t>(s), a.page));
+    const int size = static_cast<int>(a.page.d);
+    return (static_cast<long long>(page) * a.Hkv + h) * size + (s - page * size);
+}
+
+template <bool BF16>
+__device__ __forceinline__ float row_elem(const void* x, int64_t i) {
+    if constexpr (BF16) return __uint_as_float(static_cast<unsigned>(static_cast<const uint16_t*>(x)[i]) << 16);
+    else return static_cast<const float*>(x)[i];
+}
+
+// Any head dim, stride or alignment: a wave a row, an element a load.
+template <bool BF16>
+__global__ __launch_bounds__(kSlotWaves* kWave) void slot_write_generic(const SlotArgs a) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int kv = blockIdx.y;
+    const void* x = kv ? a.v_rows : a.k_rows;
+    const int64_t stride = kv ? a.v_stride : a.k_stride;
+    int8_t* qo = kv ? a.v : a.k;
+    float* so = kv ? a.vs : a.ks;
+    const unsigned rows = static_cast<unsigned>(a.T) * a.Hkv;
+    const unsigned step = gridDim.x * kSlotWaves;
+    for (unsigned r = blockIdx.x * kSlotWaves + threadIdx.x / kWave; r < rows; r += step) {
+        const int t = static_cast<int>(fastdiv(r, a.heads));
+        const int h = static_cast<int>(r - static_cast<unsigned>(t) * a.Hkv);
+        const long long orow = slot_row(a, t, h);
+        if (orow < 0) continue;
+        const int64_t x0 = t * stride + h * a.head_stride;
+        float am = 0.0f;
+        for (int i = lane; i < a.d; i += kWave) am = fmaxf(am, fabsf(row_elem<BF16>(x, x0 + i)));
+        const float scale = quant_scale(wave_max(am));
+        for (int i = lane; i < a.d; i += kWave)
+            qo[orow * a.d + i] = static_cast<int8_t>(quant_one(row_elem<BF16>(x, x0 + i), scale));
+        if (lane == 0) so[orow] = scale;
+    }
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(kSlotWaves* kWave) void slot_read_generic(const SlotArgs a) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int kv = blockIdx.y;
+    void* x = kv ? a.v_rows : a.k_rows;
+    const int64_t stride = kv ? a.v_stride : a.k_stride;
+    const int8_t* qi = kv ? a.v : a.k;
+    const float* si = kv ? a.vs : a.ks;
+    const unsigned rows = static_cast<unsigned>(a.T) * a.Hkv;
+    const unsigned step = gridDim.x * kSlotWaves;
+    for (unsigned r = blockIdx.x * kSlotWaves + threadIdx.x / kWave; r < rows; r += step) {
+        const int t = static_cast<int>(fastdiv(r, a.heads));
+        const int h = static_cast<int>(r - static_cast<unsigned>(t) * a.Hkv);
+        const long long irow = slot_row(a, t, h);
+        const float scale = irow < 0 ? 0.0f : si[irow];
+        const int64_t x0 = t * stride + h * a.head_stride;
+        for (int i = lane; i < a.d; i += kWave) {
+            const float y = irow < 0 ? 0.0f : static_cast<float>(qi[irow * a.d + i]) * scale;
+            if constexpr (BF16) static_cast<uint16_t*>(x)[x0 + i] = bf16_of(y);
+            else static_cast<float*>(x)[x0 + i] = y;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Key bounds of pages.
+// ---------------------------------------------------------------------------
+constexpr int kBoundsWaves = 4;
+
+// Any head dim, page size or alignment: a wave a (page, kv head), workgroups
+// blockIdx.y of sequence blockIdx.x striding over its pages.
+__global__ __launch_bounds__(kBoundsWaves* kWave) void page_bounds_generic(const BoundsArgs a) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int b = blockIdx.x;
+    const int len = a.lengths ? min(max(a.lengths[b], 0), a.max_len) : a.max_len;
+    const int first = a.start ? max(a.start[b], 0) : 0;
+    if (first >= len) return;
+    const int size = a.pages.size;
+    const int p0 = first / size;
+    const int pages = (len - 1) / size + 1 - p0;
+    const long long units = static_cast<long long>(pages) * a.Hkv;
+    for (long long u = static_cast<long long>(blockIdx.y) * kBoundsWaves + threadIdx.x / kWave; u < units;
+         u += static_cast<long long>(gridDim.y) * kBoundsWaves) {
+        const int pi = p0 + static_cast<int>(u / a.Hkv);
+        const int h = static_cast<int>(u % a.Hkv);
+        const int tokens = min(size, len - pi * size);
+        bounds_generic(a, b, pi, h, tokens, lane);
+    }
+}
+
+}  // namespace
+
+int page_map_groups(const PageMapArgs&) { return 1; }
+
+hipError_t launch_page_map(const PageMapArgs& a, hipStream_t stream) {
+    const size_t lds = sizeof(int) * (3 * static_cast<size_t>(a.B) + 1);
+    hipLaunchKernelGGL(page_map_kernel, dim3(static_cast<unsigned>(page_map_groups(a))), dim3(kMapThreads), lds, stream, a);
+    return hipGetLastError();
+}
+
+namespace {
+dim3 slot_grid(unsigned rows, unsigned rows_per_group) {
+    const unsigned groups = (rows + rows_per_group - 1) / rows_per_group;
+    return dim3(groups < (1u << 20) ? groups : (1u << 20), 2);
+}
+}  // namespace
+
+hipError_t launch_slot_write(const SlotArgs& a, bool bf16, bool, hipStream_t stream) {
+    if (a.T == 0) return hipSuccess;
+    const dim3 grid = slot_grid(static_cast<unsigned>(a.T) * a.Hkv, kSlotWaves), block(kSlotWaves * kWave);
+    if (bf16) hipLaunchKernelGGL((slot_write_generic<true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((slot_write_generic<false>), grid, block, 0, stream, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_slot_read(const SlotArgs& a, bool bf16, bool, hipStream_t stream) {
+    if (a.T == 0) return hipSuccess;
+    const dim3 grid = slot_grid(static_cast<unsigned>(a.T) * a.Hkv, kSlotWaves), block(kSlotWaves * kWave);
+    if (bf16) hipLaunchKernelGGL((slot_read_generic<true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((slot_read_generic<false>), grid, block, 0, stream, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_page_bounds(const BoundsArgs& a, bool, hipStream_t stream) {
+    // About 8192 workgroups at most; a sequence's workgroups stride over its pages.
+    const long long units = (static_cast<long long>(a.max_len - 1) / a.pages.size + 1) * a.Hkv;
+    const long long want = (units + kBoundsWaves - 1) / kBoundsWaves;
+    const unsigned ny = static_cast<unsigned>(min(want, max(1LL, 8192LL / a.B)));
+    hipLaunchKernelGGL(page_bounds_generic, dim3(static_cast<unsigned>(a.B), ny), dim3(kBoundsWaves * kWave), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace kvq

@@ -9,7 +9,8 @@ Entry points mirror the reference's kv_cache/ interface:
   kv_int8_split_launch(...)   -> kv_cache/KV_int8_split_optimized.cu:268
   kv_int8_simple_launch(...)  -> kv_cache/new_kvint8.cu:85
 plus the batched / GQA / ragged / append extension (decode, append,
-quantize_rows, workspace helpers).
+quantize_rows, workspace helpers) and the operators around a paged cache
+(PageMapper, slot_write, slot_read, page_bounds, SparseDecoder).
 """
 from __future__ import annotations
 
@@ -103,6 +104,55 @@ class AttentionParams(ctypes.Structure):
     ]
 
 
+PAGE_MAP_MAX_BATCH = 4096  # KVQ_PAGE_MAP_MAX_BATCH
+_i64 = ctypes.c_int64
+
+
+class PageMapParams(ctypes.Structure):
+    """struct kvq_page_map_params (include/kvq.h)."""
+    _fields_ = [
+        ("batch", _int), ("page_size", _int), ("num_pages", _int), ("max_pages_per_seq", _int), ("max_tokens", _int),
+        ("new_tokens", _vp), ("lengths", _vp), ("block_table", _vp), ("free_pages", _vp), ("free_count", _vp),
+        ("new_lengths", _vp), ("new_free_count", _vp), ("granted", _vp), ("token_offsets", _vp),
+        ("slot_map", _vp), ("token_seq", _vp), ("token_pos", _vp),
+    ]
+
+
+class SlotWriteParams(ctypes.Structure):
+    """struct kvq_slot_write_params (include/kvq.h)."""
+    _fields_ = [
+        ("tokens", _int), ("num_kv_heads", _int), ("head_dim", _int), ("page_size", _int), ("num_pages", _int),
+        ("dtype", _int), ("k_new", _vp), ("v_new", _vp), ("k_stride", _i64), ("v_stride", _i64), ("slots", _vp),
+        ("k_pages", _vp), ("v_pages", _vp), ("k_scale_pages", _vp), ("v_scale_pages", _vp),
+    ]
+
+
+class SlotReadParams(ctypes.Structure):
+    """struct kvq_slot_read_params (include/kvq.h)."""
+    _fields_ = [
+        ("tokens", _int), ("num_kv_heads", _int), ("head_dim", _int), ("page_size", _int), ("num_pages", _int),
+        ("dtype", _int), ("slots", _vp), ("k_pages", _vp), ("v_pages", _vp), ("k_scale_pages", _vp),
+        ("v_scale_pages", _vp), ("k_out", _vp), ("v_out", _vp), ("token_stride", _i64), ("head_stride", _i64),
+    ]
+
+
+class PageBoundsParams(ctypes.Structure):
+    """struct kvq_page_bounds_params (include/kvq.h)."""
+    _fields_ = [
+        ("batch", _int), ("num_kv_heads", _int), ("head_dim", _int), ("page_size", _int), ("num_pages", _int),
+        ("max_pages_per_seq", _int), ("max_seq_len", _int), ("block_table", _vp), ("start", _vp), ("lengths", _vp),
+        ("k_pages", _vp), ("k_scale_pages", _vp), ("bounds", _vp), ("bound_scale", _vp),
+    ]
+
+
+class SparseDecodeParams(ctypes.Structure):
+    """struct kvq_sparse_decode_params (include/kvq.h)."""
+    _fields_ = [
+        ("decode", PagedDecodeParams), ("max_selected", _int), ("keep_first", _int), ("keep_last", _int),
+        ("bounds", _vp), ("bound_scale", _vp), ("selected", _vp), ("selected_lengths", _vp),
+    ]
+
+
 class PlanInfo(ctypes.Structure):
     """struct kvq_plan_info (include/kvq.h part 6)."""
     _fields_ = [
@@ -121,7 +171,10 @@ EXPORTS = ("solve", "kv_int8_split_launch", "kv_int8_simple_launch", "kvq_decode
            "kvq_paged_decode_workspace_size", "kvq_paged_decode_launch", "kvq_paged_append_launch",
            "kvq_prefill_quantize_launch", "attention_online_launch", "kvq_attention_workspace_size",
            "kvq_attention_launch", "kvq_version", "kvq_reference_plan", "kvq_decode_plan", "kvq_attention_plan",
-           "kvq_diagnostics", "kvq_decode_launch_noalloc", "kvq_paged_decode_plan")
+           "kvq_diagnostics", "kvq_decode_launch_noalloc", "kvq_paged_decode_plan",
+           "kvq_page_map_workspace_size", "kvq_page_map_launch", "kvq_slot_write_launch", "kvq_slot_read_launch",
+           "kvq_page_bounds_launch", "kvq_sparse_decode_workspace_size", "kvq_sparse_decode_launch",
+           "kvq_sparse_decode_plan")
 
 
 class KvqError(RuntimeError):
@@ -181,6 +234,20 @@ def lib() -> ctypes.CDLL:
         L.kvq_attention_plan.argtypes = [ctypes.POINTER(AttentionParams), ctypes.POINTER(PlanInfo)]
         L.kvq_attention_plan.restype = _int
         L.kvq_diagnostics.restype = _int
+        L.kvq_page_map_workspace_size.argtypes = [ctypes.POINTER(PageMapParams)]
+        L.kvq_page_map_workspace_size.restype = ctypes.c_size_t
+        L.kvq_page_map_launch.argtypes = [ctypes.POINTER(PageMapParams), _vp, ctypes.c_size_t, _vp]
+        L.kvq_page_map_launch.restype = _int
+        for fn, cls in (("kvq_slot_write_launch", SlotWriteParams), ("kvq_slot_read_launch", SlotReadParams),
+                        ("kvq_page_bounds_launch", PageBoundsParams)):
+            getattr(L, fn).argtypes = [ctypes.POINTER(cls), _vp]
+            getattr(L, fn).restype = _int
+        L.kvq_sparse_decode_workspace_size.argtypes = [ctypes.POINTER(SparseDecodeParams)]
+        L.kvq_sparse_decode_workspace_size.restype = ctypes.c_size_t
+        L.kvq_sparse_decode_launch.argtypes = [ctypes.POINTER(SparseDecodeParams), _vp, ctypes.c_size_t, _vp]
+        L.kvq_sparse_decode_launch.restype = _int
+        L.kvq_sparse_decode_plan.argtypes = [ctypes.POINTER(SparseDecodeParams), ctypes.POINTER(PlanInfo)]
+        L.kvq_sparse_decode_plan.restype = _int
         _lib = L
         return L
 
@@ -517,6 +584,242 @@ def prefill(k_new, v_new, k_cache, v_cache, k_scale, v_scale, start=None, unifor
     _check("kvq_prefill_quantize_launch", lib().kvq_prefill_quantize_launch(ctypes.byref(p), _stream(stream)))
 
 
+# ---------------------------------------------------------------------------
+# a paged cache's life on the GPU (include/kvq.h part 7)
+# ---------------------------------------------------------------------------
+def _one_device(*tensors):
+    """The device that all of the tensors (None: absent) are on."""
+    device = None
+    for t in tensors:
+        if t is not None:
+            if device is not None and t.device != device:
+                raise ValueError(f"tensors on {device} and {t.device}")
+            device = t.device
+    return device
+
+
+def _call(fn, name, args, device, stream=None) -> None:
+    """One launch on `device`, whichever is current, and on `stream` (default: that device's current stream)."""
+    def launch():
+        handle = stream if isinstance(stream, int) else (stream or torch.cuda.current_stream(device)).cuda_stream
+        _check(name, fn(*args, handle))
+
+    if device.index is None or device.index == torch.cuda.current_device():
+        launch()
+    else:
+        with torch.cuda.device(device):
+            launch()
+
+
+def _new_workspace(nbytes, device, stream):
+    """A zeroed workspace that belongs to `stream` (so that memory freed after the last launch there is not handed out
+    before that launch ends); None when none is needed."""
+    if not nbytes:
+        return None
+    with torch.cuda.device(device):
+        if isinstance(stream, int):
+            # Not torch's null stream object: an external handle may be any stream of the device.
+            stream = torch.cuda.ExternalStream(stream, device) if stream else torch.cuda.default_stream(device)
+        stream = stream or torch.cuda.current_stream(device)
+        with torch.cuda.stream(stream):
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            workspace_init(ws, nbytes, stream)
+    return ws
+
+
+def _rows_of(t, name, n=None):
+    """Entries of a contiguous 1-d int32 cuda tensor (n: that many)."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 1:
+        raise ValueError(f"{name}: want a 1-d tensor")
+    _need(t, torch.int32, (t.shape[0] if n is None else n,), name)
+    return t.shape[0]
+
+
+class PageMapper:
+    """kvq_page_map_launch with its outputs and workspace: build once, launch before every step.
+
+    new_tokens [B] (negative: taken off the end), lengths [B], block_table [B, max_pages], free_pages [num_pages] (a
+    stack) and free_count [1], all int32.  lengths and free_count are updated in place unless new_lengths [B] and
+    new_free_count [1] are given; block_table and free_pages always are.  slot_map, token_seq and token_pos [T] (any of
+    them, else max_tokens) describe the packed rows.  Every output is an attribute."""
+
+    def __init__(self, new_tokens, lengths, block_table, free_pages, free_count, page_size, new_lengths=None,
+                 new_free_count=None, granted=None, token_offsets=None, slot_map=None, token_seq=None, token_pos=None,
+                 max_tokens=None, stream=None):
+        B = _rows_of(new_tokens, "new_tokens")
+        if block_table.dim() != 2 or block_table.shape[0] != B:
+            raise ValueError("block_table: want [B, max_pages_per_seq]")
+        _need(block_table, torch.int32, tuple(block_table.shape), "block_table")
+        num_pages = _rows_of(free_pages, "free_pages")
+        for name, t, n in (("lengths", lengths, B), ("free_count", free_count, 1), ("new_lengths", new_lengths, B),
+                           ("new_free_count", new_free_count, 1), ("granted", granted, B),
+                           ("token_offsets", token_offsets, B + 1)):
+            if t is not None or name in ("lengths", "free_count"):
+                _rows_of(t, name, n)
+        rows = [(name, t) for name, t in (("slot_map", slot_map), ("token_seq", token_seq), ("token_pos", token_pos)) if t is not None]
+        for name, t in rows:
+            T = _rows_of(t, name)
+            if max_tokens is not None and T != max_tokens:
+                raise ValueError(f"{name}: want {max_tokens} rows, got {T}")
+            max_tokens = T
+        max_tokens = 2**31 - 1 if max_tokens is None else int(max_tokens)
+        self.device = _one_device(new_tokens, lengths, block_table, free_pages, free_count, new_lengths, new_free_count,
+                                  granted, token_offsets, slot_map, token_seq, token_pos)
+        empty = lambda n: torch.empty(n, dtype=torch.int32, device=self.device)  # noqa: E731
+        self.new_tokens, self.lengths, self.block_table = new_tokens, lengths, block_table
+        self.free_pages, self.free_count = free_pages, free_count
+        self.new_lengths = lengths if new_lengths is None else new_lengths
+        self.new_free_count = free_count if new_free_count is None else new_free_count
+        self.granted = empty(B) if granted is None else granted
+        self.token_offsets = empty(B + 1) if token_offsets is None else token_offsets
+        self.slot_map, self.token_seq, self.token_pos = slot_map, token_seq, token_pos
+        self.params = PageMapParams(B, int(page_size), num_pages, int(block_table.shape[1]), max_tokens,
+                                    *(_ptr(t) for t in (new_tokens, lengths, block_table, free_pages, free_count,
+                                                        self.new_lengths, self.new_free_count, self.granted,
+                                                        self.token_offsets, slot_map, token_seq, token_pos)))
+        nbytes = int(lib().kvq_page_map_workspace_size(ctypes.byref(self.params)))
+        self.ws = _new_workspace(nbytes, self.device, stream)
+        self._args = (ctypes.byref(self.params), _ptr(self.ws), nbytes)
+
+    def __call__(self, stream=None) -> None:
+        """Launch on `stream` (a torch stream or a raw hipStream_t handle; default: torch's current stream)."""
+        _call(lib().kvq_page_map_launch, "kvq_page_map_launch", self._args, self.device, stream)
+
+
+def page_map(new_tokens, lengths, block_table, free_pages, free_count, page_size, stream=None, **outputs) -> PageMapper:
+    """One page map (PageMapper's arguments); returns the PageMapper, whose attributes are the outputs."""
+    m = PageMapper(new_tokens, lengths, block_table, free_pages, free_count, page_size, stream=stream, **outputs)
+    m(stream)
+    return m
+
+
+def _dtype_code(t, name):
+    if t.dtype == torch.float32:
+        return DTYPE_F32
+    if t.dtype == torch.bfloat16:
+        return DTYPE_BF16
+    raise TypeError(f"{name} must be float32 or bfloat16")
+
+
+def slot_write(k_new, v_new, slots, k_pages, v_pages, k_scale_pages, v_scale_pages, stream=None) -> None:
+    """Quantise packed rows into their slots (kvq_slot_write_launch).
+
+    k_new/v_new [T, Hkv, d] fp32 or bf16: a token's heads lie together, tokens may be any stride apart (slices of a
+    fused projection); slots [T] int32, -1 (or any outside the pool) for rows that go nowhere."""
+    P_, Hkv, page, d = _check_cache(k_pages, v_pages, k_scale_pages, v_scale_pages, "pages")
+    T = _rows_of(slots, "slots")
+    code = _dtype_code(k_new, "k_new")
+    strides = []
+    for t, n in ((k_new, "k_new"), (v_new, "v_new")):
+        if t.dtype != k_new.dtype or tuple(t.shape) != (T, Hkv, d) or t.device.type != "cuda":
+            raise ValueError(f"{n}: want cuda {k_new.dtype} {(T, Hkv, d)}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if (d > 1 and t.stride(2) != 1) or (Hkv > 1 and t.stride(1) != d) or (T > 1 and t.stride(0) < Hkv * d):
+            raise ValueError(f"{n}: a token's heads must lie together, got strides {t.stride()}")
+        strides.append(t.stride(0) if T > 1 else 0)
+    device = _one_device(k_new, v_new, slots, k_pages, v_pages, k_scale_pages, v_scale_pages)
+    if T == 0:
+        return
+    p = SlotWriteParams(T, Hkv, d, page, P_, code, _ptr(k_new), _ptr(v_new), *strides, _ptr(slots), _ptr(k_pages),
+                        _ptr(v_pages), _ptr(k_scale_pages), _ptr(v_scale_pages))
+    _call(lib().kvq_slot_write_launch, "kvq_slot_write_launch", (ctypes.byref(p),), device, stream)
+
+
+def slot_read(slots, k_pages, v_pages, k_scale_pages, v_scale_pages, k_out, v_out, stream=None):
+    """Cached rows as numbers (kvq_slot_read_launch): slots [T] int32 into k_out/v_out [T, Hkv, d] fp32 or bf16, each of
+    the same strides (a transposed [Hkv, T, d] too); returns (k_out, v_out)."""
+    P_, Hkv, page, d = _check_cache(k_pages, v_pages, k_scale_pages, v_scale_pages, "pages")
+    T = _rows_of(slots, "slots")
+    code = _dtype_code(k_out, "k_out")
+    for t, n in ((k_out, "k_out"), (v_out, "v_out")):
+        if t.dtype != k_out.dtype or tuple(t.shape) != (T, Hkv, d) or t.device.type != "cuda":
+            raise ValueError(f"{n}: want cuda {k_out.dtype} {(T, Hkv, d)}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if (d > 1 and t.stride(2) != 1) or t.stride()[:2] != k_out.stride()[:2]:
+            raise ValueError(f"{n}: rows must be contiguous and both outputs alike, got strides {t.stride()}")
+    device = _one_device(slots, k_pages, v_pages, k_scale_pages, v_scale_pages, k_out, v_out)
+    if T == 0:
+        return k_out, v_out
+    p = SlotReadParams(T, Hkv, d, page, P_, code, _ptr(slots), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale_pages),
+                       _ptr(v_scale_pages), _ptr(k_out), _ptr(v_out), k_out.stride(0), k_out.stride(1))
+    _call(lib().kvq_slot_read_launch, "kvq_slot_read_launch", (ctypes.byref(p),), device, stream)
+    return k_out, v_out
+
+
+def new_bounds(k_pages):
+    """(bounds, bound_scale) for a page pool, of empty pages."""
+    P_, Hkv, _, d = k_pages.shape
+    return (torch.zeros((P_, Hkv, 2, d), dtype=torch.int8, device=k_pages.device),
+            torch.zeros((P_, Hkv), dtype=torch.float32, device=k_pages.device))
+
+
+def _check_bounds(bounds, bound_scale, P_, Hkv, d):
+    _need(bounds, torch.int8, (P_, Hkv, 2, d), "bounds")
+    _need(bound_scale, torch.float32, (P_, Hkv), "bound_scale")
+
+
+def page_bounds(k_pages, k_scale_pages, block_table, lengths, bounds, bound_scale, start=None, max_seq_len=0,
+                stream=None) -> None:
+    """Key bounds of the pages that hold tokens [start_b, lengths_b) (kvq_page_bounds_launch).
+
+    bounds [num_pages, Hkv, 2, d] int8, bound_scale [num_pages, Hkv] fp32 (new_bounds); start [B] int32 or None."""
+    P_, Hkv, page, d = k_pages.shape
+    _need(k_pages, torch.int8, (P_, Hkv, page, d), "k_pages")
+    _need(k_scale_pages, torch.float32, (P_, Hkv, page), "k_scale_pages")
+    _check_bounds(bounds, bound_scale, P_, Hkv, d)
+    if block_table.dim() != 2:
+        raise ValueError("block_table: want [B, max_pages_per_seq]")
+    B = block_table.shape[0]
+    _need(block_table, torch.int32, tuple(block_table.shape), "block_table")
+    for t, n in ((start, "start"), (lengths, "lengths")):
+        if t is not None:
+            _rows_of(t, n, B)
+    device = _one_device(k_pages, k_scale_pages, block_table, lengths, bounds, bound_scale, start)
+    p = PageBoundsParams(B, Hkv, d, page, P_, int(block_table.shape[1]), int(max_seq_len), _ptr(block_table),
+                         _ptr(start), _ptr(lengths), _ptr(k_pages), _ptr(k_scale_pages), _ptr(bounds),
+                         _ptr(bound_scale))
+    _call(lib().kvq_page_bounds_launch, "kvq_page_bounds_launch", (ctypes.byref(p),), device, stream)
+
+
+class SparseDecoder:
+    """Decode over the pages that rank highest (kvq_sparse_decode_launch), with its own workspace.
+
+    The arguments of PagedDecoder; bounds and bound_scale as page_bounds writes them; selected [B, Hkv, max_selected]
+    and selected_lengths [B, Hkv], both int32, receive the pages attended and the tokens in them."""
+
+    def __init__(self, q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, lengths, bounds, bound_scale, out,
+                 selected, selected_lengths, max_seq_len=0, keep_first=1, keep_last=1, softmax_scale=0.0, num_splits=0,
+                 k_new=None, v_new=None, stream=None):
+        check_paged(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, lengths, out, k_new, v_new)
+        B, Hq, d = q.shape
+        P_, Hkv, page, _ = k_pages.shape
+        _check_bounds(bounds, bound_scale, P_, Hkv, d)
+        if selected.dim() != 3:
+            raise ValueError("selected: want [B, Hkv, max_selected]")
+        _need(selected, torch.int32, (B, Hkv, selected.shape[2]), "selected")
+        _need(selected_lengths, torch.int32, (B, Hkv), "selected_lengths")
+        self.keep = (q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, lengths, bounds, bound_scale, out,
+                     selected, selected_lengths, k_new, v_new)
+        self.device = _one_device(*self.keep)
+        step = PagedDecodeParams(B, Hq, Hkv, d, page, P_, int(block_table.shape[1]), int(max_seq_len),
+                                 _ptr(block_table), _ptr(lengths), _ptr(q), _ptr(k_pages), _ptr(v_pages),
+                                 _ptr(k_scale_pages), _ptr(v_scale_pages), _ptr(out), float(softmax_scale),
+                                 int(num_splits), _ptr(k_new), _ptr(v_new))
+        self.params = SparseDecodeParams(step, int(selected.shape[2]), int(keep_first), int(keep_last), _ptr(bounds),
+                                         _ptr(bound_scale), _ptr(selected), _ptr(selected_lengths))
+        self.ws_bytes = int(lib().kvq_sparse_decode_workspace_size(ctypes.byref(self.params)))
+        self.ws = _new_workspace(self.ws_bytes, self.device, stream)
+        self._args = (ctypes.byref(self.params), _ptr(self.ws), self.ws_bytes)
+
+    def __call__(self, stream=None) -> None:
+        _call(lib().kvq_sparse_decode_launch, "kvq_sparse_decode_launch", self._args, self.device, stream)
+
+
+def sparse_decode_plan(p: SparseDecodeParams) -> PlanInfo:
+    """Plan of kvq_sparse_decode_launch's attention for p (host-only)."""
+    info = PlanInfo()
+    _check("kvq_sparse_decode_plan", lib().kvq_sparse_decode_plan(ctypes.byref(p), ctypes.byref(info)))
+    return info
+
+
 def _attention_shapes(q, k, v, out):
     M, d = q.shape
     N = k.shape[0]
@@ -624,4 +927,6 @@ __all__ = ["lib", "version", "solve", "kv_int8_split_launch", "DecodeParams", "A
            "PagedAppendParams", "PagedDecoder", "paged_append", "PrefillParams", "prefill", "DTYPE_F32",
            "DTYPE_BF16", "AttentionParams", "attention_online", "attention_params", "attention_workspace_size",
            "attention", "PlanInfo", "reference_plan", "decode_plan", "paged_decode_plan", "attention_plan", "diagnostics",
-           "attention_lib", "attention_solve", "decode_launch_noalloc", "NOALLOC_SCRATCH_BYTES"]
+           "attention_lib", "attention_solve", "decode_launch_noalloc", "NOALLOC_SCRATCH_BYTES", "PAGE_MAP_MAX_BATCH",
+           "PageMapParams", "SlotWriteParams", "SlotReadParams", "PageBoundsParams", "SparseDecodeParams", "PageMapper",
+           "page_map", "slot_write", "slot_read", "new_bounds", "page_bounds", "SparseDecoder", "sparse_decode_plan"]

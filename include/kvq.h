@@ -378,6 +378,167 @@ hipError_t kvq_attention_plan(const kvq_attention_params* p, kvq_plan_info* info
  *        kernel), 2 = "generic" (decode plans avoid both tuned kernels). */
 int kvq_diagnostics(void);
 
+/* ============ Part 7: a paged cache's life on the GPU (no counterpart in the reference) ============
+ *
+ * What a serving loop does around paged decode, without host round trips:
+ *   kvq_page_map_launch       block tables, free pages and slots from request lengths
+ *   kvq_slot_write_launch     a packed (ragged) batch of K/V rows quantised into its slots
+ *   kvq_slot_read_launch      cached tokens as fp32 or bf16 rows
+ *   kvq_page_bounds_launch    int8 bounds of each page's keys
+ *   kvq_sparse_decode_launch  a decode step over the pages that the bounds rank highest
+ * A slot is a token's place in the pool: page id * page_size + its place in the
+ * page; pool layouts and block tables are those of part 3.  Every entry point
+ * returns hipErrorInvalidValue before any HIP call on a bad argument, is
+ * asynchronous on `stream`, allocates nothing and can be captured. */
+
+/* Most sequences of one page map. */
+#define KVQ_PAGE_MAP_MAX_BATCH 4096
+
+typedef struct kvq_page_map_params {
+    int batch;               /* B in [1, KVQ_PAGE_MAP_MAX_BATCH] */
+    int page_size;           /* tokens per page, >= 1 */
+    int num_pages;           /* pages in the pool; num_pages * page_size <= INT_MAX */
+    int max_pages_per_seq;   /* row stride of block_table; a sequence holds at most
+                                max_pages_per_seq * page_size tokens */
+    int max_tokens;          /* T >= 0: rows of the packed batch */
+    const int32_t* new_tokens; /* device [B]: tokens to add; negative: to take off the end */
+    const int32_t* lengths;  /* device [B]: tokens held, each clamped to [0, capacity] */
+    int32_t* block_table;    /* device [B, max_pages_per_seq], updated in place */
+    int32_t* free_pages;     /* device [num_pages]: the free stack, updated in place */
+    const int32_t* free_count; /* device [1]: its entries, clamped to [0, num_pages] */
+    int32_t* new_lengths;    /* device [B]; may be `lengths` */
+    int32_t* new_free_count; /* device [1]; may be `free_count` */
+    int32_t* granted;        /* device [B]: tokens added (taken off: negative; refused: 0) */
+    int32_t* token_offsets;  /* device [B + 1]: first packed row of each sequence, then the rows' number */
+    int32_t* slot_map;       /* device [T]: slot of each packed row, or NULL */
+    int32_t* token_seq;      /* device [T]: its sequence, or NULL */
+    int32_t* token_pos;      /* device [T]: its position in the sequence, or NULL */
+} kvq_page_map_params;
+
+/* Grows and shrinks the sequences of a paged cache.
+ * - Sequence b asks for max(new_tokens[b], 0) packed rows, which follow those of
+ *   the sequences before it; offsets saturate at max_tokens.
+ * - A request is granted whole or refused whole (length, table and pages stay).
+ *   It is refused when it does not fit block_table's row or the packed rows;
+ *   and, if it needs a page, when the pages that it and the sequences before it
+ *   need (those refused for want of pages among them) are more than there are.
+ * - Sequences that shrink give up the pages behind their new end first: these go
+ *   onto the free stack in the order (sequence, page), so the same call can hand
+ *   them out.  The i-th page that growing sequences take, in that order, is the
+ *   i-th from the stack's top.  Entries behind the end of the stack, and table
+ *   entries behind a sequence's last page, have no meaning and are left as they
+ *   were.
+ * - slot_map, token_seq and token_pos are wholly written: a refused request's
+ *   rows have slot -1; rows behind the last have -1 in all three.  A row whose
+ *   page id lies outside the pool has slot -1.
+ * - Pages belong to one sequence; a page in two tables is given up twice.
+ * Workspace: kvq_page_map_workspace_size bytes (0 for small batches), zero-filled
+ * once (kvq_workspace_init) and left zeroed.  Calls on one pool must be ordered. */
+size_t kvq_page_map_workspace_size(const kvq_page_map_params* p);
+hipError_t kvq_page_map_launch(const kvq_page_map_params* p, void* workspace, size_t workspace_bytes,
+                               hipStream_t stream);
+
+typedef struct kvq_slot_write_params {
+    int tokens;               /* T >= 0 packed rows; T * num_kv_heads < 2^31 */
+    int num_kv_heads, head_dim;
+    int page_size, num_pages; /* num_pages * page_size <= INT_MAX */
+    int dtype;                /* KVQ_DTYPE_F32 or KVQ_DTYPE_BF16 */
+    const void* k_new;        /* [T, Hkv, d]: a token's heads lie together */
+    const void* v_new;
+    int64_t k_stride;         /* elements from a token to the next, >= Hkv * d (0: Hkv * d) */
+    int64_t v_stride;
+    const int32_t* slots;     /* device [T]; a slot outside the pool skips its row */
+    int8_t* k_pages;          /* [num_pages, Hkv, page_size, d] */
+    int8_t* v_pages;
+    float* k_scale_pages;     /* [num_pages, Hkv, page_size] */
+    float* v_scale_pages;
+} kvq_slot_write_params;
+
+/* The quantiser of kvq_append_launch (same bits) over a packed batch.  Slots
+ * must be distinct: a slot that is named twice holds some mixture of its rows. */
+hipError_t kvq_slot_write_launch(const kvq_slot_write_params* p, hipStream_t stream);
+
+typedef struct kvq_slot_read_params {
+    int tokens;               /* T >= 0; T * num_kv_heads < 2^31 */
+    int num_kv_heads, head_dim;
+    int page_size, num_pages; /* num_pages * page_size <= INT_MAX */
+    int dtype;                /* of the outputs: KVQ_DTYPE_F32 or KVQ_DTYPE_BF16 */
+    const int32_t* slots;     /* device [T], in any order and number */
+    const int8_t* k_pages;    /* [num_pages, Hkv, page_size, d] */
+    const int8_t* v_pages;
+    const float* k_scale_pages;
+    const float* v_scale_pages;
+    void* k_out;              /* row (t, h) at t * token_stride + h * head_stride, wholly written */
+    void* v_out;
+    int64_t token_stride;     /* elements, for both outputs; [T, Hkv, d]: Hkv * d, d; */
+    int64_t head_stride;      /* [Hkv, T, d]: d, T * d.  Rows must not overlap */
+} kvq_slot_read_params;
+
+/* Cached rows as numbers: code * scale in fp32, rounded to nearest even for
+ * bf16; a slot outside the pool gives a zero row. */
+hipError_t kvq_slot_read_launch(const kvq_slot_read_params* p, hipStream_t stream);
+
+typedef struct kvq_page_bounds_params {
+    int batch, num_kv_heads, head_dim;
+    int page_size, num_pages, max_pages_per_seq;
+    int max_seq_len;            /* as kvq_paged_decode_params */
+    const int32_t* block_table; /* device [B, max_pages_per_seq] */
+    const int32_t* start;       /* device [B]: first token whose page is to be done (clamped at 0), or NULL: 0 */
+    const int32_t* lengths;     /* device [B] or NULL; clamped on device to [0, max_seq_len] */
+    const int8_t* k_pages;      /* [num_pages, Hkv, page_size, d] */
+    const float* k_scale_pages; /* [num_pages, Hkv, page_size] */
+    int8_t* bounds;             /* [num_pages, Hkv, 2, d]: highs, then lows */
+    float* bound_scale;         /* [num_pages, Hkv] */
+} kvq_page_bounds_params;
+
+/* Bounds of the keys of every page that holds a token in [start_b, length_b),
+ * over its tokens below length_b: with s_t the tokens' scales and k_t their
+ * codes, S = max |s_t|, highs ceil(max_t k_t r_t) and lows floor(min_t k_t r_t)
+ * per dim for r_t = s_t / S (quotient and product rounded in fp32), so every key
+ * lies in S * [low, high] but for those roundings.  S = 0: bounds 0.  S not
+ * finite: bounds 127 and -127 under the scale +inf, which rank first. */
+hipError_t kvq_page_bounds_launch(const kvq_page_bounds_params* p, hipStream_t stream);
+
+typedef struct kvq_sparse_decode_params {
+    kvq_paged_decode_params decode; /* the dense step: attends to at most max_selected pages of it */
+    int max_selected;         /* pages per (sequence, kv head), >= keep_first + keep_last */
+    int keep_first;           /* leading pages attended whatever their score, >= 0 */
+    int keep_last;            /* trailing pages, >= 1 */
+    int8_t* bounds;           /* [num_pages, Hkv, 2, d], as kvq_page_bounds_launch writes them */
+    float* bound_scale;       /* [num_pages, Hkv] */
+    int32_t* selected;        /* [B, Hkv, max_selected] out: page id * Hkv + kv head of the pages attended,
+                                 ascending in the sequence, then -1 */
+    int32_t* selected_lengths;/* [B, Hkv] out: tokens in them */
+} kvq_sparse_decode_params;
+
+/* Decode attention over the pages of each sequence that rank highest for the
+ * query, per kv head.  A sequence of at most max_selected pages is attended
+ * whole (as kvq_paged_decode_launch does).  Of a longer one, keep_first leading
+ * and keep_last trailing pages, and of the others those with the highest scores,
+ * equal ones in page order.
+ * Score of a page, for the G query heads of a kv head: the heads' q are quantised
+ * with one scale (max |q| over all of them / 127, the rule of kvq_append_launch);
+ * score = float(max over heads of sum_i max(q_i high_i, q_i low_i)) * bound_scale,
+ * an exact integer with two fp32 roundings, so every implementation ranks alike.
+ * A NaN score ranks first.
+ * Bounds: of every page but the last keep_last they must be current.  When the
+ * step's token opens a page (length_b - 1 is a multiple of page_size), the page
+ * before it has become whole and its bounds are written by this call; so decode
+ * steps of one token keep them current, while tokens written otherwise need
+ * kvq_page_bounds_launch.
+ * `selected` is a block table of the pool seen as num_pages * Hkv pages of one kv
+ * head ([num_pages * Hkv, 1, page_size, d]), for batch * Hkv sequences of
+ * selected_lengths tokens.
+ * Workspace as for kvq_paged_decode_launch: kvq_sparse_decode_workspace_size
+ * bytes, zero-filled once, left ready by every completed launch.  num_pages * Hkv
+ * and B * Hkv * max_selected must fit an int. */
+size_t kvq_sparse_decode_workspace_size(const kvq_sparse_decode_params* p);
+hipError_t kvq_sparse_decode_launch(const kvq_sparse_decode_params* p, void* workspace, size_t workspace_bytes,
+                                    hipStream_t stream);
+/* The plan of the attention over the selected pages; workspace_bytes is the
+ * whole call's.  Host-only (as part 6). */
+hipError_t kvq_sparse_decode_plan(const kvq_sparse_decode_params* p, kvq_plan_info* info);
+
 #ifdef __cplusplus
 }
 #endif

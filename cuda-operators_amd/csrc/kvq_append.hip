@@ -63,20 +63,6 @@ __device__ __forceinline__ float load_elem(const void* row, int e) {
     else return static_cast<const float*>(row)[e];
 }
 
-// Max over aligned groups of N lanes (N a power of two <= 64) of the lanes'
-// |x| maxima (non-negative; fmaxf drops NaN elements, so never NaN).
-template <int N>
-__device__ __forceinline__ float lanes_max(float x) {
-    if constexpr (N <= 16) {
-        return group_max_nonneg<N>(x);
-    } else {
-        x = group_max_nonneg<16>(x);
-        x = fmaxf(x, __shfl_xor(x, 16));
-        if constexpr (N == 64) x = fmaxf(x, __shfl_xor(x, 32));
-        return x;
-    }
-}
-
 // Tuned path: LPR lanes read one row with a 16-byte load each (fp32: 4
 // elements, bf16: 8), so one wave load covers 64 / LPR whole rows; U wave
 // loads are in flight per lane (fp32: 8, bf16: 4).  Each lane packs its

@@ -174,6 +174,20 @@ __device__ __forceinline__ int buffer_load4(buf_rsrc r, int voff, int soff) {
 // v_exp_f32: 2^x, exp2(-inf) == 0.
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Max over aligned groups of N lanes (N a power of two <= 64) of the lanes'
+// |x| maxima (non-negative; fmaxf drops NaN elements, so never NaN).
+template <int N>
+__device__ __forceinline__ float lanes_max(float x) {
+    if constexpr (N <= 16) {
+        return group_max_nonneg<N>(x);
+    } else {
+        x = group_max_nonneg<16>(x);
+        x = fmaxf(x, __shfl_xor(x, 16));
+        if constexpr (N == 64) x = fmaxf(x, __shfl_xor(x, 32));
+        return x;
+    }
+}
+
 // fp32 to bf16, to nearest even (v_cvt_pk_bf16_f32).
 __device__ __forceinline__ uint16_t bf16_of(float x) {
     return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));

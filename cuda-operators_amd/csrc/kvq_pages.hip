@@ -230,6 +230,132 @@ __device__ __forceinline__ float row_elem(const void* x, int64_t i) {
     else return static_cast<const float*>(x)[i];
 }
 
+// Tuned rows: LPR lanes a row with 16 bytes of it each (fp32: 4 elements, bf16:
+// 8), U loads in flight a lane.  A wave takes U * RPW consecutive tokens of one
+// kv head: in the pool these are as a rule consecutive rows of a page, so its
+// codes and scales go out (or come in) in whole cache lines, while neighbouring
+// waves take the other heads of the same tokens, whose packed rows lie beside.
+// PAD: a row of d < D elements, whole 16-byte pieces; the lanes past its last
+// piece read that piece again and store nothing.
+template <int D, bool BF16>
+struct SlotGeom {
+    static constexpr int EPL = BF16 ? 8 : 4;  // elements a lane
+    static constexpr int LPR = D / EPL;       // lanes a row
+    static constexpr int RPW = kWave / LPR;   // rows a wave load
+    static constexpr int U = BF16 ? 4 : 8;
+    static constexpr int TB = RPW * U;        // tokens a wave
+    static_assert(LPR >= 1 && LPR <= kWave && kWave % LPR == 0, "row geometry");
+};
+
+// The wave's unit (token block, head): false past the last one.
+__device__ __forceinline__ bool slot_unit(const SlotArgs& a, int tb, int& t0, int& h) {
+    const unsigned unit = blockIdx.x * kSlotWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const unsigned blk = fastdiv(unit, a.heads);
+    h = static_cast<int>(unit - blk * a.Hkv);
+    const long long first = static_cast<long long>(blk) * tb;
+    t0 = static_cast<int>(first);
+    return first < a.T;
+}
+
+template <int D, bool BF16, bool PAD>
+__global__ __launch_bounds__(kSlotWaves* kWave) void slot_write_kernel(const SlotArgs a) {
+    using Geo = SlotGeom<D, BF16>;
+    constexpr int EPL = Geo::EPL, LPR = Geo::LPR, RPW = Geo::RPW, U = Geo::U;
+    int t0, h;
+    if (!slot_unit(a, Geo::TB, t0, h)) return;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int d = PAD ? a.d : D;
+    const int ls = PAD ? min(lane % LPR, d / EPL - 1) : lane % LPR;  // 16-byte piece of the row
+    const bool owner = !PAD || ls == lane % LPR;
+    const int kv = blockIdx.y;
+    const int64_t stride = kv ? a.v_stride : a.k_stride;
+    const char* x = static_cast<const char*>(kv ? a.v_rows : a.k_rows) +
+                    (static_cast<int64_t>(h) * a.head_stride + ls * EPL) * (BF16 ? 2 : 4);
+    int8_t* qo = kv ? a.v : a.k;
+    float* so = kv ? a.vs : a.ks;
+    int4 raw[U];
+    long long orow[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {  // a token past the end reads the last one again and is dropped
+        const int tc = min(t0 + u * RPW + lane / LPR, a.T - 1);
+        raw[u] = *reinterpret_cast<const int4*>(x + tc * stride * (BF16 ? 2 : 4));
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int t = t0 + u * RPW + lane / LPR;
+        orow[u] = slot_row(a, min(t, a.T - 1), h);
+        if (t >= a.T) orow[u] = -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        float e[EPL];
+        const int w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+        float am = 0.0f;
+#pragma unroll
+        for (int i = 0; i < EPL; i++) {
+            if constexpr (BF16) e[i] = __uint_as_float((i & 1) ? (static_cast<unsigned>(w[i >> 1]) & 0xffff0000u)
+                                                             : (static_cast<unsigned>(w[i >> 1]) << 16));
+            else e[i] = __int_as_float(w[i]);
+            am = fmaxf(am, fabsf(e[i]));
+        }
+        const float scale = quant_scale(lanes_max<LPR>(am));
+        if (orow[u] < 0 || !owner) continue;
+        int qv[EPL];
+        quant_row<EPL>(e, scale, qv);
+        int8_t* o = qo + orow[u] * d + ls * EPL;
+        if constexpr (BF16)
+            *reinterpret_cast<int2*>(o) = make_int2(pack4(qv[0], qv[1], qv[2], qv[3]), pack4(qv[4], qv[5], qv[6], qv[7]));
+        else *reinterpret_cast<int*>(o) = pack4(qv[0], qv[1], qv[2], qv[3]);
+        if (ls == 0) so[orow[u]] = scale;
+    }
+}
+
+template <int D, bool BF16, bool PAD>
+__global__ __launch_bounds__(kSlotWaves* kWave) void slot_read_kernel(const SlotArgs a) {
+    using Geo = SlotGeom<D, BF16>;
+    constexpr int EPL = Geo::EPL, LPR = Geo::LPR, RPW = Geo::RPW, U = Geo::U;
+    int t0, h;
+    if (!slot_unit(a, Geo::TB, t0, h)) return;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int d = PAD ? a.d : D;
+    const int ls = PAD ? min(lane % LPR, d / EPL - 1) : lane % LPR;
+    const bool owner = !PAD || ls == lane % LPR;
+    const int kv = blockIdx.y;
+    const int64_t stride = kv ? a.v_stride : a.k_stride;
+    char* x = static_cast<char*>(kv ? a.v_rows : a.k_rows) +
+              (static_cast<int64_t>(h) * a.head_stride + ls * EPL) * (BF16 ? 2 : 4);
+    const int8_t* qi = kv ? a.v : a.k;
+    const float* si = kv ? a.vs : a.ks;
+    long long irow[U];
+    int2 raw[U];
+    float scale[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) irow[u] = slot_row(a, min(t0 + u * RPW + lane / LPR, a.T - 1), h);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const long long r = max(irow[u], 0LL);  // a row that is nowhere reads the pool's first and gives zeros
+        const int8_t* p = qi + r * d + ls * EPL;
+        if constexpr (BF16) raw[u] = *reinterpret_cast<const int2*>(p);
+        else raw[u] = make_int2(*reinterpret_cast<const int*>(p), 0);
+        scale[u] = si[r];
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int t = t0 + u * RPW + lane / LPR;
+        if (t >= a.T || !owner) continue;
+        float y[EPL];
+#pragma unroll
+        for (int i = 0; i < EPL; i++) y[i] = irow[u] < 0 ? 0.0f : sbyte(i < 4 ? raw[u].x : raw[u].y, i & 3) * scale[u];
+        v4i_t out;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (BF16) out[i] = static_cast<int>(bf16_of(y[2 * i]) | (static_cast<unsigned>(bf16_of(y[2 * i + 1])) << 16));
+            else out[i] = __float_as_int(y[i]);
+        }
+        *reinterpret_cast<v4i_t*>(x + t * stride * (BF16 ? 2 : 4)) = out;
+    }
+}
+
 // Any head dim, stride or alignment: a wave a row, an element a load.
 template <bool BF16>
 __global__ __launch_bounds__(kSlotWaves* kWave) void slot_write_generic(const SlotArgs a) {
@@ -285,24 +411,50 @@ __global__ __launch_bounds__(kSlotWaves* kWave) void slot_read_generic(const Slo
 // ---------------------------------------------------------------------------
 constexpr int kBoundsWaves = 4;
 
+// Pages that sequence b asks for: [p0, p0 + n), and its length.
+struct PageRange {
+    int len, p0, n;
+};
+__device__ __forceinline__ PageRange bounds_range(const BoundsArgs& a, int b) {
+    PageRange r;
+    r.len = a.lengths ? min(max(a.lengths[b], 0), a.max_len) : a.max_len;
+    const int first = a.start ? max(a.start[b], 0) : 0;
+    r.p0 = first / a.pages.size;
+    r.n = first < r.len ? (r.len - 1) / a.pages.size + 1 - r.p0 : 0;
+    return r;
+}
+
+// Tuned head dims: a wave takes 64 / (LPT * groups) (page, kv head) units, the
+// heads of a page one after the other as they lie in the pool.
+template <int LPT>
+__global__ __launch_bounds__(kBoundsWaves* kWave) void page_bounds_kernel(const BoundsArgs a, int groups) {
+    const int b = blockIdx.x;
+    const PageRange r = bounds_range(a, b);
+    const long long units = static_cast<long long>(r.n) * a.Hkv;
+    const int per = kWave / (LPT * groups);
+    const int mine = (threadIdx.x & (kWave - 1)) / (LPT * groups);
+    for (long long u0 = (static_cast<long long>(blockIdx.y) * kBoundsWaves + threadIdx.x / kWave) * per; u0 < units;
+         u0 += static_cast<long long>(gridDim.y) * kBoundsWaves * per) {
+        const bool live = u0 + mine < units;
+        const long long u = live ? u0 + mine : u0;
+        const int pi = r.p0 + static_cast<int>(u / a.Hkv);
+        const int h = static_cast<int>(u % a.Hkv);
+        bounds_wave<LPT>(a, groups, live, b, pi, h, min(a.pages.size, r.len - pi * a.pages.size));
+    }
+}
+
 // Any head dim, page size or alignment: a wave a (page, kv head), workgroups
 // blockIdx.y of sequence blockIdx.x striding over its pages.
 __global__ __launch_bounds__(kBoundsWaves* kWave) void page_bounds_generic(const BoundsArgs a) {
     const int lane = threadIdx.x & (kWave - 1);
     const int b = blockIdx.x;
-    const int len = a.lengths ? min(max(a.lengths[b], 0), a.max_len) : a.max_len;
-    const int first = a.start ? max(a.start[b], 0) : 0;
-    if (first >= len) return;
-    const int size = a.pages.size;
-    const int p0 = first / size;
-    const int pages = (len - 1) / size + 1 - p0;
-    const long long units = static_cast<long long>(pages) * a.Hkv;
+    const PageRange r = bounds_range(a, b);
+    const long long units = static_cast<long long>(r.n) * a.Hkv;
     for (long long u = static_cast<long long>(blockIdx.y) * kBoundsWaves + threadIdx.x / kWave; u < units;
          u += static_cast<long long>(gridDim.y) * kBoundsWaves) {
-        const int pi = p0 + static_cast<int>(u / a.Hkv);
+        const int pi = r.p0 + static_cast<int>(u / a.Hkv);
         const int h = static_cast<int>(u % a.Hkv);
-        const int tokens = min(size, len - pi * size);
-        bounds_generic(a, b, pi, h, tokens, lane);
+        bounds_generic(a, b, pi, h, min(a.pages.size, r.len - pi * a.pages.size), lane);
     }
 }
 
@@ -323,28 +475,58 @@ dim3 slot_grid(unsigned rows, unsigned rows_per_group) {
 }
 }  // namespace
 
-hipError_t launch_slot_write(const SlotArgs& a, bool bf16, bool, hipStream_t stream) {
+namespace {
+template <bool BF16>
+hipError_t launch_slots(const SlotArgs& a, bool write, bool vec_ok, hipStream_t stream) {
     if (a.T == 0) return hipSuccess;
-    const dim3 grid = slot_grid(static_cast<unsigned>(a.T) * a.Hkv, kSlotWaves), block(kSlotWaves * kWave);
-    if (bf16) hipLaunchKernelGGL((slot_write_generic<true>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((slot_write_generic<false>), grid, block, 0, stream, a);
+    const dim3 block(kSlotWaves * kWave);
+    // Rows of whole 16-byte pieces up to 256 elements; others, and misaligned
+    // ones, go to the generic kernels.
+    if (vec_ok && a.d <= 256 && a.d % SlotGeom<256, BF16>::EPL == 0) {
+#define KVQ_SLOT_CASE(DD)                                                                                        \
+    if (a.d <= DD) {                                                                                             \
+        const long long units = (static_cast<long long>(a.T) + SlotGeom<DD, BF16>::TB - 1) / SlotGeom<DD, BF16>::TB * a.Hkv; \
+        const dim3 grid(static_cast<unsigned>((units + kSlotWaves - 1) / kSlotWaves), 2);                        \
+        if (write && a.d == DD) hipLaunchKernelGGL((slot_write_kernel<DD, BF16, false>), grid, block, 0, stream, a); \
+        else if (write) hipLaunchKernelGGL((slot_write_kernel<DD, BF16, true>), grid, block, 0, stream, a);      \
+        else if (a.d == DD) hipLaunchKernelGGL((slot_read_kernel<DD, BF16, false>), grid, block, 0, stream, a);  \
+        else hipLaunchKernelGGL((slot_read_kernel<DD, BF16, true>), grid, block, 0, stream, a);                  \
+        return hipGetLastError();                                                                                \
+    }
+        KVQ_SLOT_CASE(32)
+        KVQ_SLOT_CASE(64)
+        KVQ_SLOT_CASE(128)
+        KVQ_SLOT_CASE(256)
+#undef KVQ_SLOT_CASE
+    }
+    const dim3 grid = slot_grid(static_cast<unsigned>(a.T) * a.Hkv, kSlotWaves);
+    if (write) hipLaunchKernelGGL((slot_write_generic<BF16>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((slot_read_generic<BF16>), grid, block, 0, stream, a);
     return hipGetLastError();
 }
+}  // namespace
 
-hipError_t launch_slot_read(const SlotArgs& a, bool bf16, bool, hipStream_t stream) {
-    if (a.T == 0) return hipSuccess;
-    const dim3 grid = slot_grid(static_cast<unsigned>(a.T) * a.Hkv, kSlotWaves), block(kSlotWaves * kWave);
-    if (bf16) hipLaunchKernelGGL((slot_read_generic<true>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((slot_read_generic<false>), grid, block, 0, stream, a);
-    return hipGetLastError();
+hipError_t launch_slot_write(const SlotArgs& a, bool bf16, bool vec_ok, hipStream_t stream) {
+    return bf16 ? launch_slots<true>(a, true, vec_ok, stream) : launch_slots<false>(a, true, vec_ok, stream);
+}
+hipError_t launch_slot_read(const SlotArgs& a, bool bf16, bool vec_ok, hipStream_t stream) {
+    return bf16 ? launch_slots<true>(a, false, vec_ok, stream) : launch_slots<false>(a, false, vec_ok, stream);
 }
 
-hipError_t launch_page_bounds(const BoundsArgs& a, bool, hipStream_t stream) {
+hipError_t launch_page_bounds(const BoundsArgs& a, bool vec_ok, hipStream_t stream) {
+    const bool tuned = vec_ok && a.d <= 256 && a.d % 16 == 0;
+    const int lanes = bounds_lanes(a.d);
+    const int groups = bounds_groups(a.pages.size, lanes);
     // About 8192 workgroups at most; a sequence's workgroups stride over its pages.
     const long long units = (static_cast<long long>(a.max_len - 1) / a.pages.size + 1) * a.Hkv;
-    const long long want = (units + kBoundsWaves - 1) / kBoundsWaves;
-    const unsigned ny = static_cast<unsigned>(min(want, max(1LL, 8192LL / a.B)));
-    hipLaunchKernelGGL(page_bounds_generic, dim3(static_cast<unsigned>(a.B), ny), dim3(kBoundsWaves * kWave), 0, stream, a);
+    const int per = tuned ? kBoundsWaves * (kWave / (lanes * groups)) : kBoundsWaves;
+    const unsigned ny = static_cast<unsigned>(min((units + per - 1) / per, max(1LL, 8192LL / a.B)));
+    const dim3 grid(static_cast<unsigned>(a.B), ny), block(kBoundsWaves * kWave);
+    if (!tuned) hipLaunchKernelGGL(page_bounds_generic, grid, block, 0, stream, a);
+    else if (lanes == 2) hipLaunchKernelGGL(page_bounds_kernel<2>, grid, block, 0, stream, a, groups);
+    else if (lanes == 4) hipLaunchKernelGGL(page_bounds_kernel<4>, grid, block, 0, stream, a, groups);
+    else if (lanes == 8) hipLaunchKernelGGL(page_bounds_kernel<8>, grid, block, 0, stream, a, groups);
+    else hipLaunchKernelGGL(page_bounds_kernel<16>, grid, block, 0, stream, a, groups);
     return hipGetLastError();
 }
 

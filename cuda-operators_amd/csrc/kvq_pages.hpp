@@ -70,11 +70,14 @@ struct SelectArgs {
     int splits;      // workgroups per (sequence, kv head)
 };
 struct SelectPlan {
-    int splits, key_stride;
+    int splits;
+    int lds_keys;  // ranks a workgroup keeps in LDS, 0: none
+    int key_stride;
     size_t key_bytes;
 };
 // Workgroups per unit and where the ranks go, for sequences of up to max_pages pages.
-SelectPlan select_plan(int units, int max_pages, int max_selected);
-hipError_t launch_select(const SelectArgs& a, bool vec_ok, hipStream_t stream);
+// vec_ok: 16-byte aligned q, keys and bounds.
+SelectPlan select_plan(int units, int G, int d, bool vec_ok, int max_pages, int max_selected);
+hipError_t launch_select(const SelectArgs& a, const SelectPlan& p, bool vec_ok, hipStream_t stream);
 
 }  // namespace kvq

@@ -75,6 +75,7 @@ size_t map_bytes(const kvq::PageMapArgs& a) { return kvq::page_map_groups(a) > 1
 struct SparsePlan {
     kvq_paged_decode_params step;  // the attention: one sequence per (sequence, kv head) over `selected`
     kvq::SelectPlan select;
+    bool vec_ok;
     size_t step_bytes, keys_at, bytes;
 };
 
@@ -110,7 +111,8 @@ SparsePlan sparse_plan(const kvq_sparse_decode_params* p) {
     s.block_table = p->selected;
     s.lengths = p->selected_lengths;
     r.step_bytes = kvq_paged_decode_workspace_size(&s);
-    r.select = kvq::select_plan(s.batch, (max_len - 1) / s.page_size + 1, p->max_selected);
+    r.vec_ok = ((bits(s.k_pages) | bits(p->bounds) | bits(s.q)) & 15u) == 0;
+    r.select = kvq::select_plan(s.batch, s.num_q_heads, s.head_dim, r.vec_ok, (max_len - 1) / s.page_size + 1, p->max_selected);
     // The selection's arrival counters share the workspace's counter prefix with
     // the attention's: the launches are ordered and each leaves them at zero.
     const size_t base = std::max(r.step_bytes, r.select.splits > 1 ? kCounterBytes : 0);
@@ -263,8 +265,7 @@ hipError_t kvq_sparse_decode_launch(const kvq_sparse_decode_params* p, void* wor
     a.counters = plan.select.splits > 1 ? reinterpret_cast<int*>(base) : nullptr;
     a.keys = plan.select.key_bytes ? reinterpret_cast<unsigned*>(base + plan.keys_at) : nullptr;
     a.key_stride = plan.select.key_stride;
-    const bool vec_ok = ((bits(s.k_pages) | bits(p->bounds) | bits(s.q)) & 15u) == 0;
-    const hipError_t err = checked_call(stream, [&] { return kvq::launch_select(a, vec_ok, stream); });
+    const hipError_t err = checked_call(stream, [&] { return kvq::launch_select(a, plan.select, plan.vec_ok, stream); });
     if (err != hipSuccess) return err;
     return kvq_paged_decode_launch(&plan.step, workspace, plan.step_bytes, stream);
 }

@@ -15,6 +15,8 @@
 #include <limits.h>
 #include <math.h>
 
+#include <algorithm>
+
 #include "kvq_bounds.hpp"
 #include "kvq_device.hpp"
 #include "kvq_pages.hpp"
@@ -190,6 +192,172 @@ __device__ inline void write_kept(const SelectArgs& a, const Unit& u, int unit) 
     if (threadIdx.x == 0) a.selected_lengths[unit] = u.len > 0 ? (n - 1) * size + (u.len - 1) % size + 1 : 0;
 }
 
+// Tuned head dims (multiples of 16 up to 256): scores on matrix cores.
+//
+// max(c high, c low) = max(c, 0) high + min(c, 0) low, so with a page's highs
+// and lows as one row of 2 d bytes, which is how they lie in memory, and each
+// head's max(c, 0) and min(c, 0) as one column of 2 d bytes, sixteen pages times
+// sixteen heads are ND = 2 d / 64 int8 matrix products.  The rows come straight
+// from memory into the A operand (16 bytes a lane, four lanes a 64-byte piece),
+// the columns from LDS; columns past the last head repeat one, and bytes past
+// 2 d are zero in the columns.  Reading the bounds is all that costs: 16 pages
+// a wave at a time, the next 16 on their way, their ids one step further ahead.
+//
+// A unit's pages go to `splits` workgroups in whole steps of 128; the last one
+// to arrive ranks.  One workgroup keeps its keys in LDS; several pass them
+// through memory coherently (as split records do, kvq_split.hpp).
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+constexpr int kSelTile = 16;                      // pages a wave scores at a time
+constexpr int kSelStep = kSelTile * kSelWaves;    // pages a workgroup does
+constexpr int kSelLdsKeys = 12288;                // ranks kept in LDS, at most
+
+template <int CTRL>
+__device__ __forceinline__ int dpp_max(int x) {
+    return max(x, __builtin_amdgcn_update_dpp(0, x, CTRL, 0xF, 0xF, false));
+}
+// Signed maximum over each 16 lanes.
+__device__ __forceinline__ int row16_max(int x) {
+    x = dpp_max<kDppQuadXor1>(x);
+    x = dpp_max<kDppQuadXor2>(x);
+    x = dpp_max<kDppRowHalfMirror>(x);
+    return dpp_max<kDppRowMirror>(x);
+}
+
+template <int ND>
+__global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectArgs a, int lds_keys) {
+    extern __shared__ __align__(16) unsigned char s_dyn[];  // columns [passes][ND][64] x 16 bytes, then lds_keys ranks
+    __shared__ RankScratch s;
+    __shared__ float s_max[kSelWaves];
+    __shared__ int s_last;
+    const int t = threadIdx.x;
+    const int lane = t & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(t / kWave);
+    const int units = a.b.B * a.b.Hkv;
+    const int split = blockIdx.x / units;
+    const int unit = blockIdx.x - split * units;
+    const int d = a.b.d;
+    const int passes = (a.G + 15) / 16;
+    unsigned* s_keys = reinterpret_cast<unsigned*>(s_dyn + static_cast<size_t>(passes) * ND * 1024);
+    const Unit u = unit_of(a, unit);
+
+    // This workgroup's pages, and how many workgroups have any.
+    const int n = u.wanted > 0 ? u.scored : 0;
+    const int steps = (n + kSelStep - 1) / kSelStep;
+    const int chunk = (steps + a.splits - 1) / a.splits * kSelStep;
+    const int active = n > 0 ? (n + chunk - 1) / chunk : 1;
+    if (split >= active) return;
+    const int i0 = split * chunk, i1 = min(n, i0 + chunk);
+
+    // The page that has just become whole belongs to the last workgroup, which
+    // ranks it if it is ranked.
+    if (u.renewed >= 0 && split == active - 1 && wave == 0) {
+        constexpr int LPT = ND <= 1 ? 2 : ND <= 2 ? 4 : ND <= 4 ? 8 : 16;
+        bounds_wave<LPT>(a.b, kWave / LPT, true, u.b, u.renewed, u.h, a.b.pages.size);
+    }
+    if (split == 0) write_kept(a, u, unit);
+    if (n == 0) return;
+
+    // The heads' codes.
+    const float* q = a.q + static_cast<size_t>(unit) * a.G * d;
+    float amax = 0.0f;
+    for (int i = t; i < a.G * d / 4; i += kSelThreads) {
+        const float4 x = reinterpret_cast<const float4*>(q)[i];
+        amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+    }
+    amax = wave_max(amax);
+    if (lane == 0) s_max[wave] = amax;
+    __syncthreads();  // and the renewed bounds are written
+#pragma unroll
+    for (int w = 0; w < kSelWaves; w++) amax = fmaxf(amax, s_max[w]);
+    const float qs = quant_scale(amax);
+    for (int w = t; w < passes * ND * 256; w += kSelThreads) {
+        const int col = (w >> 2) & 63;  // operand lane
+        const int step = (w >> 8) % ND, pass = (w >> 8) / ND;
+        const int off = step * 64 + (col >> 4) * 16 + (w & 3) * 4;
+        const int g = pass * 16 + (col & 15);
+        int c[4] = {0, 0, 0, 0};
+        if (off < 2 * d) {
+            const float4 x = *reinterpret_cast<const float4*>(q + static_cast<size_t>(g < a.G ? g : pass * 16) * d + (off < d ? off : off - d));
+            const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) c[j] = off < d ? max(quant_one(y[j], qs), 0) : min(quant_one(y[j], qs), 0);
+        }
+        reinterpret_cast<int*>(s_dyn)[w] = pack4(c[0], c[1], c[2], c[3]);
+    }
+    __syncthreads();
+
+    const bool shared = active > 1 || n > lds_keys;  // keys in memory
+    unsigned* keys = shared ? a.keys + static_cast<size_t>(unit) * a.key_stride : nullptr;
+    const int r = lane & 15, c16 = (lane >> 4) * 16;
+    auto row_of = [&](int i) { return static_cast<size_t>(pool_row(a, u, a.keep_first + min(i, i1 - 1))); };
+    auto load = [&](size_t row, i32x4 (&x)[ND], float& scale) {
+        const int8_t* p = a.b.bounds + row * 2 * d;
+#pragma unroll
+        for (int j = 0; j < ND; j++) x[j] = *reinterpret_cast<const i32x4*>(p + min(j * 64 + c16, 2 * d - 16));
+        scale = a.b.scale[row];
+    };
+    i32x4 next[ND];
+    float next_scale;
+    int base = i0 + wave * kSelTile;
+    size_t row = row_of(base + r);
+    load(row, next, next_scale);
+    row = row_of(base + kSelStep + r);
+    for (; base < i1; base += kSelStep) {
+        i32x4 x[ND];
+#pragma unroll
+        for (int j = 0; j < ND; j++) x[j] = next[j];
+        const float scale = next_scale;
+        load(row, next, next_scale);
+        row = row_of(base + 2 * kSelStep + r);
+        i32x4 top = {INT_MIN, INT_MIN, INT_MIN, INT_MIN};
+        for (int pass = 0; pass < passes; pass++) {
+            i32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < ND; j++) {
+                const i32x4 y = reinterpret_cast<const i32x4*>(s_dyn)[(pass * ND + j) * 64 + lane];
+                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[j], y, acc, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) top[i] = max(top[i], acc[i]);
+        }
+        // Lane 16 g + c holds pages 4 g .. 4 g + 3 of head c; lanes c < 4 write page 4 g + c.
+#pragma unroll
+        for (int i = 0; i < 4; i++) top[i] = row16_max(top[i]);
+        const int best = (r & 2) ? ((r & 1) ? top[3] : top[2]) : ((r & 1) ? top[1] : top[0]);
+        const int page = 4 * (lane >> 4) + (r & 3);
+        const float sc = __shfl(scale, page);
+        const int i = base + page;
+        if (r < 4 && i < i1) {
+            const unsigned key = rank_key(static_cast<float>(best) * sc);
+            if (shared) __hip_atomic_store(keys + i, key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            else s_keys[i] = key;
+        }
+    }
+    if (active > 1) {
+        __builtin_amdgcn_s_waitcnt(0);  // this thread's keys have arrived
+        __syncthreads();
+        if (t == 0) {
+            s_last = __hip_atomic_fetch_add(a.counters + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == active - 1;
+            if (s_last) __hip_atomic_store(a.counters + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (!s_last) return;
+    }
+    if (shared && n <= lds_keys) {
+        for (int i = t; i < n; i += kSelThreads) s_keys[i] = __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    } else if (shared) {
+        __builtin_amdgcn_s_waitcnt(0);
+    }
+    __syncthreads();
+    int32_t* out = a.selected + static_cast<size_t>(unit) * a.max_selected + a.keep_first;
+    auto finish = [&](const auto& key) {
+        const Cut cut = rank_cut(key, n, u.wanted, s);
+        rank_emit(key, n, cut, s, [&](int place, int i) { out[place] = pool_row(a, u, a.keep_first + i); });
+    };
+    if (n <= lds_keys) finish([&](int i) { return s_keys[i]; });
+    else finish([&](int i) { return __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
+}
+
 // Any head dim or alignment: a workgroup a unit, a wave a page, keys in global memory.
 __global__ __launch_bounds__(kSelThreads) void select_generic(const SelectArgs a) {
     __shared__ RankScratch s;
@@ -238,16 +406,50 @@ __global__ __launch_bounds__(kSelThreads) void select_generic(const SelectArgs a
 
 }  // namespace
 
-SelectPlan select_plan(int units, int max_pages, int max_selected) {
-    SelectPlan p{1, 0, 0};
+// A workgroup's columns fit LDS beside the ranks: up to 32 KB of them.
+static bool select_tuned(int G, int d) {
+    return d <= 256 && d % 16 == 0 && (G + 15) / 16 * ((2 * d + 63) / 64) <= 32;
+}
+
+SelectPlan select_plan(int units, int G, int d, bool vec_ok, int max_pages, int max_selected) {
+    SelectPlan p{1, 0, 0, 0};
     if (max_pages <= max_selected) return p;
+    if (vec_ok && select_tuned(G, d)) {
+        // About two workgroups a CU, each with at least one step of pages.
+        const long steps = (static_cast<long>(max_pages) + kSelStep - 1) / kSelStep;
+        if (units <= static_cast<int>(kCounterBytes / sizeof(int)))
+            p.splits = static_cast<int>(std::max(1L, std::min(steps, 512L / units)));
+        p.lds_keys = max_pages <= kSelLdsKeys ? max_pages : 0;
+        if (p.splits == 1 && p.lds_keys > 0) return p;
+    }
     p.key_stride = max_pages;
     p.key_bytes = static_cast<size_t>(units) * max_pages * sizeof(unsigned);
     return p;
 }
 
-hipError_t launch_select(const SelectArgs& a, bool, hipStream_t stream) {
-    hipLaunchKernelGGL(select_generic, dim3(static_cast<unsigned>(a.b.B * a.b.Hkv)), dim3(kSelThreads), 0, stream, a);
+hipError_t launch_select(const SelectArgs& a, const SelectPlan& p, bool vec_ok, hipStream_t stream) {
+    const unsigned units = static_cast<unsigned>(a.b.B * a.b.Hkv);
+    const dim3 block(kSelThreads);
+    if (!vec_ok || !select_tuned(a.G, a.b.d)) {
+        hipLaunchKernelGGL(select_generic, dim3(units), block, 0, stream, a);
+        return hipGetLastError();
+    }
+    const int nd = (2 * a.b.d + 63) / 64;
+    const dim3 grid(units * static_cast<unsigned>(p.splits));
+    const size_t lds = static_cast<size_t>((a.G + 15) / 16) * nd * 1024 + static_cast<size_t>(p.lds_keys) * sizeof(unsigned);
+#define KVQ_SELECT_CASE(ND) \
+    case ND: hipLaunchKernelGGL(select_kernel<ND>, grid, block, lds, stream, a, p.lds_keys); break;
+    switch (nd) {
+        KVQ_SELECT_CASE(1)
+        KVQ_SELECT_CASE(2)
+        KVQ_SELECT_CASE(3)
+        KVQ_SELECT_CASE(4)
+        KVQ_SELECT_CASE(5)
+        KVQ_SELECT_CASE(6)
+        KVQ_SELECT_CASE(7)
+        KVQ_SELECT_CASE(8)
+    }
+#undef KVQ_SELECT_CASE
     return hipGetLastError();
 }
 

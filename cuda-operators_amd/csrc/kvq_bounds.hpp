@@ -46,24 +46,27 @@ __device__ inline void bounds_generic(const BoundsArgs& a, int b, int pi, int h,
     if (lane == 0) a.scale[unit] = fine ? S : INFINITY;
 }
 
-// Tuned: LPT lanes a token with 16 bytes of its row each (LPT: d / 16 rounded up
-// to a power of two; the lanes past the row's end read its last piece again),
-// groups of LPT lanes a page (a power of two up to 64 / LPT), so a wave holds
+// Tuned: LPT lanes a token with 8 bytes of its row each (LPT: d / 8 rounded up to
+// a power of two; the lanes past the row's end read its last piece again), groups
+// of LPT lanes a page (a power of two up to 64 / LPT), so a wave holds
 // 64 / (LPT * groups) pages.  Group g of a page takes tokens g, g + groups, ..,
-// 16 at a time with 8 loads in flight a lane; a token past the page's last one
-// repeats that one, which changes no maximum.  The ratios are divided once a
-// token (lane j of a group those of tokens j, j + LPT, ..) and handed round.
-// live: this lane's page exists (others run along on page entry pi = 0 of it
-// and store nothing).
+// 16 loads at a time; a token past the page's last one repeats that one, which
+// changes no maximum.  The ratios are divided once a token (lane j of a group
+// that of token j) and handed round.  What bounds it is the chain of loads (the
+// page's id, its scales, its keys) of waves that each read a few KB: 8 bytes a
+// lane leave 16 results instead of 32 in its registers, so that twice as many
+// waves are there to wait.
+// live: this lane's page exists (others run along on another page and store nothing).
 template <int LPT>
 __device__ inline void bounds_wave(const BoundsArgs& a, int groups, bool live, int b, int pi, int h, int tokens) {
     constexpr int NT = 16;                            // tokens a group takes at a time
     constexpr int NS = NT / LPT > 1 ? NT / LPT : 1;  // scales a lane holds of them
+    typedef int v2i_t __attribute__((ext_vector_type(2)));
     const int lane = threadIdx.x & (kWave - 1);
     const int ds = lane % LPT;
     const int g = lane / LPT % groups;
     const int d = a.d;
-    const int off = min(ds * 16, d - 16);
+    const int off = min(ds * 8, d - 8);
     const int id = a.pages.table[static_cast<size_t>(b) * a.pages.max_pages + pi];
     const size_t unit = static_cast<size_t>(min(max(id, 0), a.pages.num_pages - 1)) * a.Hkv + h;
     const int8_t* k = a.k + unit * a.pages.size * d + off;
@@ -74,17 +77,17 @@ __device__ inline void bounds_wave(const BoundsArgs& a, int groups, bool live, i
 #pragma unroll
         for (int j = 0; j < NS; j++) x[j] = s[min((pass * NT + (ds + j * LPT) % NT) * groups + g, tokens - 1)];
     };
-    auto load = [&](int pass, int half, int4 (&x)[NT / 2]) {
+    v2i_t raw[NT];
+    auto load = [&](int pass) {
 #pragma unroll
-        for (int u = 0; u < NT / 2; u++) {
-            const int t = min((pass * NT + half * (NT / 2) + u) * groups + g, tokens - 1);
-            x[u] = load16_stream(k + static_cast<size_t>(t) * d);
+        for (int u = 0; u < NT; u++) {
+            const int t = min((pass * NT + u) * groups + g, tokens - 1);
+            raw[u] = __builtin_nontemporal_load(reinterpret_cast<const v2i_t*>(k + static_cast<size_t>(t) * d));
         }
     };
-    int4 raw[NT / 2];
     float sc[NS];
     scales(0, sc);
-    load(0, 0, raw);  // on its way while the scales are reduced
+    load(0);  // on its way while the scales are reduced
     float S = 0.0f;
     for (int pass = 0; pass < passes; pass++) {
         if (pass > 0) scales(pass, sc);
@@ -94,70 +97,61 @@ __device__ inline void bounds_wave(const BoundsArgs& a, int groups, bool live, i
     for (int o = 1; o < LPT * groups; o <<= 1) S = max_or_nan(S, __shfl_xor(S, o));
     const bool fine = S < INFINITY;
 
-    float hi[16], lo[16];
+    float hi[8], lo[8];
 #pragma unroll
-    for (int i = 0; i < 16; i++) hi[i] = -INFINITY, lo[i] = INFINITY;
+    for (int i = 0; i < 8; i++) hi[i] = -INFINITY, lo[i] = INFINITY;
     if (passes > 1) scales(0, sc);
     for (int pass = 0; pass < passes; pass++) {
         if (pass > 0) {
             scales(pass, sc);
-            load(pass, 0, raw);
+            load(pass);
         }
         float r[NS];
 #pragma unroll
         for (int j = 0; j < NS; j++) r[j] = bound_ratio(sc[j], S);
+        // Keeps the conversions here: moved up into the two blocks that load raw,
+        // they would hold every token's 8 products at once (230 registers).
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-            if (half == 1) load(pass, 1, raw);
+        for (int u = 0; u < NT; u++) asm volatile("" : "+v"(raw[u]));
 #pragma unroll
-            for (int u = 0; u < NT / 2; u += 2) {
-                const int t0 = half * (NT / 2) + u;
-                const float r0 = __shfl(r[t0 / LPT], (lane & ~(LPT - 1)) + t0 % LPT);
-                const float r1 = __shfl(r[(t0 + 1) / LPT], (lane & ~(LPT - 1)) + (t0 + 1) % LPT);
-                float x0[16], x1[16];
-                unpack16(raw[u], x0);
-                unpack16(raw[u + 1], x1);
+        for (int u = 0; u < NT; u += 2) {
+            const float r0 = __shfl(r[u / LPT], (lane & ~(LPT - 1)) + u % LPT);
+            const float r1 = __shfl(r[(u + 1) / LPT], (lane & ~(LPT - 1)) + (u + 1) % LPT);
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    x0[i] *= r0;
-                    x1[i] *= r1;
-                    hi[i] = fmaxf(fmaxf(x0[i], x1[i]), hi[i]);
-                    lo[i] = fminf(fminf(x0[i], x1[i]), lo[i]);
-                }
+            for (int i = 0; i < 8; i++) {
+                const float x0 = sbyte(raw[u][i / 4], i & 3) * r0;
+                const float x1 = sbyte(raw[u + 1][i / 4], i & 3) * r1;
+                hi[i] = fmaxf(fmaxf(x0, x1), hi[i]);
+                lo[i] = fminf(fminf(x0, x1), lo[i]);
             }
         }
     }
     // (high, -low) as two 16-bit codes, so one packed maximum joins the groups' both.
     typedef short s16x2 __attribute__((ext_vector_type(2)));
-    s16x2 m[16];
+    s16x2 m[8];
 #pragma unroll
-    for (int i = 0; i < 16; i++)
+    for (int i = 0; i < 8; i++)
         m[i] = fine ? s16x2{static_cast<short>(bound_code(ceilf(hi[i]))), static_cast<short>(-bound_code(floorf(lo[i])))}
                     : s16x2{127, 127};
     for (int o = LPT; o < LPT * groups; o <<= 1) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
+        for (int i = 0; i < 8; i++) {
             const int x = __shfl_xor(__builtin_bit_cast(int, m[i]), o);
             m[i] = __builtin_elementwise_max(m[i], __builtin_bit_cast(s16x2, x));
         }
     }
     if (!live || g != 0) return;
-    if (ds * 16 < d) {
-        int h4[4], l4[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            h4[j] = pack4(m[4 * j].x, m[4 * j + 1].x, m[4 * j + 2].x, m[4 * j + 3].x);
-            l4[j] = pack4(-m[4 * j].y, -m[4 * j + 1].y, -m[4 * j + 2].y, -m[4 * j + 3].y);
-        }
+    if (ds * 8 < d) {
         int8_t* o = a.bounds + unit * 2 * d + off;
-        *reinterpret_cast<int4*>(o) = make_int4(h4[0], h4[1], h4[2], h4[3]);
-        *reinterpret_cast<int4*>(o + d) = make_int4(l4[0], l4[1], l4[2], l4[3]);
+        *reinterpret_cast<int2*>(o) = make_int2(pack4(m[0].x, m[1].x, m[2].x, m[3].x), pack4(m[4].x, m[5].x, m[6].x, m[7].x));
+        *reinterpret_cast<int2*>(o + d) =
+            make_int2(pack4(-m[0].y, -m[1].y, -m[2].y, -m[3].y), pack4(-m[4].y, -m[5].y, -m[6].y, -m[7].y));
     }
     if (ds == 0) a.scale[unit] = fine ? S : INFINITY;
 }
 
 // Lanes a token of bounds_wave takes, and groups a page that leave a group 16 tokens or fewer where it can.
-constexpr int bounds_lanes(int d) { return d <= 32 ? 2 : d <= 64 ? 4 : d <= 128 ? 8 : 16; }
+constexpr int bounds_lanes(int d) { return d <= 32 ? 4 : d <= 64 ? 8 : d <= 128 ? 16 : 32; }
 __host__ __device__ inline int bounds_groups(int page_size, int lanes) {
     int g = 1;
     while (g < kWave / lanes && g * 16 < page_size) g *= 2;

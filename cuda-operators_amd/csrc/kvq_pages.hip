@@ -25,52 +25,14 @@ namespace {
 // to hand out, [F + R - A, F) and pages given up, are never written, so the
 // workgroups need no order among them; only lengths and the free count, which
 // may be updated in place, are written by the last workgroup to arrive.
-// Bound by latency: the loads of the lengths, two scans, a dependent load of a
-// page id, the stores.
+// Bound by latency: every workgroup loads the lengths and scans them (so a call
+// is one launch), then takes its share of the rows and pages, each a search in
+// LDS, a dependent load of a page id and a store.
 constexpr int kMapThreads = 1024;
 constexpr int kMapWaves = kMapThreads / kWave;
 
-__device__ __forceinline__ unsigned long long wave_inclusive_scan64(unsigned long long v, int lane) {
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-        const unsigned long long x = __shfl_up(v, off);
-        if (lane >= off) v += x;
-    }
-    return v;
-}
-
-// Inclusive scan of one value a thread over the workgroup; part: one entry a
-// wave, used by this scan alone.
-__device__ __forceinline__ unsigned long long group_inclusive_scan(unsigned long long v, unsigned long long* part) {
-    const int lane = threadIdx.x & (kWave - 1);
-    const int wave = threadIdx.x / kWave;
-    v = wave_inclusive_scan64(v, lane);
-    if (lane == kWave - 1) part[wave] = v;
-    __syncthreads();
-    for (int w = 0; w < wave; w++) v += part[w];
-    return v;
-}
-
 __device__ __forceinline__ int pages_of(int tokens, const FastDiv& page) {
     return static_cast<int>(fastdiv(static_cast<uint32_t>(tokens) + page.d - 1, page));
-}
-
-// What sequence b asks for.  off: its first packed row, saturated at a.T.
-struct Request {
-    int old, want;  // tokens held, and if its pages are granted
-    int rows, need, gives;
-};
-__device__ __forceinline__ Request request_of(const PageMapArgs& a, int b, long long off) {
-    Request r;
-    const int n = a.new_tokens[b];
-    r.old = min(max(a.lengths[b], 0), a.cap);
-    r.rows = max(n, 0);
-    if (n < 0) r.want = max(r.old + n, 0);
-    else r.want = n <= a.cap - r.old && off + n <= a.T ? r.old + n : r.old;
-    const int p0 = pages_of(r.old, a.page), p1 = pages_of(r.want, a.page);
-    r.need = max(p1 - p0, 0);
-    r.gives = max(p0 - p1, 0);
-    return r;
 }
 
 // The last i in [0, n) with v[i] <= x, for ascending v with v[0] <= x.
@@ -84,99 +46,159 @@ __device__ __forceinline__ int last_not_above(const int* v, int n, int x) {
     return lo;
 }
 
+// Inclusive scans of K values a thread over the workgroup, and their totals;
+// part: this scan's own scratch.
+template <int K>
+__device__ __forceinline__ void group_inclusive_scan(int (&v)[K], int (&total)[K], int (&part)[K][kMapWaves]) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = threadIdx.x / kWave;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        v[k] = wave_inclusive_scan(v[k]);
+        if (lane == kWave - 1) part[k][wave] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const int x = wave_inclusive_scan(lane < kMapWaves ? part[k][lane] : 0);
+        total[k] = __builtin_amdgcn_readlane(x, kMapWaves - 1);
+        const int w = __builtin_amdgcn_readfirstlane(wave);
+        if (w > 0) v[k] += __builtin_amdgcn_readlane(x, w - 1);
+    }
+}
+
+// PER sequences a thread: thread t has sequences [t * PER, (t + 1) * PER).
+template <int PER>
 __global__ __launch_bounds__(kMapThreads) void page_map_kernel(const PageMapArgs a) {
-    extern __shared__ int s_map[];  // B + 1 row offsets, B needs, B gives (exclusive prefix sums)
-    __shared__ unsigned long long s_part[2][kMapWaves];
-    __shared__ int s_taken[kMapWaves];
+    // Exclusive prefix sums of rows (saturated at a.T), pages needed and pages
+    // given up, each with its total behind it; and the lengths, bit 31 set where
+    // a request is refused.
+    extern __shared__ int s_map[];
+    __shared__ int s_rows[2][kMapWaves], s_pages[2][kMapWaves], s_taken[kMapWaves];
     __shared__ int s_last;
+    const int B = a.B;
     int* s_off = s_map;
-    int* s_need = s_map + a.B + 1;
-    int* s_gives = s_need + a.B;
+    int* s_need = s_off + B + 1;
+    int* s_gives = s_need + B + 1;
+    int* s_old = s_gives + B + 1;
     const int t = threadIdx.x;
     const int lane = t & (kWave - 1);
-    const int wave = t / kWave;
-    const int per = (a.B + kMapThreads - 1) / kMapThreads;
-    const int b0 = min(t * per, a.B), b1 = min(b0 + per, a.B);
+    const int b0 = t * PER;
 
-    unsigned long long rows = 0;
-    for (int b = b0; b < b1; b++) rows += static_cast<unsigned>(max(a.new_tokens[b], 0));
-    unsigned long long at = group_inclusive_scan(rows, s_part[0]) - rows;
-    for (int b = b0; b < b1; b++) {
-        s_off[b] = static_cast<int>(min(at, static_cast<unsigned long long>(a.T)));
-        at += static_cast<unsigned>(max(a.new_tokens[b], 0));
+    int n[PER], old[PER];
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+        const int b = b0 + k;
+        n[k] = b < B ? a.new_tokens[b] : 0;
+        old[k] = b < B ? min(max(a.lengths[b], 0), a.cap) : 0;
     }
-    if (b1 == a.B) s_off[a.B] = static_cast<int>(min(at, static_cast<unsigned long long>(a.T)));  // every such thread alike
-
-    // Pages: needs in the low half, gives in the high half (both below 2^31:
-    // B * max_pages is).
-    unsigned long long sum = 0;
-    for (int b = b0; b < b1; b++) {
-        const Request r = request_of(a, b, s_off[b]);
-        sum += (static_cast<unsigned long long>(static_cast<unsigned>(r.gives)) << 32) | static_cast<unsigned>(r.need);
-    }
-    at = group_inclusive_scan(sum, s_part[1]) - sum;
-    unsigned long long total = 0;
-    for (int w = 0; w < kMapWaves; w++) total += s_part[1][w];
     const int F = min(max(*a.free_count, 0), a.num_pages);
-    const long long have = static_cast<long long>(F) + static_cast<long long>(total >> 32);  // F + R
-    int taken = 0;
-    for (int b = b0; b < b1; b++) {
-        const Request r = request_of(a, b, s_off[b]);
-        s_need[b] = static_cast<int>(at & 0xffffffffu);
-        s_gives[b] = static_cast<int>(at >> 32);
-        at += (static_cast<unsigned long long>(static_cast<unsigned>(r.gives)) << 32) | static_cast<unsigned>(r.need);
-        const int incl = s_need[b] + r.need;
-        if (incl <= have) taken = max(taken, incl);
+
+    // Rows: sums of up to 4096 requests below 2^31, as sums of their halves.
+    int half[2] = {0, 0}, sum[2];
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+        half[0] += max(n[k], 0) & 0xffff;
+        half[1] += max(n[k], 0) >> 16;
+    }
+    int scan[2] = {half[0], half[1]};
+    group_inclusive_scan(scan, sum, s_rows);
+    long long at = static_cast<long long>(scan[0] - half[0]) + (static_cast<long long>(scan[1] - half[1]) << 16);
+    const long long all = static_cast<long long>(sum[0]) + (static_cast<long long>(sum[1]) << 16);
+
+    // Pages.  Totals stay below 2^31: B * max_pages does.
+    int want[PER], p0[PER], moves[PER];  // moves: pages needed, or those given up as a negative number
+    int pages[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+        const int b = b0 + k;
+        if (b < B) s_off[b] = static_cast<int>(min(at, static_cast<long long>(a.T)));
+        at += max(n[k], 0);
+        want[k] = n[k] < 0 ? max(old[k] + n[k], 0) : n[k] <= a.cap - old[k] && at <= a.T ? old[k] + n[k] : old[k];
+        p0[k] = pages_of(old[k], a.page);
+        moves[k] = pages_of(want[k], a.page) - p0[k];
+        pages[0] += max(moves[k], 0);
+        pages[1] += max(-moves[k], 0);
+    }
+    int pscan[2] = {pages[0], pages[1]}, ptotal[2];
+    group_inclusive_scan(pscan, ptotal, s_pages);
+    const int R = ptotal[1];
+    const long long have = static_cast<long long>(F) + R;
+    int need = pscan[0] - pages[0], gives = pscan[1] - pages[1], taken = 0;
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+        const int b = b0 + k;
+        const int incl = need + max(moves[k], 0);
+        const bool enough = incl <= have;
+        const bool refused = n[k] > 0 && (want[k] == old[k] || (moves[k] > 0 && !enough));
+        if (b < B) {
+            s_need[b] = need;
+            s_gives[b] = gives;
+            s_old[b] = old[k] | (refused ? INT_MIN : 0);
+        }
+        if (refused) want[k] = old[k];
+        if (enough) taken = max(taken, incl);
+        need = incl;
+        gives += max(-moves[k], 0);
     }
 #pragma unroll
     for (int off = kWave / 2; off > 0; off >>= 1) taken = max(taken, __shfl_xor(taken, off));
-    if (lane == 0) s_taken[wave] = taken;
+    if (lane == 0) s_taken[t / kWave] = taken;
+    if (t == 0) {
+        s_off[B] = static_cast<int>(min(all, static_cast<long long>(a.T)));
+        s_need[B] = ptotal[0];
+        s_gives[B] = R;
+    }
     __syncthreads();
-    int A = 0;
+    int A = 0;  // pages taken
+#pragma unroll
     for (int w = 0; w < kMapWaves; w++) A = max(A, s_taken[w]);
     const long long left = have - A;  // entries of the stack afterwards
 
-    auto granted = [&](int b, const Request& r) { return r.need == 0 || s_need[b] + r.need <= have; };
     auto given_up = [&](int g) {  // the g-th page given up
-        const int c = last_not_above(s_gives, a.B, g);
-        const Request r = request_of(a, c, s_off[c]);
-        return a.table[static_cast<size_t>(c) * a.max_pages + pages_of(r.want, a.page) + (g - s_gives[c])];
+        const int c = last_not_above(s_gives, B, g);
+        const int end = pages_of(s_old[c], a.page);  // a shrinking sequence is not refused
+        return a.table[static_cast<size_t>(c) * a.max_pages + end - (s_gives[c + 1] - s_gives[c]) + (g - s_gives[c])];
     };
     auto stack_at = [&](long long i) { return i < F ? a.free_pages[i] : given_up(static_cast<int>(i - F)); };
 
-    // Pages: a wave a sequence.
-    const int waves = gridDim.x * kMapWaves;
-    for (int b = blockIdx.x * kMapWaves + wave; b < a.B; b += waves) {
-        const Request r = request_of(a, b, s_off[b]);
-        int32_t* row = a.table + static_cast<size_t>(b) * a.max_pages;
-        if (r.need > 0 && granted(b, r)) {
-            const int p0 = pages_of(r.old, a.page);
-            for (int i = lane; i < r.need; i += kWave) row[p0 + i] = stack_at(have - 1 - (s_need[b] + i));
-        }
-        const int p1 = pages_of(r.want, a.page);
-        for (int i = lane; i < r.gives; i += kWave) {
-            const long long to = static_cast<long long>(F) + s_gives[b] + i;
-            if (to < left && to < a.num_pages) a.free_pages[to] = row[p1 + i];
-        }
+    // Each job begins at another third of the threads, so that small ones run at
+    // the same time in different waves instead of one load after the other.
+    const int step = gridDim.x * kMapThreads;
+    const int me = blockIdx.x * kMapThreads + t;
+    const int third = step / 3 / kWave * kWave;
+    for (long long i = me; i < A; i += step) {
+        const int page = static_cast<int>(i);
+        const int b = last_not_above(s_need, B, page);
+        a.table[static_cast<size_t>(b) * a.max_pages + pages_of(s_old[b], a.page) + (page - s_need[b])] = stack_at(have - 1 - i);
+    }
+    const long long back = min(left, static_cast<long long>(a.num_pages)) - F;  // pages given up that stay on the stack
+    constexpr int kBack = 4;  // loads in flight
+    for (long long i = me < third ? me - third + step : me - third; i < back; i += static_cast<long long>(kBack) * step) {
+        int id[kBack];
+#pragma unroll
+        for (int k = 0; k < kBack; k++) id[k] = given_up(static_cast<int>(min(i + static_cast<long long>(k) * step, back - 1)));
+#pragma unroll
+        for (int k = 0; k < kBack; k++)
+            if (i + static_cast<long long>(k) * step < back) a.free_pages[F + i + static_cast<long long>(k) * step] = id[k];
     }
 
     // Packed rows.  A new page's id is taken from the stack again rather than
     // from the table, which another wave may not have written yet.
     if (a.slot_map || a.token_seq || a.token_pos) {
-        const long long step = static_cast<long long>(gridDim.x) * kMapThreads;
-        for (long long i = static_cast<long long>(blockIdx.x) * kMapThreads + t; i < a.T; i += step) {
+        for (long long i = me < 2 * third ? me - 2 * third + step : me - 2 * third; i < a.T; i += step) {
             int slot = -1, seq = -1, pos = -1;
             const int row = static_cast<int>(i);
-            if (row < s_off[a.B]) {
-                seq = last_not_above(s_off, a.B, row);
-                const Request r = request_of(a, seq, s_off[seq]);
-                const int k = row - s_off[seq];
-                pos = static_cast<int>(min(static_cast<long long>(r.old) + k, static_cast<long long>(INT_MAX)));
-                if (k < r.want - r.old && granted(seq, r)) {
+            if (row < s_off[B]) {
+                seq = last_not_above(s_off, B, row);
+                const int held = s_old[seq];
+                const unsigned at_pos = static_cast<unsigned>(held & INT_MAX) + static_cast<unsigned>(row - s_off[seq]);
+                pos = static_cast<int>(min(at_pos, static_cast<unsigned>(INT_MAX)));
+                if (held >= 0) {
                     const int pi = static_cast<int>(fastdiv(static_cast<uint32_t>(pos), a.page));
-                    const int p0 = pages_of(r.old, a.page);
-                    const int id = pi < p0 ? a.table[static_cast<size_t>(seq) * a.max_pages + pi]
-                                           : stack_at(have - 1 - (s_need[seq] + pi - p0));
+                    const int first = pages_of(held, a.page);
+                    const int id = pi < first ? a.table[static_cast<size_t>(seq) * a.max_pages + pi]
+                                              : stack_at(have - 1 - (s_need[seq] + pi - first));
                     const int size = static_cast<int>(a.page.d);
                     if (id >= 0 && id < a.num_pages) slot = id * size + (pos - pi * size);
                 }
@@ -188,24 +210,26 @@ __global__ __launch_bounds__(kMapThreads) void page_map_kernel(const PageMapArgs
     }
 
     // The last workgroup writes what the others read.
-    __syncthreads();
     if (a.arrivals) {
-        if (t == 0)
+        __syncthreads();
+        if (t == 0) {
             s_last = __hip_atomic_fetch_add(a.arrivals, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
                      static_cast<int>(gridDim.x) - 1;
+            if (s_last) __hip_atomic_store(a.arrivals, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
         __syncthreads();
         if (!s_last) return;
-        if (t == 0) __hip_atomic_store(a.arrivals, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    for (int b = b0; b < b1; b++) {
-        const Request r = request_of(a, b, s_off[b]);
-        const int now = granted(b, r) ? r.want : r.old;
-        a.new_lengths[b] = now;
-        a.granted[b] = now - r.old;
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+        const int b = b0 + k;
+        if (b >= B) break;
+        a.new_lengths[b] = want[k];
+        a.granted[b] = want[k] - old[k];
         a.offsets[b] = s_off[b];
     }
     if (t == 0) {
-        a.offsets[a.B] = s_off[a.B];
+        a.offsets[B] = s_off[B];
         *a.new_free_count = static_cast<int>(min(left, static_cast<long long>(a.num_pages)));
     }
 }
@@ -460,11 +484,26 @@ __global__ __launch_bounds__(kBoundsWaves* kWave) void page_bounds_generic(const
 
 }  // namespace
 
-int page_map_groups(const PageMapArgs&) { return 1; }
+// Workgroups of 1024 threads, two rows a thread, up to 64 (each scans the whole
+// batch).  Without arrays of rows the pages are what there is to do.
+#ifndef KVQ_MAP_ROWS
+#define KVQ_MAP_ROWS 2048
+#endif
+#ifndef KVQ_MAP_GROUPS
+#define KVQ_MAP_GROUPS 64
+#endif
+int page_map_groups(const PageMapArgs& a) {
+    const long long work = a.slot_map || a.token_seq || a.token_pos
+                               ? a.T
+                               : min(static_cast<long long>(a.T / static_cast<int>(a.page.d)) + a.B, static_cast<long long>(a.num_pages));
+    return static_cast<int>(max(1LL, min(static_cast<long long>(KVQ_MAP_GROUPS), (work + KVQ_MAP_ROWS - 1) / KVQ_MAP_ROWS)));
+}
 
 hipError_t launch_page_map(const PageMapArgs& a, hipStream_t stream) {
-    const size_t lds = sizeof(int) * (3 * static_cast<size_t>(a.B) + 1);
-    hipLaunchKernelGGL(page_map_kernel, dim3(static_cast<unsigned>(page_map_groups(a))), dim3(kMapThreads), lds, stream, a);
+    const dim3 grid(static_cast<unsigned>(page_map_groups(a))), block(kMapThreads);
+    const size_t lds = sizeof(int) * (4 * static_cast<size_t>(a.B) + 3);
+    if (a.B <= kMapThreads) hipLaunchKernelGGL(page_map_kernel<1>, grid, block, lds, stream, a);
+    else hipLaunchKernelGGL(page_map_kernel<4>, grid, block, lds, stream, a);
     return hipGetLastError();
 }
 
@@ -523,10 +562,10 @@ hipError_t launch_page_bounds(const BoundsArgs& a, bool vec_ok, hipStream_t stre
     const unsigned ny = static_cast<unsigned>(min((units + per - 1) / per, max(1LL, 8192LL / a.B)));
     const dim3 grid(static_cast<unsigned>(a.B), ny), block(kBoundsWaves * kWave);
     if (!tuned) hipLaunchKernelGGL(page_bounds_generic, grid, block, 0, stream, a);
-    else if (lanes == 2) hipLaunchKernelGGL(page_bounds_kernel<2>, grid, block, 0, stream, a, groups);
     else if (lanes == 4) hipLaunchKernelGGL(page_bounds_kernel<4>, grid, block, 0, stream, a, groups);
     else if (lanes == 8) hipLaunchKernelGGL(page_bounds_kernel<8>, grid, block, 0, stream, a, groups);
-    else hipLaunchKernelGGL(page_bounds_kernel<16>, grid, block, 0, stream, a, groups);
+    else if (lanes == 16) hipLaunchKernelGGL(page_bounds_kernel<16>, grid, block, 0, stream, a, groups);
+    else hipLaunchKernelGGL(page_bounds_kernel<32>, grid, block, 0, stream, a, groups);
     return hipGetLastError();
 }
 

@@ -50,18 +50,14 @@ struct Cut {
     int ties;
 };
 
-// Cut of the k largest of n keys (0 < k < n), by the whole workgroup; key(i) reads key i.
+// Cut of the k largest of n keys (0 < k < n), by the whole workgroup; key(i)
+// reads key i, lo and hi are the smallest and largest that this thread has seen,
+// all threads together having seen all.
 template <class Key>
-__device__ inline Cut rank_cut(const Key& key, int n, int k, RankScratch& s) {
+__device__ inline Cut rank_cut(const Key& key, int n, int k, unsigned lo, unsigned hi, RankScratch& s) {
     const int t = threadIdx.x;
     const int lane = t & (kWave - 1);
     const int wave = t / kWave;
-    unsigned lo = 0xffffffffu, hi = 0;
-    for (int i = t; i < n; i += kSelThreads) {
-        const unsigned x = key(i);
-        lo = min(lo, x);
-        hi = max(hi, x);
-    }
 #pragma unroll
     for (int off = kWave / 2; off > 0; off >>= 1) {
         lo = min(lo, static_cast<unsigned>(__shfl_xor(static_cast<int>(lo), off)));
@@ -159,17 +155,20 @@ struct Unit {
     int wanted;   // of those, how many are attended
     int renewed;  // page entry whose bounds this launch writes, or -1
 };
+__device__ __forceinline__ int page_entry(const SelectArgs& a, int token) {
+    return a.b.pages.shift >= 0 ? token >> a.b.pages.shift : token / a.b.pages.size;
+}
 __device__ __forceinline__ Unit unit_of(const SelectArgs& a, int unit) {
     Unit u;
     u.b = unit / a.b.Hkv;
     u.h = unit - u.b * a.b.Hkv;
     u.len = a.b.lengths ? min(max(a.b.lengths[u.b], 0), a.b.max_len) : a.b.max_len;
     const int size = a.b.pages.size;
-    u.pages = u.len > 0 ? (u.len - 1) / size + 1 : 0;
+    u.pages = u.len > 0 ? page_entry(a, u.len - 1) + 1 : 0;
     const bool rank = u.pages > a.max_selected;
     u.scored = rank ? u.pages - a.keep_first - a.keep_last : 0;
     u.wanted = rank ? a.max_selected - a.keep_first - a.keep_last : 0;
-    u.renewed = u.len > 1 && (u.len - 1) % size == 0 ? u.pages - 2 : -1;
+    u.renewed = u.len > 1 && (u.pages - 1) * size == u.len - 1 ? u.pages - 2 : -1;
     return u;
 }
 
@@ -189,7 +188,7 @@ __device__ inline void write_kept(const SelectArgs& a, const Unit& u, int unit) 
         else if (i >= n) out[i] = -1;
         else if (i >= n - a.keep_last) out[i] = pool_row(a, u, u.pages - n + i);
     }
-    if (threadIdx.x == 0) a.selected_lengths[unit] = u.len > 0 ? (n - 1) * size + (u.len - 1) % size + 1 : 0;
+    if (threadIdx.x == 0) a.selected_lengths[unit] = u.len > 0 ? (n - u.pages) * size + u.len : 0;
 }
 
 // Tuned head dims (multiples of 16 up to 256): scores on matrix cores.
@@ -224,7 +223,7 @@ __device__ __forceinline__ int row16_max(int x) {
 }
 
 template <int ND>
-__global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectArgs a, int lds_keys) {
+__global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))) void select_kernel(const SelectArgs a, int lds_keys) {
     extern __shared__ __align__(16) unsigned char s_dyn[];  // columns [passes][ND][64] x 16 bytes, then lds_keys ranks
     __shared__ RankScratch s;
     __shared__ float s_max[kSelWaves];
@@ -251,11 +250,29 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectArgs a,
     // The page that has just become whole belongs to the last workgroup, which
     // ranks it if it is ranked.
     if (u.renewed >= 0 && split == active - 1 && wave == 0) {
-        constexpr int LPT = ND <= 1 ? 2 : ND <= 2 ? 4 : ND <= 4 ? 8 : 16;
+        constexpr int LPT = bounds_lanes(32 * ND);
         bounds_wave<LPT>(a.b, kWave / LPT, true, u.b, u.renewed, u.h, a.b.pages.size);
     }
     if (split == 0) write_kept(a, u, unit);
     if (n == 0) return;
+
+    const int r = lane & 15, c16 = (lane >> 4) * 16;
+    auto row_of = [&](int i) { return static_cast<size_t>(pool_row(a, u, a.keep_first + min(i, i1 - 1))); };
+    auto load = [&](size_t row, i32x4 (&x)[ND], float& scale) {
+        const int8_t* p = a.b.bounds + row * 2 * d;
+#pragma unroll
+        for (int j = 0; j < ND; j++) x[j] = *reinterpret_cast<const i32x4*>(p + min(j * 64 + c16, 2 * d - 16));
+        scale = a.b.scale[row];
+    };
+    // The first pages' bounds are on their way while the heads' codes are made,
+    // unless this workgroup is writing some of them.
+    i32x4 next[ND];
+    float next_scale = 0.0f;
+    int base = i0 + wave * kSelTile;
+    const size_t row0 = row_of(base + r);
+    size_t row = row_of(base + kSelStep + r);
+    const bool renews = u.renewed >= 0 && split == active - 1;
+    if (!renews) load(row0, next, next_scale);
 
     // The heads' codes.
     const float* q = a.q + static_cast<size_t>(unit) * a.G * d;
@@ -288,20 +305,8 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectArgs a,
 
     const bool shared = active > 1 || n > lds_keys;  // keys in memory
     unsigned* keys = shared ? a.keys + static_cast<size_t>(unit) * a.key_stride : nullptr;
-    const int r = lane & 15, c16 = (lane >> 4) * 16;
-    auto row_of = [&](int i) { return static_cast<size_t>(pool_row(a, u, a.keep_first + min(i, i1 - 1))); };
-    auto load = [&](size_t row, i32x4 (&x)[ND], float& scale) {
-        const int8_t* p = a.b.bounds + row * 2 * d;
-#pragma unroll
-        for (int j = 0; j < ND; j++) x[j] = *reinterpret_cast<const i32x4*>(p + min(j * 64 + c16, 2 * d - 16));
-        scale = a.b.scale[row];
-    };
-    i32x4 next[ND];
-    float next_scale;
-    int base = i0 + wave * kSelTile;
-    size_t row = row_of(base + r);
-    load(row, next, next_scale);
-    row = row_of(base + kSelStep + r);
+    if (renews) load(row0, next, next_scale);
+    unsigned lo = 0xffffffffu, hi = 0;  // of the keys this thread has seen
     for (; base < i1; base += kSelStep) {
         i32x4 x[ND];
 #pragma unroll
@@ -329,6 +334,8 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectArgs a,
         const int i = base + page;
         if (r < 4 && i < i1) {
             const unsigned key = rank_key(static_cast<float>(best) * sc);
+            lo = min(lo, key);
+            hi = max(hi, key);
             if (shared) __hip_atomic_store(keys + i, key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             else s_keys[i] = key;
         }
@@ -344,14 +351,20 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectArgs a,
         if (!s_last) return;
     }
     if (shared && n <= lds_keys) {
-        for (int i = t; i < n; i += kSelThreads) s_keys[i] = __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int i = t; i < n; i += kSelThreads) {
+            const unsigned key = __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            s_keys[i] = key;
+            lo = min(lo, key);
+            hi = max(hi, key);
+        }
     } else if (shared) {
         __builtin_amdgcn_s_waitcnt(0);
+        lo = 0, hi = 0xffffffffu;
     }
     __syncthreads();
     int32_t* out = a.selected + static_cast<size_t>(unit) * a.max_selected + a.keep_first;
     auto finish = [&](const auto& key) {
-        const Cut cut = rank_cut(key, n, u.wanted, s);
+        const Cut cut = rank_cut(key, n, u.wanted, lo, hi, s);
         rank_emit(key, n, cut, s, [&](int place, int i) { out[place] = pool_row(a, u, a.keep_first + i); });
     };
     if (n <= lds_keys) finish([&](int i) { return s_keys[i]; });
@@ -399,7 +412,7 @@ __global__ __launch_bounds__(kSelThreads) void select_generic(const SelectArgs a
     }
     __syncthreads();
     auto key = [&](int i) { return keys[i]; };
-    const Cut cut = rank_cut(key, u.scored, u.wanted, s);
+    const Cut cut = rank_cut(key, u.scored, u.wanted, 0u, 0xffffffffu, s);
     int32_t* out = a.selected + static_cast<size_t>(unit) * a.max_selected + a.keep_first;
     rank_emit(key, u.scored, cut, s, [&](int place, int i) { out[place] = pool_row(a, u, a.keep_first + i); });
 }

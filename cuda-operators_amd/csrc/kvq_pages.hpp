@@ -54,6 +54,7 @@ struct BoundsArgs {
     int8_t* bounds;
     float* scale;
     int B, Hkv, d, max_len;
+    FastDiv heads;  // division by Hkv
 };
 hipError_t launch_page_bounds(const BoundsArgs& a, bool vec_ok, hipStream_t stream);
 

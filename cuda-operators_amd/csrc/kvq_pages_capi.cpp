@@ -27,6 +27,9 @@ bool heads_ok(int num_kv_heads, int head_dim) {
     return num_kv_heads > 0 && head_dim > 0 && head_dim <= KVQ_MAX_HEAD_DIM;
 }
 
+// The tuned bounds kernels address a page's keys with 32-bit offsets.
+bool page_fits(int page_size, int head_dim) { return static_cast<long long>(page_size) * head_dim < (1LL << 30); }
+
 bool dtype_ok(int dtype) { return dtype == KVQ_DTYPE_F32 || dtype == KVQ_DTYPE_BF16; }
 
 kvq::PageMap page_map(const int32_t* table, int size, int max_pages, int num_pages) {
@@ -123,7 +126,7 @@ SparsePlan sparse_plan(const kvq_sparse_decode_params* p) {
         if (kvq_paged_decode_plan(&u, &info) == hipSuccess) s.num_splits = std::max(1, std::min(info.splits, s.max_seq_len / 256));
     }
     r.step_bytes = kvq_paged_decode_workspace_size(&s);
-    r.vec_ok = ((bits(s.k_pages) | bits(p->bounds) | bits(s.q)) & 15u) == 0;
+    r.vec_ok = ((bits(s.k_pages) | bits(p->bounds) | bits(s.q)) & 15u) == 0 && page_fits(s.page_size, s.head_dim);
     r.select = kvq::select_plan(s.batch, s.num_q_heads, s.head_dim, r.vec_ok, (max_len - 1) / s.page_size + 1, p->max_selected);
     // The selection's arrival counters share the workspace's counter prefix with
     // the attention's: the launches are ordered and each leaves them at zero.
@@ -225,7 +228,8 @@ hipError_t kvq_page_bounds_launch(const kvq_page_bounds_params* p, hipStream_t s
         return hipErrorInvalidValue;
     const long long cap = static_cast<long long>(p->max_pages_per_seq) * p->page_size;
     if (cap > INT_MAX || p->max_seq_len > cap || (p->max_seq_len > 0 ? p->max_seq_len : cap) > KVQ_MAX_SEQ_LEN ||
-        static_cast<long long>(p->batch) * p->max_pages_per_seq > INT_MAX)
+        static_cast<long long>(p->batch) * p->max_pages_per_seq > INT_MAX ||
+        static_cast<long long>(p->max_pages_per_seq) * p->num_kv_heads > INT_MAX)
         return hipErrorInvalidValue;
     if (!p->block_table || !p->k_pages || !p->k_scale_pages || !p->bounds || !p->bound_scale) return hipErrorInvalidValue;
     kvq::BoundsArgs a{};
@@ -240,7 +244,8 @@ hipError_t kvq_page_bounds_launch(const kvq_page_bounds_params* p, hipStream_t s
     a.Hkv = p->num_kv_heads;
     a.d = p->head_dim;
     a.max_len = p->max_seq_len > 0 ? p->max_seq_len : static_cast<int>(cap);
-    const bool vec_ok = ((bits(p->k_pages) | bits(p->bounds)) & 15u) == 0;
+    a.heads = kvq::make_fastdiv(static_cast<uint32_t>(p->num_kv_heads));
+    const bool vec_ok = ((bits(p->k_pages) | bits(p->bounds)) & 15u) == 0 && page_fits(p->page_size, p->head_dim);
     return checked_call(stream, [&] { return kvq::launch_page_bounds(a, vec_ok, stream); });
 }
 

@@ -251,7 +251,10 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
     // ranks it if it is ranked.
     if (u.renewed >= 0 && split == active - 1 && wave == 0) {
         constexpr int LPT = bounds_lanes(32 * ND);
-        bounds_wave<LPT>(a.b, kWave / LPT, true, u.b, u.renewed, u.h, a.b.pages.size);
+        const BoundsWave<LPT, Pages::Passes> w(a.b, kWave / LPT);
+        typename BoundsWave<LPT, Pages::Passes>::Piece piece;
+        w.fetch(piece, a.b.pages.table[static_cast<size_t>(u.b) * a.b.pages.max_pages + u.renewed], u.h, a.b.pages.size);
+        w.finish(piece, true);
     }
     if (split == 0) write_kept(a, u, unit);
     if (n == 0) return;

@@ -587,42 +587,49 @@ def prefill(k_new, v_new, k_cache, v_cache, k_scale, v_scale, start=None, unifor
 # ---------------------------------------------------------------------------
 # a paged cache's life on the GPU (include/kvq.h part 7)
 # ---------------------------------------------------------------------------
+def _needs(*specs) -> None:
+    """_need for each (tensor, dtype, shape, name), at a third of its time where all is well."""
+    for t, dtype, shape, name in specs:
+        if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.is_cuda and t.is_contiguous()):
+            _need(t, dtype, shape, name)
+
+
 def _one_device(*tensors):
-    """The device that all of the tensors (None: absent) are on."""
-    device = None
+    """The index of the device that all of the tensors (None: absent) are on."""
+    index = None
     for t in tensors:
-        if t is not None:
-            if device is not None and t.device != device:
-                raise ValueError(f"tensors on {device} and {t.device}")
-            device = t.device
-    return device
+        if t is not None and t.get_device() != index:
+            if index is not None:
+                raise ValueError(f"tensors on devices {index} and {t.get_device()}")
+            index = t.get_device()
+    return index
 
 
-def _call(fn, name, args, device, stream=None) -> None:
-    """One launch on `device`, whichever is current, and on `stream` (default: that device's current stream)."""
-    def launch():
-        handle = stream if isinstance(stream, int) else (stream or torch.cuda.current_stream(device)).cuda_stream
-        _check(name, fn(*args, handle))
+def _call(fn, name, args, index, stream=None) -> None:
+    """One launch on device `index`, whichever is current, and on `stream` (default: that device's current stream)."""
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _call(fn, name, args, index, stream)
+    if stream is None:
+        stream = torch._C._cuda_getCurrentRawStream(index)
+    elif not isinstance(stream, int):
+        stream = stream.cuda_stream
+    code = fn(*args, stream)
+    if code != HIP_SUCCESS:
+        raise KvqError(name, code)
 
-    if device.index is None or device.index == torch.cuda.current_device():
-        launch()
-    else:
-        with torch.cuda.device(device):
-            launch()
 
-
-def _new_workspace(nbytes, device, stream):
+def _new_workspace(nbytes, index, stream):
     """A zeroed workspace that belongs to `stream` (so that memory freed after the last launch there is not handed out
     before that launch ends); None when none is needed."""
     if not nbytes:
         return None
-    with torch.cuda.device(device):
+    with torch.cuda.device(index):
         if isinstance(stream, int):
-            # Not torch's null stream object: an external handle may be any stream of the device.
-            stream = torch.cuda.ExternalStream(stream, device) if stream else torch.cuda.default_stream(device)
-        stream = stream or torch.cuda.current_stream(device)
+            stream = torch.cuda.ExternalStream(stream, index) if stream else torch.cuda.default_stream(index)
+        stream = stream or torch.cuda.current_stream(index)
         with torch.cuda.stream(stream):
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
             workspace_init(ws, nbytes, stream)
     return ws
 
@@ -631,7 +638,7 @@ def _rows_of(t, name, n=None):
     """Entries of a contiguous 1-d int32 cuda tensor (n: that many)."""
     if not isinstance(t, torch.Tensor) or t.dim() != 1:
         raise ValueError(f"{name}: want a 1-d tensor")
-    _need(t, torch.int32, (t.shape[0] if n is None else n,), name)
+    _needs((t, torch.int32, t.shape if n is None else (n,), name))
     return t.shape[0]
 
 
@@ -665,7 +672,7 @@ class PageMapper:
         max_tokens = 2**31 - 1 if max_tokens is None else int(max_tokens)
         self.device = _one_device(new_tokens, lengths, block_table, free_pages, free_count, new_lengths, new_free_count,
                                   granted, token_offsets, slot_map, token_seq, token_pos)
-        empty = lambda n: torch.empty(n, dtype=torch.int32, device=self.device)  # noqa: E731
+        empty = lambda n: torch.empty(n, dtype=torch.int32, device=new_tokens.device)  # noqa: E731
         self.new_tokens, self.lengths, self.block_table = new_tokens, lengths, block_table
         self.free_pages, self.free_count = free_pages, free_count
         self.new_lengths = lengths if new_lengths is None else new_lengths
@@ -693,10 +700,28 @@ def page_map(new_tokens, lengths, block_table, free_pages, free_count, page_size
     return m
 
 
+def _check_pool(k_pages, v_pages, k_scale_pages, v_scale_pages):
+    """A page pool's four tensors; (num_pages, Hkv, page_size, d)."""
+    shape = k_pages.shape
+    if len(shape) != 4:
+        raise ValueError("k_pages: want [num_pages, Hkv, page_size, d]")
+    _needs((k_pages, torch.int8, shape, "k_pages"), (v_pages, torch.int8, shape, "v_pages"),
+           (k_scale_pages, torch.float32, shape[:3], "k_scale_pages"),
+           (v_scale_pages, torch.float32, shape[:3], "v_scale_pages"))
+    return shape
+
+
+def _check_rows(t, dtype, shape, name):
+    if t.dtype is not dtype or t.shape != shape or not t.is_cuda:
+        raise ValueError(f"{name}: want cuda {dtype} {shape}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"{name}: rows must be contiguous, got strides {t.stride()}")
+
+
 def _dtype_code(t, name):
-    if t.dtype == torch.float32:
+    if t.dtype is torch.float32:
         return DTYPE_F32
-    if t.dtype == torch.bfloat16:
+    if t.dtype is torch.bfloat16:
         return DTYPE_BF16
     raise TypeError(f"{name} must be float32 or bfloat16")
 
@@ -706,41 +731,42 @@ def slot_write(k_new, v_new, slots, k_pages, v_pages, k_scale_pages, v_scale_pag
 
     k_new/v_new [T, Hkv, d] fp32 or bf16: a token's heads lie together, tokens may be any stride apart (slices of a
     fused projection); slots [T] int32, -1 (or any outside the pool) for rows that go nowhere."""
-    P_, Hkv, page, d = _check_cache(k_pages, v_pages, k_scale_pages, v_scale_pages, "pages")
+    P_, Hkv, page, d = _check_pool(k_pages, v_pages, k_scale_pages, v_scale_pages)
     T = _rows_of(slots, "slots")
     code = _dtype_code(k_new, "k_new")
-    strides = []
-    for t, n in ((k_new, "k_new"), (v_new, "v_new")):
-        if t.dtype != k_new.dtype or tuple(t.shape) != (T, Hkv, d) or t.device.type != "cuda":
-            raise ValueError(f"{n}: want cuda {k_new.dtype} {(T, Hkv, d)}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-        if (d > 1 and t.stride(2) != 1) or (Hkv > 1 and t.stride(1) != d) or (T > 1 and t.stride(0) < Hkv * d):
-            raise ValueError(f"{n}: a token's heads must lie together, got strides {t.stride()}")
-        strides.append(t.stride(0) if T > 1 else 0)
-    device = _one_device(k_new, v_new, slots, k_pages, v_pages, k_scale_pages, v_scale_pages)
+    _check_rows(k_new, k_new.dtype, (T, Hkv, d), "k_new")
+    _check_rows(v_new, k_new.dtype, (T, Hkv, d), "v_new")
+    ks, vs = k_new.stride(), v_new.stride()
+    for s, n in ((ks, "k_new"), (vs, "v_new")):
+        if (Hkv > 1 and s[1] != d) or (T > 1 and s[0] < Hkv * d):
+            raise ValueError(f"{n}: a token's heads must lie together, got strides {s}")
+    index = _one_device(k_new, v_new, slots, k_pages, v_pages, k_scale_pages, v_scale_pages)
     if T == 0:
         return
-    p = SlotWriteParams(T, Hkv, d, page, P_, code, _ptr(k_new), _ptr(v_new), *strides, _ptr(slots), _ptr(k_pages),
-                        _ptr(v_pages), _ptr(k_scale_pages), _ptr(v_scale_pages))
-    _call(lib().kvq_slot_write_launch, "kvq_slot_write_launch", (ctypes.byref(p),), device, stream)
+    p = SlotWriteParams(T, Hkv, d, page, P_, code, k_new.data_ptr(), v_new.data_ptr(), ks[0] if T > 1 else 0,
+                        vs[0] if T > 1 else 0, slots.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                        k_scale_pages.data_ptr(), v_scale_pages.data_ptr())
+    _call(lib().kvq_slot_write_launch, "kvq_slot_write_launch", (ctypes.byref(p),), index, stream)
 
 
 def slot_read(slots, k_pages, v_pages, k_scale_pages, v_scale_pages, k_out, v_out, stream=None):
     """Cached rows as numbers (kvq_slot_read_launch): slots [T] int32 into k_out/v_out [T, Hkv, d] fp32 or bf16, each of
     the same strides (a transposed [Hkv, T, d] too); returns (k_out, v_out)."""
-    P_, Hkv, page, d = _check_cache(k_pages, v_pages, k_scale_pages, v_scale_pages, "pages")
+    P_, Hkv, page, d = _check_pool(k_pages, v_pages, k_scale_pages, v_scale_pages)
     T = _rows_of(slots, "slots")
     code = _dtype_code(k_out, "k_out")
-    for t, n in ((k_out, "k_out"), (v_out, "v_out")):
-        if t.dtype != k_out.dtype or tuple(t.shape) != (T, Hkv, d) or t.device.type != "cuda":
-            raise ValueError(f"{n}: want cuda {k_out.dtype} {(T, Hkv, d)}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-        if (d > 1 and t.stride(2) != 1) or t.stride()[:2] != k_out.stride()[:2]:
-            raise ValueError(f"{n}: rows must be contiguous and both outputs alike, got strides {t.stride()}")
-    device = _one_device(slots, k_pages, v_pages, k_scale_pages, v_scale_pages, k_out, v_out)
+    _check_rows(k_out, k_out.dtype, (T, Hkv, d), "k_out")
+    _check_rows(v_out, k_out.dtype, (T, Hkv, d), "v_out")
+    strides = k_out.stride()
+    if v_out.stride()[:2] != strides[:2]:
+        raise ValueError(f"k_out and v_out must have the same strides, got {strides} and {v_out.stride()}")
+    index = _one_device(slots, k_pages, v_pages, k_scale_pages, v_scale_pages, k_out, v_out)
     if T == 0:
         return k_out, v_out
-    p = SlotReadParams(T, Hkv, d, page, P_, code, _ptr(slots), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale_pages),
-                       _ptr(v_scale_pages), _ptr(k_out), _ptr(v_out), k_out.stride(0), k_out.stride(1))
-    _call(lib().kvq_slot_read_launch, "kvq_slot_read_launch", (ctypes.byref(p),), device, stream)
+    p = SlotReadParams(T, Hkv, d, page, P_, code, slots.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                       k_scale_pages.data_ptr(), v_scale_pages.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
+                       strides[0], strides[1])
+    _call(lib().kvq_slot_read_launch, "kvq_slot_read_launch", (ctypes.byref(p),), index, stream)
     return k_out, v_out
 
 
@@ -751,32 +777,23 @@ def new_bounds(k_pages):
             torch.zeros((P_, Hkv), dtype=torch.float32, device=k_pages.device))
 
 
-def _check_bounds(bounds, bound_scale, P_, Hkv, d):
-    _need(bounds, torch.int8, (P_, Hkv, 2, d), "bounds")
-    _need(bound_scale, torch.float32, (P_, Hkv), "bound_scale")
-
-
 def page_bounds(k_pages, k_scale_pages, block_table, lengths, bounds, bound_scale, start=None, max_seq_len=0,
                 stream=None) -> None:
     """Key bounds of the pages that hold tokens [start_b, lengths_b) (kvq_page_bounds_launch).
 
     bounds [num_pages, Hkv, 2, d] int8, bound_scale [num_pages, Hkv] fp32 (new_bounds); start [B] int32 or None."""
-    P_, Hkv, page, d = k_pages.shape
-    _need(k_pages, torch.int8, (P_, Hkv, page, d), "k_pages")
-    _need(k_scale_pages, torch.float32, (P_, Hkv, page), "k_scale_pages")
-    _check_bounds(bounds, bound_scale, P_, Hkv, d)
-    if block_table.dim() != 2:
-        raise ValueError("block_table: want [B, max_pages_per_seq]")
-    B = block_table.shape[0]
-    _need(block_table, torch.int32, tuple(block_table.shape), "block_table")
+    P_, Hkv, page, d = shape = k_pages.shape
+    B, per = block_table.shape
+    _needs((k_pages, torch.int8, shape, "k_pages"), (k_scale_pages, torch.float32, shape[:3], "k_scale_pages"),
+           (bounds, torch.int8, (P_, Hkv, 2, d), "bounds"), (bound_scale, torch.float32, (P_, Hkv), "bound_scale"),
+           (block_table, torch.int32, (B, per), "block_table"))
     for t, n in ((start, "start"), (lengths, "lengths")):
         if t is not None:
-            _rows_of(t, n, B)
-    device = _one_device(k_pages, k_scale_pages, block_table, lengths, bounds, bound_scale, start)
-    p = PageBoundsParams(B, Hkv, d, page, P_, int(block_table.shape[1]), int(max_seq_len), _ptr(block_table),
-                         _ptr(start), _ptr(lengths), _ptr(k_pages), _ptr(k_scale_pages), _ptr(bounds),
-                         _ptr(bound_scale))
-    _call(lib().kvq_page_bounds_launch, "kvq_page_bounds_launch", (ctypes.byref(p),), device, stream)
+            _needs((t, torch.int32, (B,), n))
+    index = _one_device(k_pages, k_scale_pages, block_table, lengths, bounds, bound_scale, start)
+    p = PageBoundsParams(B, Hkv, d, page, P_, per, int(max_seq_len), block_table.data_ptr(), _ptr(start), _ptr(lengths),
+                         k_pages.data_ptr(), k_scale_pages.data_ptr(), bounds.data_ptr(), bound_scale.data_ptr())
+    _call(lib().kvq_page_bounds_launch, "kvq_page_bounds_launch", (ctypes.byref(p),), index, stream)
 
 
 class SparseDecoder:
@@ -791,7 +808,7 @@ class SparseDecoder:
         check_paged(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, lengths, out, k_new, v_new)
         B, Hq, d = q.shape
         P_, Hkv, page, _ = k_pages.shape
-        _check_bounds(bounds, bound_scale, P_, Hkv, d)
+        _needs((bounds, torch.int8, (P_, Hkv, 2, d), "bounds"), (bound_scale, torch.float32, (P_, Hkv), "bound_scale"))
         if selected.dim() != 3:
             raise ValueError("selected: want [B, Hkv, max_selected]")
         _need(selected, torch.int32, (B, Hkv, selected.shape[2]), "selected")

@@ -480,7 +480,7 @@ hipError_t kvq_slot_read_launch(const kvq_slot_read_params* p, hipStream_t strea
 
 typedef struct kvq_page_bounds_params {
     int batch, num_kv_heads, head_dim;
-    int page_size, num_pages, max_pages_per_seq;
+    int page_size, num_pages, max_pages_per_seq; /* max_pages_per_seq * num_kv_heads must fit an int */
     int max_seq_len;            /* as kvq_paged_decode_params */
     const int32_t* block_table; /* device [B, max_pages_per_seq] */
     const int32_t* start;       /* device [B]: first token whose page is to be done (clamped at 0), or NULL: 0 */

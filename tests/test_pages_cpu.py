@@ -118,7 +118,7 @@ def test_slot_read_refuses(bad):
 @pytest.mark.parametrize("bad", [
     dict(batch=0), dict(num_kv_heads=0), dict(head_dim=0), dict(head_dim=4097), dict(page_size=0), dict(num_pages=0),
     dict(max_pages_per_seq=0), dict(max_pages_per_seq=1 << 28), dict(max_seq_len=-1), dict(max_seq_len=65),
-    dict(lengths=None), dict(page_size=1 << 26, max_pages_per_seq=17), dict(batch=1 << 30)] +
+    dict(lengths=None), dict(page_size=1 << 26, max_pages_per_seq=17), dict(batch=1 << 30), dict(num_kv_heads=1 << 30)] +
     [{n: None} for n in ("block_table", "k_pages", "k_scale_pages", "bounds", "bound_scale")])
 def test_page_bounds_refuses(bad):
     assert launch("kvq_page_bounds_launch", bounds_params(**bad)) == INVALID

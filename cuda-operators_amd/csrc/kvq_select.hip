@@ -36,13 +36,36 @@ __device__ __forceinline__ unsigned rank_key(float score) {
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
+// The largest and smallest of a wave's unsigned values (the steps of
+// wave_inclusive_scan; lanes shifted in from outside a row give 0).
+__device__ __forceinline__ unsigned wave_max_u32(unsigned x) {
+    int v = static_cast<int>(x);
+#define KVQ_STEP(CTRL, ROWS) \
+    v = static_cast<int>(max(static_cast<unsigned>(v), static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false))));
+    KVQ_STEP(0x111, 0xF)
+    KVQ_STEP(0x112, 0xF)
+    KVQ_STEP(0x114, 0xF)
+    KVQ_STEP(0x118, 0xF)
+    KVQ_STEP(0x142, 0xA)
+    KVQ_STEP(0x143, 0xC)
+#undef KVQ_STEP
+    return static_cast<unsigned>(__builtin_amdgcn_readlane(v, kWave - 1));
+}
+__device__ __forceinline__ unsigned wave_min_u32(unsigned x) { return ~wave_max_u32(~x); }
+
+constexpr int kSelList = kWave;  // keys of one bin that a wave ranks by comparing each with each
 struct RankScratch {
-    unsigned hist[kSelBins];
+    unsigned hist[kSelBins];  // zero whenever rank_cut begins (clear_bins)
+    unsigned list[kSelList];
     unsigned lo[kSelWaves], hi[kSelWaves];
     int sums[kSelWaves];
     int gt[kSelWaves], eq[kSelWaves];
-    int bin, above, count;
+    int bin, above, count, listed;
 };
+__device__ __forceinline__ void clear_bins(RankScratch& s) {
+    for (int i = threadIdx.x; i < kSelBins; i += kSelThreads) s.hist[i] = 0;
+    if (threadIdx.x == 0) s.listed = 0;
+}
 
 // The keys above `key`, and the first `ties` of those equal to it.
 struct Cut {
@@ -58,11 +81,8 @@ __device__ inline Cut rank_cut(const Key& key, int n, int k, unsigned lo, unsign
     const int t = threadIdx.x;
     const int lane = t & (kWave - 1);
     const int wave = t / kWave;
-#pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) {
-        lo = min(lo, static_cast<unsigned>(__shfl_xor(static_cast<int>(lo), off)));
-        hi = max(hi, static_cast<unsigned>(__shfl_xor(static_cast<int>(hi), off)));
-    }
+    lo = wave_min_u32(lo);
+    hi = wave_max_u32(hi);
     if (lane == 0) {
         s.lo[wave] = lo;
         s.hi[wave] = hi;
@@ -74,13 +94,11 @@ __device__ inline Cut rank_cut(const Key& key, int n, int k, unsigned lo, unsign
         hi = max(hi, s.hi[w]);
     }
     // The k largest keys of [lo, hi] are wanted; every round leaves a bin of the
-    // last one's range, at most a 2048th of it, so three rounds end it.
+    // last one's range, at most a 2048th of it, so three rounds end it.  As a
+    // rule the first leaves a few keys, which every wave ranks for itself.
     for (;;) {
         if (lo == hi) return Cut{lo, k};
         const int shift = max(0, 32 - __clz(static_cast<int>(hi - lo)) - kSelLogBins);
-        __syncthreads();
-        for (int i = t; i < kSelBins; i += kSelThreads) s.hist[i] = 0;
-        __syncthreads();
         for (int i = t; i < n; i += kSelThreads) {
             const unsigned x = key(i);
             if (x >= lo && x <= hi) atomicAdd(&s.hist[(x - lo) >> shift], 1u);
@@ -89,26 +107,54 @@ __device__ inline Cut rank_cut(const Key& key, int n, int k, unsigned lo, unsign
         // Thread t sums bins from the top: [2047 - 4 t - 3, 2047 - 4 t].
         constexpr int kPer = kSelBins / kSelThreads;
         const int top = kSelBins - 1 - t * kPer;
-        int sum = 0;
+        int bins[kPer], sum = 0;
 #pragma unroll
-        for (int j = 0; j < kPer; j++) sum += static_cast<int>(s.hist[top - j]);
+        for (int j = 0; j < kPer; j++) sum += bins[j] = static_cast<int>(s.hist[top - j]);
         const int incl_wave = wave_inclusive_scan(sum);
         if (lane == kWave - 1) s.sums[wave] = incl_wave;
         __syncthreads();
         int above = incl_wave - sum;
-        for (int w = 0; w < wave; w++) above += s.sums[w];
+#pragma unroll
+        for (int w = 0; w < kSelWaves; w++) above += w < wave ? s.sums[w] : 0;
         if (above < k && k <= above + sum) {
-            int j = 0;
-            while (j < kPer - 1 && above + static_cast<int>(s.hist[top - j]) < k) above += static_cast<int>(s.hist[top - j++]);
-            s.bin = top - j;
-            s.above = above;
-            s.count = static_cast<int>(s.hist[top - j]);
+            bool found = false;
+#pragma unroll
+            for (int j = 0; j < kPer; j++) {
+                if (!found && k <= above + bins[j]) {
+                    found = true;
+                    s.bin = top - j;
+                    s.above = above;
+                    s.count = bins[j];
+                }
+                above += bins[j];
+            }
         }
         __syncthreads();
         lo += static_cast<unsigned>(s.bin) << shift;
         k -= s.above;
-        if (k == s.count) return Cut{lo, INT_MAX};  // the whole bin
+        const int count = s.count;
+        if (k == count) return Cut{lo, INT_MAX};  // the whole bin
         if (hi - lo > (1u << shift) - 1u) hi = lo + ((1u << shift) - 1u);
+        if (count <= kSelList) {
+            for (int i = t; i < n; i += kSelThreads) {
+                const unsigned x = key(i);
+                if (x >= lo && x <= hi) s.list[atomicAdd(&s.listed, 1)] = x;
+            }
+            __syncthreads();
+            const unsigned mine = lane < count ? s.list[lane] : 0;
+            int more = 0, same = 0;  // keys above this lane's, and equal ones
+            for (int j = 0; j < count; j++) {
+                const unsigned x = static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(mine), j));
+                more += x > mine;
+                same += x == mine;
+            }
+            const unsigned long long at = __builtin_amdgcn_ballot_w64(lane < count && more < k && k <= more + same);
+            const int l = __builtin_ctzll(at);  // a lane with the k-th key: there is one
+            return Cut{static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(mine), l)),
+                       k - __builtin_amdgcn_readlane(more, l)};
+        }
+        for (int i = t; i < kSelBins; i += kSelThreads) s.hist[i] = 0;
+        __syncthreads();
     }
 }
 
@@ -198,8 +244,8 @@ __device__ inline void write_kept(const SelectArgs& a, const Unit& u, int unit) 
 // head's max(c, 0) and min(c, 0) as one column of 2 d bytes, sixteen pages times
 // sixteen heads are ND = 2 d / 64 int8 matrix products.  The rows come straight
 // from memory into the A operand (16 bytes a lane, four lanes a 64-byte piece),
-// the columns from LDS; columns past the last head repeat one, and bytes past
-// 2 d are zero in the columns.  Reading the bounds is all that costs: 16 pages
+// the columns from LDS; columns past the last head are left out of the maximum,
+// and bytes past 2 d are zero in the columns.  Reading the bounds is all that costs: 16 pages
 // a wave at a time, the next 16 on their way, their ids one step further ahead.
 //
 // A unit's pages go to `splits` workgroups in whole steps of 128; the last one
@@ -256,8 +302,10 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
         w.fetch(piece, a.b.pages.table[static_cast<size_t>(u.b) * a.b.pages.max_pages + u.renewed], u.h, a.b.pages.size);
         w.finish(piece, true);
     }
-    if (split == 0) write_kept(a, u, unit);
-    if (n == 0) return;
+    if (n == 0) {
+        write_kept(a, u, unit);
+        return;
+    }
 
     const int r = lane & 15, c16 = (lane >> 4) * 16;
     auto row_of = [&](int i) { return static_cast<size_t>(pool_row(a, u, a.keep_first + min(i, i1 - 1))); };
@@ -277,34 +325,42 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
     const bool renews = u.renewed >= 0 && split == active - 1;
     if (!renews) load(row0, next, next_scale);
 
-    // The heads' codes.
-    const float* q = a.q + static_cast<size_t>(unit) * a.G * d;
-    float amax = 0.0f;
-    for (int i = t; i < a.G * d / 4; i += kSelThreads) {
-        const float4 x = reinterpret_cast<const float4*>(q)[i];
-        amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-    }
-    amax = wave_max(amax);
+    // The heads' codes: four of one head a thread, once into the highs' half of
+    // its column (those above zero) and once into the lows' half (those below).
+    const float4* q = reinterpret_cast<const float4*>(a.q + static_cast<size_t>(unit) * a.G * d);
+    const int quads = a.G * d / 4;
+    const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float4 mine = t < quads ? q[t] : zero;
+    auto largest = [](const float4& x) { return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))); };
+    float amax = largest(mine);
+    for (int i = t + kSelThreads; i < quads; i += kSelThreads) amax = fmaxf(amax, largest(q[i]));
+    amax = __uint_as_float(wave_max_u32(__float_as_uint(amax)));  // not negative, so ordered as its bits; never NaN
     if (lane == 0) s_max[wave] = amax;
+    clear_bins(s);
+    int* columns = reinterpret_cast<int*>(s_dyn);
+    auto word = [&](int g, int off) {  // of byte `off` of head g's column
+        return (((g >> 4) * ND + (off >> 6)) * 64 + ((off >> 4) & 3) * 16 + (g & 15)) * 4 + ((off >> 2) & 3);
+    };
+    if (2 * d < ND * 64)  // what a column has behind its end
+        for (int i = t; i < a.G * (ND * 64 - 2 * d) / 4; i += kSelThreads) {
+            const int per = (ND * 64 - 2 * d) / 4;
+            columns[word(i / per, 2 * d + (i % per) * 4)] = 0;
+        }
     __syncthreads();  // and the renewed bounds are written
 #pragma unroll
     for (int w = 0; w < kSelWaves; w++) amax = fmaxf(amax, s_max[w]);
     const float qs = quant_scale(amax);
-    for (int w = t; w < passes * ND * 256; w += kSelThreads) {
-        const int col = (w >> 2) & 63;  // operand lane
-        const int step = (w >> 8) % ND, pass = (w >> 8) / ND;
-        const int off = step * 64 + (col >> 4) * 16 + (w & 3) * 4;
-        const int g = pass * 16 + (col & 15);
-        int c[4] = {0, 0, 0, 0};
-        if (off < 2 * d) {
-            const float4 x = *reinterpret_cast<const float4*>(q + static_cast<size_t>(g < a.G ? g : pass * 16) * d + (off < d ? off : off - d));
-            const float y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) c[j] = off < d ? max(quant_one(y[j], qs), 0) : min(quant_one(y[j], qs), 0);
-        }
-        reinterpret_cast<int*>(s_dyn)[w] = pack4(c[0], c[1], c[2], c[3]);
+    for (int i = t; i < quads; i += kSelThreads) {
+        const float4 x = i == t ? mine : q[i];
+        const float y[4] = {x.x, x.y, x.z, x.w};
+        int c[4];
+        quant_row<4>(y, qs, c);
+        const int g = 4 * i / d, off = 4 * i - g * d;
+        columns[word(g, off)] = pack4(max(c[0], 0), max(c[1], 0), max(c[2], 0), max(c[3], 0));
+        columns[word(g, d + off)] = pack4(min(c[0], 0), min(c[1], 0), min(c[2], 0), min(c[3], 0));
     }
     __syncthreads();
+    if (split == 0) write_kept(a, u, unit);
 
     const bool shared = active > 1 || n > lds_keys;  // keys in memory
     unsigned* keys = shared ? a.keys + static_cast<size_t>(unit) * a.key_stride : nullptr;
@@ -325,8 +381,10 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
                 const i32x4 y = reinterpret_cast<const i32x4*>(s_dyn)[(pass * ND + j) * 64 + lane];
                 acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[j], y, acc, 0, 0, 0);
             }
+            if (pass * 16 + r < a.G) {  // columns past the last head hold anything
 #pragma unroll
-            for (int i = 0; i < 4; i++) top[i] = max(top[i], acc[i]);
+                for (int i = 0; i < 4; i++) top[i] = max(top[i], acc[i]);
+            }
         }
         // Lane 16 g + c holds pages 4 g .. 4 g + 3 of head c; lanes c < 4 write page 4 g + c.
 #pragma unroll
@@ -391,6 +449,7 @@ __global__ __launch_bounds__(kSelThreads) void select_generic(const SelectArgs a
     for (int i = threadIdx.x; i < a.G * d; i += kSelThreads) amax = fmaxf(amax, fabsf(q[i]));
     amax = wave_max(amax);
     if (lane == 0) s_max[wave] = amax;
+    clear_bins(s);
     __syncthreads();  // and the renewed bounds are written
 #pragma unroll
     for (int w = 0; w < kSelWaves; w++) amax = fmaxf(amax, s_max[w]);
@@ -431,10 +490,13 @@ SelectPlan select_plan(int units, int G, int d, bool vec_ok, int max_pages, int 
     SelectPlan p{1, 0, 0, 0};
     if (max_pages <= max_selected) return p;
     if (vec_ok && select_tuned(G, d)) {
-        // About two workgroups a CU, each with at least one step of pages.
+        // About two workgroups a CU, each with at least one step of pages; units
+        // that fill the CUs alone are not split (whole steps: 2048 pages of 8
+        // units 22.1 us in 16 parts, 24.2 in 4, 28.3 in 2; 1024 pages of 128 units
+        // 42.6 us in 4 parts, 43.5 in 2, 44.8 in one; of 256 units 45.6 in 2, 44.4 in
+        // one).
         const long steps = (static_cast<long>(max_pages) + kSelStep - 1) / kSelStep;
-        if (units <= static_cast<int>(kCounterBytes / sizeof(int)))
-            p.splits = static_cast<int>(std::max(1L, std::min(steps, 512L / units)));
+        if (units < 256) p.splits = static_cast<int>(std::min(steps, 512L / units));
         p.lds_keys = max_pages <= kSelLdsKeys ? max_pages : 0;
         if (p.splits == 1 && p.lds_keys > 0) return p;
     }

@@ -35,15 +35,25 @@ __device__ __forceinline__ int pages_of(int tokens, const FastDiv& page) {
     return static_cast<int>(fastdiv(static_cast<uint32_t>(tokens) + page.d - 1, page));
 }
 
-// The last i in [0, n) with v[i] <= x, for ascending v with v[0] <= x.
-__device__ __forceinline__ int last_not_above(const int* v, int n, int x) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (v[mid] <= x) lo = mid;
-        else hi = mid;
+// For each x the last i in [0, n) with v[i] <= x, for ascending v with v[0] <= x;
+// the K searches' loads go out together.
+template <int K>
+__device__ __forceinline__ void last_not_above(const int* v, int n, const int (&x)[K], int (&at)[K]) {
+#pragma unroll
+    for (int k = 0; k < K; k++) at[k] = 0;
+    for (int step = 1 << (31 - __clz(n)); step > 0; step >>= 1) {
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int i = at[k] + step;
+            if (i < n && v[min(i, n - 1)] <= x[k]) at[k] = i;
+        }
     }
-    return lo;
+}
+__device__ __forceinline__ int last_not_above(const int* v, int n, int x) {
+    const int xs[1] = {x};
+    int at[1];
+    last_not_above<1>(v, n, xs, at);
+    return at[0];
 }
 
 // Inclusive scans of K values a thread over the workgroup, and their totals;
@@ -155,12 +165,15 @@ __global__ __launch_bounds__(kMapThreads) void page_map_kernel(const PageMapArgs
     for (int w = 0; w < kMapWaves; w++) A = max(A, s_taken[w]);
     const long long left = have - A;  // entries of the stack afterwards
 
-    auto given_up = [&](int g) {  // the g-th page given up
-        const int c = last_not_above(s_gives, B, g);
+    auto given_up = [&](int g, int c) {  // the g-th page given up, by sequence c
         const int end = pages_of(s_old[c], a.page);  // a shrinking sequence is not refused
         return a.table[static_cast<size_t>(c) * a.max_pages + end - (s_gives[c + 1] - s_gives[c]) + (g - s_gives[c])];
     };
-    auto stack_at = [&](long long i) { return i < F ? a.free_pages[i] : given_up(static_cast<int>(i - F)); };
+    auto stack_at = [&](long long i) {
+        if (i < F) return a.free_pages[i];
+        const int g = static_cast<int>(i - F);
+        return given_up(g, last_not_above(s_gives, B, g));
+    };
 
     // Each job begins at another third of the threads, so that small ones run at
     // the same time in different waves instead of one load after the other.
@@ -175,9 +188,12 @@ __global__ __launch_bounds__(kMapThreads) void page_map_kernel(const PageMapArgs
     const long long back = min(left, static_cast<long long>(a.num_pages)) - F;  // pages given up that stay on the stack
     constexpr int kBack = 4;  // loads in flight
     for (long long i = me < third ? me - third + step : me - third; i < back; i += static_cast<long long>(kBack) * step) {
-        int id[kBack];
+        int g[kBack], c[kBack], id[kBack];
 #pragma unroll
-        for (int k = 0; k < kBack; k++) id[k] = given_up(static_cast<int>(min(i + static_cast<long long>(k) * step, back - 1)));
+        for (int k = 0; k < kBack; k++) g[k] = static_cast<int>(min(i + static_cast<long long>(k) * step, back - 1));
+        last_not_above<kBack>(s_gives, B, g, c);
+#pragma unroll
+        for (int k = 0; k < kBack; k++) id[k] = given_up(g[k], c[k]);
 #pragma unroll
         for (int k = 0; k < kBack; k++)
             if (i + static_cast<long long>(k) * step < back) a.free_pages[F + i + static_cast<long long>(k) * step] = id[k];
@@ -254,35 +270,27 @@ __device__ __forceinline__ float row_elem(const void* x, int64_t i) {
     else return static_cast<const float*>(x)[i];
 }
 
-#ifndef KVQ_SLOT_NT
-#define KVQ_SLOT_NT 9
-#endif
-typedef int v2i_t __attribute__((ext_vector_type(2)));
-template <bool NT, class T>
-__device__ __forceinline__ T stream_load(const void* p) {
-    typedef int V __attribute__((ext_vector_type(sizeof(T) / 4)));
-    if constexpr (NT) return __builtin_bit_cast(T, __builtin_nontemporal_load(static_cast<const V*>(p)));
-    else return *static_cast<const T*>(p);
-}
-template <bool NT, class T>
-__device__ __forceinline__ void stream_store(void* p, T x) {
-    if constexpr (NT) __builtin_nontemporal_store(x, static_cast<T*>(p));
-    else *static_cast<T*>(p) = x;
-}
-
 // Tuned rows: LPR lanes a row with 16 bytes of it each (fp32: 4 elements, bf16:
 // 8), U loads in flight a lane.  A wave takes U * RPW consecutive tokens of one
 // kv head: in the pool these are as a rule consecutive rows of a page, so its
 // codes and scales go out (or come in) in whole cache lines, while neighbouring
 // waves take the other heads of the same tokens, whose packed rows lie beside.
+// The packed side streams past the caches.  Bound by the mixed stream of reads
+// and writes (a large copy moves 4.8 TB/s): writes of 24,560 tokens, 8 heads, d =
+// 128 and bf16 34 us out of a fused projection (4.5 TB/s; U = 1 35 us, 4 39 us, 8
+// 42 us; without streaming loads 46 us at U = 4), 30 us packed, fp32 47 us packed
+// (5.3 TB/s); reads of 98,304 tokens as bf16 113 us (5.4 TB/s; U = 2 134 us, 4
+// 120 us; without streaming stores 2 us more).  A small read is bound by its
+// chain of loads, and shorter waves are done sooner: 4099 tokens as fp32 7.4 us
+// at U = 2, 8.4 at 8.
 // PAD: a row of d < D elements, whole 16-byte pieces; the lanes past its last
 // piece read that piece again and store nothing.
-template <int D, bool BF16>
+template <int D, bool BF16, int LOADS>
 struct SlotGeom {
     static constexpr int EPL = BF16 ? 8 : 4;  // elements a lane
     static constexpr int LPR = D / EPL;       // lanes a row
     static constexpr int RPW = kWave / LPR;   // rows a wave load
-    static constexpr int U = BF16 ? 4 : 8;
+    static constexpr int U = LOADS;
     static constexpr int TB = RPW * U;        // tokens a wave
     static_assert(LPR >= 1 && LPR <= kWave && kWave % LPR == 0, "row geometry");
 };
@@ -297,9 +305,11 @@ __device__ __forceinline__ bool slot_unit(const SlotArgs& a, int tb, int& t0, in
     return first < a.T;
 }
 
+constexpr int kWriteLoads = 2, kReadLoads = 8, kSmallReadLoads = 2;
+
 template <int D, bool BF16, bool PAD>
 __global__ __launch_bounds__(kSlotWaves* kWave) void slot_write_kernel(const SlotArgs a) {
-    using Geo = SlotGeom<D, BF16>;
+    using Geo = SlotGeom<D, BF16, kWriteLoads>;
     constexpr int EPL = Geo::EPL, LPR = Geo::LPR, RPW = Geo::RPW, U = Geo::U;
     int t0, h;
     if (!slot_unit(a, Geo::TB, t0, h)) return;
@@ -318,7 +328,8 @@ __global__ __launch_bounds__(kSlotWaves* kWave) void slot_write_kernel(const Slo
 #pragma unroll
     for (int u = 0; u < U; u++) {  // a token past the end reads the last one again and is dropped
         const int tc = min(t0 + u * RPW + lane / LPR, a.T - 1);
-        raw[u] = stream_load<(KVQ_SLOT_NT & 1) != 0, int4>(x + tc * stride * (BF16 ? 2 : 4));
+        const v4i_t w = __builtin_nontemporal_load(reinterpret_cast<const v4i_t*>(x + tc * stride * (BF16 ? 2 : 4)));
+        raw[u] = make_int4(w.x, w.y, w.z, w.w);
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -344,15 +355,15 @@ __global__ __launch_bounds__(kSlotWaves* kWave) void slot_write_kernel(const Slo
         quant_row<EPL>(e, scale, qv);
         int8_t* o = qo + orow[u] * d + ls * EPL;
         if constexpr (BF16)
-            stream_store<(KVQ_SLOT_NT & 2) != 0>(o, v2i_t{pack4(qv[0], qv[1], qv[2], qv[3]), pack4(qv[4], qv[5], qv[6], qv[7])});
-        else stream_store<(KVQ_SLOT_NT & 2) != 0>(o, pack4(qv[0], qv[1], qv[2], qv[3]));
+            *reinterpret_cast<int2*>(o) = make_int2(pack4(qv[0], qv[1], qv[2], qv[3]), pack4(qv[4], qv[5], qv[6], qv[7]));
+        else *reinterpret_cast<int*>(o) = pack4(qv[0], qv[1], qv[2], qv[3]);
         if (ls == 0) so[orow[u]] = scale;
     }
 }
 
-template <int D, bool BF16, bool PAD>
+template <int D, bool BF16, bool PAD, int LOADS>
 __global__ __launch_bounds__(kSlotWaves* kWave) void slot_read_kernel(const SlotArgs a) {
-    using Geo = SlotGeom<D, BF16>;
+    using Geo = SlotGeom<D, BF16, LOADS>;
     constexpr int EPL = Geo::EPL, LPR = Geo::LPR, RPW = Geo::RPW, U = Geo::U;
     int t0, h;
     if (!slot_unit(a, Geo::TB, t0, h)) return;
@@ -375,8 +386,8 @@ __global__ __launch_bounds__(kSlotWaves* kWave) void slot_read_kernel(const Slot
     for (int u = 0; u < U; u++) {
         const long long r = max(irow[u], 0LL);  // a row that is nowhere reads the pool's first and gives zeros
         const int8_t* p = qi + r * d + ls * EPL;
-        if constexpr (BF16) raw[u] = stream_load<(KVQ_SLOT_NT & 4) != 0, int2>(p);
-        else raw[u] = make_int2(stream_load<(KVQ_SLOT_NT & 4) != 0, int>(p), 0);
+        if constexpr (BF16) raw[u] = *reinterpret_cast<const int2*>(p);
+        else raw[u] = make_int2(*reinterpret_cast<const int*>(p), 0);
         scale[u] = si[r];
     }
 #pragma unroll
@@ -392,7 +403,7 @@ __global__ __launch_bounds__(kSlotWaves* kWave) void slot_read_kernel(const Slot
             if constexpr (BF16) out[i] = static_cast<int>(bf16_of(y[2 * i]) | (static_cast<unsigned>(bf16_of(y[2 * i + 1])) << 16));
             else out[i] = __float_as_int(y[i]);
         }
-        stream_store<(KVQ_SLOT_NT & 8) != 0>(x + t * stride * (BF16 ? 2 : 4), out);
+        __builtin_nontemporal_store(out, reinterpret_cast<v4i_t*>(x + t * stride * (BF16 ? 2 : 4)));
     }
 }
 
@@ -559,22 +570,29 @@ hipError_t launch_slots(const SlotArgs& a, bool write, bool vec_ok, hipStream_t 
     const dim3 block(kSlotWaves * kWave);
     // Rows of whole 16-byte pieces up to 256 elements; others, and misaligned
     // ones, go to the generic kernels.
-    if (vec_ok && a.d <= 256 && a.d % SlotGeom<256, BF16>::EPL == 0) {
-#define KVQ_SLOT_CASE(DD)                                                                                        \
-    if (a.d <= DD) {                                                                                             \
-        const long long units = (static_cast<long long>(a.T) + SlotGeom<DD, BF16>::TB - 1) / SlotGeom<DD, BF16>::TB * a.Hkv; \
-        const dim3 grid(static_cast<unsigned>((units + kSlotWaves - 1) / kSlotWaves), 2);                        \
-        if (write && a.d == DD) hipLaunchKernelGGL((slot_write_kernel<DD, BF16, false>), grid, block, 0, stream, a); \
-        else if (write) hipLaunchKernelGGL((slot_write_kernel<DD, BF16, true>), grid, block, 0, stream, a);      \
-        else if (a.d == DD) hipLaunchKernelGGL((slot_read_kernel<DD, BF16, false>), grid, block, 0, stream, a);  \
-        else hipLaunchKernelGGL((slot_read_kernel<DD, BF16, true>), grid, block, 0, stream, a);                  \
-        return hipGetLastError();                                                                                \
+    if (vec_ok && a.d <= 256 && a.d % (BF16 ? 8 : 4) == 0) {
+        auto units = [&](int tb) { return (static_cast<long long>(a.T) + tb - 1) / tb * a.Hkv; };  // waves of K or of V
+        auto grid = [&](int tb) { return dim3(static_cast<unsigned>((units(tb) + kSlotWaves - 1) / kSlotWaves), 2); };
+#define KVQ_SLOT_LAUNCH(KERNEL, LOADS) \
+    hipLaunchKernelGGL(KERNEL, grid(SlotGeom<DD, BF16, LOADS>::TB), block, 0, stream, a)
+#define KVQ_SLOT_CASE(DIM)                                                                                             \
+    if (a.d <= DIM) {                                                                                                  \
+        constexpr int DD = DIM;                                                                                        \
+        const bool few = units(SlotGeom<DD, BF16, kReadLoads>::TB) < 4096;                                             \
+        if (write && a.d == DD) KVQ_SLOT_LAUNCH((slot_write_kernel<DD, BF16, false>), kWriteLoads);                    \
+        else if (write) KVQ_SLOT_LAUNCH((slot_write_kernel<DD, BF16, true>), kWriteLoads);                             \
+        else if (few && a.d == DD) KVQ_SLOT_LAUNCH((slot_read_kernel<DD, BF16, false, kSmallReadLoads>), kSmallReadLoads); \
+        else if (few) KVQ_SLOT_LAUNCH((slot_read_kernel<DD, BF16, true, kSmallReadLoads>), kSmallReadLoads);           \
+        else if (a.d == DD) KVQ_SLOT_LAUNCH((slot_read_kernel<DD, BF16, false, kReadLoads>), kReadLoads);              \
+        else KVQ_SLOT_LAUNCH((slot_read_kernel<DD, BF16, true, kReadLoads>), kReadLoads);                              \
+        return hipGetLastError();                                                                                      \
     }
         KVQ_SLOT_CASE(32)
         KVQ_SLOT_CASE(64)
         KVQ_SLOT_CASE(128)
         KVQ_SLOT_CASE(256)
 #undef KVQ_SLOT_CASE
+#undef KVQ_SLOT_LAUNCH
     }
     const dim3 grid = slot_grid(static_cast<unsigned>(a.T) * a.Hkv, kSlotWaves);
     if (write) hipLaunchKernelGGL((slot_write_generic<BF16>), grid, block, 0, stream, a);

@@ -648,11 +648,12 @@ class PageMapper:
     new_tokens [B] (negative: taken off the end), lengths [B], block_table [B, max_pages], free_pages [num_pages] (a
     stack) and free_count [1], all int32.  lengths and free_count are updated in place unless new_lengths [B] and
     new_free_count [1] are given; block_table and free_pages always are.  slot_map, token_seq and token_pos [T] (any of
-    them, else max_tokens) describe the packed rows.  Every output is an attribute."""
+    them, else max_tokens) describe the packed rows.  Every output is an attribute.  workspace: a function of the bytes
+    needed that returns a zeroed workspace of at least as many (default: one of its own)."""
 
     def __init__(self, new_tokens, lengths, block_table, free_pages, free_count, page_size, new_lengths=None,
                  new_free_count=None, granted=None, token_offsets=None, slot_map=None, token_seq=None, token_pos=None,
-                 max_tokens=None, stream=None):
+                 max_tokens=None, stream=None, workspace=None):
         B = _rows_of(new_tokens, "new_tokens")
         if block_table.dim() != 2 or block_table.shape[0] != B:
             raise ValueError("block_table: want [B, max_pages_per_seq]")
@@ -685,7 +686,7 @@ class PageMapper:
                                                         self.new_lengths, self.new_free_count, self.granted,
                                                         self.token_offsets, slot_map, token_seq, token_pos)))
         nbytes = int(lib().kvq_page_map_workspace_size(ctypes.byref(self.params)))
-        self.ws = _new_workspace(nbytes, self.device, stream)
+        self.ws = workspace(nbytes) if workspace and nbytes else _new_workspace(nbytes, self.device, stream)
         self._args = (ctypes.byref(self.params), _ptr(self.ws), nbytes)
 
     def __call__(self, stream=None) -> None:
@@ -800,11 +801,12 @@ class SparseDecoder:
     """Decode over the pages that rank highest (kvq_sparse_decode_launch), with its own workspace.
 
     The arguments of PagedDecoder; bounds and bound_scale as page_bounds writes them; selected [B, Hkv, max_selected]
-    and selected_lengths [B, Hkv], both int32, receive the pages attended and the tokens in them."""
+    and selected_lengths [B, Hkv], both int32, receive the pages attended and the tokens in them.  workspace: as
+    PageMapper's."""
 
     def __init__(self, q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, lengths, bounds, bound_scale, out,
                  selected, selected_lengths, max_seq_len=0, keep_first=1, keep_last=1, softmax_scale=0.0, num_splits=0,
-                 k_new=None, v_new=None, stream=None):
+                 k_new=None, v_new=None, stream=None, workspace=None):
         check_paged(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, lengths, out, k_new, v_new)
         B, Hq, d = q.shape
         P_, Hkv, page, _ = k_pages.shape
@@ -823,7 +825,7 @@ class SparseDecoder:
         self.params = SparseDecodeParams(step, int(selected.shape[2]), int(keep_first), int(keep_last), _ptr(bounds),
                                          _ptr(bound_scale), _ptr(selected), _ptr(selected_lengths))
         self.ws_bytes = int(lib().kvq_sparse_decode_workspace_size(ctypes.byref(self.params)))
-        self.ws = _new_workspace(self.ws_bytes, self.device, stream)
+        self.ws = workspace(self.ws_bytes) if workspace and self.ws_bytes else _new_workspace(self.ws_bytes, self.device, stream)
         self._args = (ctypes.byref(self.params), _ptr(self.ws), self.ws_bytes)
 
     def __call__(self, stream=None) -> None:

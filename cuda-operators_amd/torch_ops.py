@@ -21,6 +21,22 @@ allocates nothing once its workspace exists.
   torch.ops.kvq.attention(q, k, v, softmax_scale, num_splits) -> out
       kvq_attention_launch: dense fp32 softmax(q k^T * scale) v, q [M, d],
       k/v [N, d] (scale 0: 1/sqrt(d)).
+  torch.ops.kvq.page_map(new_tokens, lengths, block_table, free_pages, free_count, page_size,
+                         max_tokens) -> (granted, token_offsets, slot_map, token_seq, token_pos)
+      kvq_page_map_launch in place (mutates lengths, block_table, free_pages, free_count).
+  torch.ops.kvq.slot_write(k_new, v_new, slots, k_pages, v_pages, k_scale_pages, v_scale_pages) -> ()
+      kvq_slot_write_launch of packed rows [T, Hkv, d] (mutates the pool).
+  torch.ops.kvq.slot_read(slots, k_pages, v_pages, k_scale_pages, v_scale_pages, dtype,
+                          head_major) -> (k, v)
+      kvq_slot_read_launch into [T, Hkv, d], or [Hkv, T, d] with head_major.
+  torch.ops.kvq.page_bounds(k_pages, k_scale_pages, block_table, lengths, bounds, bound_scale,
+                            start, max_seq_len) -> ()
+      kvq_page_bounds_launch (mutates bounds and bound_scale).
+  torch.ops.kvq.sparse_decode(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table,
+                              lengths, bounds, bound_scale, max_selected, keep_first, keep_last,
+                              max_seq_len, softmax_scale, num_splits, k_new, v_new)
+                              -> (out, selected, selected_lengths)
+      kvq_sparse_decode_launch (mutates the pool with k_new/v_new, and the bounds).
 
 Workspaces are cached per (operator, device, stream) and grown on demand:
 launches on one stream are ordered, so they may share one; launches on
@@ -40,7 +56,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
@@ -196,4 +212,95 @@ def _attention_fake(q, k, v, softmax_scale, num_splits):
     return torch.empty_like(q)
 
 
-__all__ = ["decode", "paged_decode", "append", "prefill", "attention"]
+@torch.library.custom_op("kvq::page_map", mutates_args=("lengths", "block_table", "free_pages", "free_count"))
+def page_map(new_tokens: Tensor, lengths: Tensor, block_table: Tensor, free_pages: Tensor, free_count: Tensor,
+             page_size: int, max_tokens: int) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    rows = [torch.empty(max_tokens, dtype=torch.int32, device=lengths.device) for _ in range(3)]
+    m = kvq.PageMapper(new_tokens, lengths, block_table, free_pages, free_count, page_size, slot_map=rows[0],
+                       token_seq=rows[1], token_pos=rows[2], workspace=_workspace_for("page_map", lengths.device))
+    m()
+    return m.granted, m.token_offsets, rows[0], rows[1], rows[2]
+
+
+def _workspace_for(op, device):
+    """This operator's cached workspace of the device's current stream, as a function of the bytes needed."""
+    return lambda n: _workspace((op, device.index, torch.cuda.current_stream(device).cuda_stream), n, device)
+
+
+@page_map.register_fake
+def _page_map_fake(new_tokens, lengths, block_table, free_pages, free_count, page_size, max_tokens):
+    e = lambda n: torch.empty(n, dtype=torch.int32, device=lengths.device)  # noqa: E731
+    B = lengths.shape[0]
+    return e(B), e(B + 1), e(max_tokens), e(max_tokens), e(max_tokens)
+
+
+_POOL = ("k_pages", "v_pages", "k_scale_pages", "v_scale_pages")
+
+
+@torch.library.custom_op("kvq::slot_write", mutates_args=_POOL)
+def slot_write(k_new: Tensor, v_new: Tensor, slots: Tensor, k_pages: Tensor, v_pages: Tensor, k_scale_pages: Tensor,
+               v_scale_pages: Tensor) -> None:
+    kvq.slot_write(k_new, v_new, slots, k_pages, v_pages, k_scale_pages, v_scale_pages)
+
+
+@slot_write.register_fake
+def _slot_write_fake(k_new, v_new, slots, k_pages, v_pages, k_scale_pages, v_scale_pages):
+    return None
+
+
+@torch.library.custom_op("kvq::slot_read", mutates_args=())
+def slot_read(slots: Tensor, k_pages: Tensor, v_pages: Tensor, k_scale_pages: Tensor, v_scale_pages: Tensor,
+              dtype: torch.dtype, head_major: bool) -> Tuple[Tensor, Tensor]:
+    k, v = _slot_read_fake(slots, k_pages, v_pages, k_scale_pages, v_scale_pages, dtype, head_major)
+    rows = (k.transpose(0, 1), v.transpose(0, 1)) if head_major else (k, v)
+    kvq.slot_read(slots, k_pages, v_pages, k_scale_pages, v_scale_pages, *rows)
+    return k, v
+
+
+@slot_read.register_fake
+def _slot_read_fake(slots, k_pages, v_pages, k_scale_pages, v_scale_pages, dtype, head_major):
+    T, Hkv, d = slots.shape[0], k_pages.shape[1], k_pages.shape[3]
+    shape = (Hkv, T, d) if head_major else (T, Hkv, d)
+    return (torch.empty(shape, dtype=dtype, device=k_pages.device),
+            torch.empty(shape, dtype=dtype, device=k_pages.device))
+
+
+@torch.library.custom_op("kvq::page_bounds", mutates_args=("bounds", "bound_scale"))
+def page_bounds(k_pages: Tensor, k_scale_pages: Tensor, block_table: Tensor, lengths: Optional[Tensor],
+                bounds: Tensor, bound_scale: Tensor, start: Optional[Tensor], max_seq_len: int) -> None:
+    kvq.page_bounds(k_pages, k_scale_pages, block_table, lengths, bounds, bound_scale, start=start,
+                    max_seq_len=max_seq_len)
+
+
+@page_bounds.register_fake
+def _page_bounds_fake(k_pages, k_scale_pages, block_table, lengths, bounds, bound_scale, start, max_seq_len):
+    return None
+
+
+@torch.library.custom_op("kvq::sparse_decode", mutates_args=_POOL + ("bounds", "bound_scale"))
+def sparse_decode(q: Tensor, k_pages: Tensor, v_pages: Tensor, k_scale_pages: Tensor, v_scale_pages: Tensor,
+                  block_table: Tensor, lengths: Optional[Tensor], bounds: Tensor, bound_scale: Tensor,
+                  max_selected: int, keep_first: int, keep_last: int, max_seq_len: int, softmax_scale: float,
+                  num_splits: int, k_new: Optional[Tensor], v_new: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
+    out, selected, selected_lengths = _sparse_outputs(q, k_pages, max_selected)
+    kvq.SparseDecoder(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, lengths, bounds, bound_scale, out,
+                      selected, selected_lengths, max_seq_len=max_seq_len, keep_first=keep_first, keep_last=keep_last,
+                      softmax_scale=softmax_scale, num_splits=num_splits, k_new=k_new, v_new=v_new,
+                      workspace=_workspace_for("sparse", q.device))()
+    return out, selected, selected_lengths
+
+
+def _sparse_outputs(q, k_pages, max_selected):
+    shape = (q.shape[0], k_pages.shape[1])
+    return (torch.empty_like(q), torch.empty(shape + (max_selected,), dtype=torch.int32, device=q.device),
+            torch.empty(shape, dtype=torch.int32, device=q.device))
+
+
+@sparse_decode.register_fake
+def _sparse_decode_fake(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, lengths, bounds, bound_scale,
+                        max_selected, keep_first, keep_last, max_seq_len, softmax_scale, num_splits, k_new, v_new):
+    return _sparse_outputs(q, k_pages, max_selected)
+
+
+__all__ = ["decode", "paged_decode", "append", "prefill", "attention", "page_map", "slot_write", "slot_read",
+           "page_bounds", "sparse_decode"]

@@ -173,3 +173,32 @@ def test_python_wrappers_refuse():
     with pytest.raises(ValueError, match="q: want contiguous cuda"):
         kvq.SparseDecoder(torch.zeros(1, 4, 64), *pool, i32(1, 4), i32(1), torch.zeros(4, 2, 2, 64, dtype=torch.int8),
                           torch.zeros(4, 2), torch.zeros(1, 4, 64), i32(1, 2, 3), i32(1, 2))
+
+
+def _mutated(op):
+    return {a.name for a in op.default._schema.arguments if a.alias_info is not None and a.alias_info.is_write}
+
+
+def test_torch_operators_register_and_trace():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    importlib.import_module("cuda-operators_amd.torch_ops")
+    ops = torch.ops.kvq
+    pool_names = {"k_pages", "v_pages", "k_scale_pages", "v_scale_pages"}
+    assert _mutated(ops.page_map) == {"lengths", "block_table", "free_pages", "free_count"}
+    assert _mutated(ops.slot_write) == pool_names and _mutated(ops.slot_read) == set()
+    assert _mutated(ops.page_bounds) == {"bounds", "bound_scale"}
+    assert _mutated(ops.sparse_decode) == pool_names | {"bounds", "bound_scale"}
+    with FakeTensorMode():
+        i32 = lambda *s: torch.empty(s, dtype=torch.int32)  # noqa: E731
+        got = ops.page_map(i32(3), i32(3), i32(3, 8), i32(90), i32(1), 16, 50)
+        assert [t.shape[0] for t in got] == [3, 4, 50, 50, 50] and all(t.dtype == torch.int32 for t in got)
+        kp, sp = torch.empty(9, 2, 16, 64, dtype=torch.int8), torch.empty(9, 2, 16)
+        rows = torch.empty(5, 2, 64, dtype=torch.bfloat16)
+        ops.slot_write(rows, rows, i32(5), kp, kp.clone(), sp, sp.clone())
+        k, v = ops.slot_read(i32(5), kp, kp, sp, sp, torch.float32, True)
+        assert k.shape == v.shape == (2, 5, 64) and k.dtype == torch.float32
+        b, s = torch.empty(9, 2, 2, 64, dtype=torch.int8), torch.empty(9, 2)
+        ops.page_bounds(kp, sp, i32(3, 8), i32(3), b, s, None, 0)
+        out, sel, n = ops.sparse_decode(torch.empty(3, 8, 64), kp, kp.clone(), sp, sp.clone(), i32(3, 8), i32(3), b, s, 4, 1,
+                                        1, 0, 0.0, 0, None, None)
+        assert out.shape == (3, 8, 64) and sel.shape == (3, 2, 4) and n.shape == (3, 2)

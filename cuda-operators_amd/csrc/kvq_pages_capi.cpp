@@ -130,9 +130,9 @@ SparsePlan sparse_plan(const kvq_sparse_decode_params* p) {
     r.select = kvq::select_plan(s.batch, s.num_q_heads, s.head_dim, r.vec_ok, (max_len - 1) / s.page_size + 1, p->max_selected);
     // The selection's arrival counters share the workspace's counter prefix with
     // the attention's: the launches are ordered and each leaves them at zero.
-    const size_t base = std::max(r.step_bytes, r.select.splits > 1 ? kCounterBytes : 0);
-    r.keys_at = round_up(base, kAlign);
-    r.bytes = r.select.key_bytes ? r.keys_at + r.select.key_bytes : base;
+    // Ranks never lie in the prefix, which another shape may count in.
+    r.keys_at = round_up(std::max(r.step_bytes, kCounterBytes), kAlign);
+    r.bytes = r.select.key_bytes ? r.keys_at + r.select.key_bytes : r.step_bytes;
     return r;
 }
 

@@ -605,18 +605,34 @@ def _one_device(*tensors):
     return index
 
 
-def _call(fn, name, args, index, stream=None) -> None:
-    """One launch on device `index`, whichever is current, and on `stream` (default: that device's current stream)."""
+def _call(fn, name, args, index, stream=None, own=()) -> None:
+    """One launch on device `index`, whichever is current, and on `stream` (default: that device's current stream).
+
+    own: the call's tensors; on another stream than the current one their memory is kept from being handed out, should
+    they be dropped, before the launch has run."""
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
-            return _call(fn, name, args, index, stream)
+            return _call(fn, name, args, index, stream, own)
     if stream is None:
         stream = torch._C._cuda_getCurrentRawStream(index)
-    elif not isinstance(stream, int):
-        stream = stream.cuda_stream
+    else:
+        handle = stream if isinstance(stream, int) else stream.cuda_stream
+        if own and handle != torch._C._cuda_getCurrentRawStream(index):
+            s = _torch_stream(stream, index)
+            for t in own:
+                if t is not None:
+                    t.record_stream(s)
+        stream = handle
     code = fn(*args, stream)
     if code != HIP_SUCCESS:
         raise KvqError(name, code)
+
+
+def _torch_stream(stream, index):
+    """The torch stream of a torch stream or a raw hipStream_t handle."""
+    if not isinstance(stream, int):
+        return stream
+    return torch.cuda.ExternalStream(stream, index) if stream else torch.cuda.default_stream(index)
 
 
 def _new_workspace(nbytes, index, stream):
@@ -625,9 +641,7 @@ def _new_workspace(nbytes, index, stream):
     if not nbytes:
         return None
     with torch.cuda.device(index):
-        if isinstance(stream, int):
-            stream = torch.cuda.ExternalStream(stream, index) if stream else torch.cuda.default_stream(index)
-        stream = stream or torch.cuda.current_stream(index)
+        stream = torch.cuda.current_stream(index) if stream is None else _torch_stream(stream, index)
         with torch.cuda.stream(stream):
             ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
             workspace_init(ws, nbytes, stream)
@@ -687,11 +701,13 @@ class PageMapper:
                                                         self.token_offsets, slot_map, token_seq, token_pos)))
         nbytes = int(lib().kvq_page_map_workspace_size(ctypes.byref(self.params)))
         self.ws = workspace(nbytes) if workspace and nbytes else _new_workspace(nbytes, self.device, stream)
+        self._keep = (new_tokens, lengths, block_table, free_pages, free_count, self.new_lengths, self.new_free_count,
+                      self.granted, self.token_offsets, slot_map, token_seq, token_pos, self.ws)
         self._args = (ctypes.byref(self.params), _ptr(self.ws), nbytes)
 
     def __call__(self, stream=None) -> None:
         """Launch on `stream` (a torch stream or a raw hipStream_t handle; default: torch's current stream)."""
-        _call(lib().kvq_page_map_launch, "kvq_page_map_launch", self._args, self.device, stream)
+        _call(lib().kvq_page_map_launch, "kvq_page_map_launch", self._args, self.device, stream, self._keep)
 
 
 def page_map(new_tokens, lengths, block_table, free_pages, free_count, page_size, stream=None, **outputs) -> PageMapper:
@@ -741,13 +757,14 @@ def slot_write(k_new, v_new, slots, k_pages, v_pages, k_scale_pages, v_scale_pag
     for s, n in ((ks, "k_new"), (vs, "v_new")):
         if (Hkv > 1 and s[1] != d) or (T > 1 and s[0] < Hkv * d):
             raise ValueError(f"{n}: a token's heads must lie together, got strides {s}")
-    index = _one_device(k_new, v_new, slots, k_pages, v_pages, k_scale_pages, v_scale_pages)
+    tensors = (k_new, v_new, slots, k_pages, v_pages, k_scale_pages, v_scale_pages)
+    index = _one_device(*tensors)
     if T == 0:
         return
     p = SlotWriteParams(T, Hkv, d, page, P_, code, k_new.data_ptr(), v_new.data_ptr(), ks[0] if T > 1 else 0,
                         vs[0] if T > 1 else 0, slots.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                         k_scale_pages.data_ptr(), v_scale_pages.data_ptr())
-    _call(lib().kvq_slot_write_launch, "kvq_slot_write_launch", (ctypes.byref(p),), index, stream)
+    _call(lib().kvq_slot_write_launch, "kvq_slot_write_launch", (ctypes.byref(p),), index, stream, tensors)
 
 
 def slot_read(slots, k_pages, v_pages, k_scale_pages, v_scale_pages, k_out, v_out, stream=None):
@@ -759,15 +776,16 @@ def slot_read(slots, k_pages, v_pages, k_scale_pages, v_scale_pages, k_out, v_ou
     _check_rows(k_out, k_out.dtype, (T, Hkv, d), "k_out")
     _check_rows(v_out, k_out.dtype, (T, Hkv, d), "v_out")
     strides = k_out.stride()
-    if v_out.stride()[:2] != strides[:2]:
+    if v_out.stride()[:2] != strides[:2] and any(n > 1 and a != b for n, a, b in zip((T, Hkv), strides, v_out.stride())):
         raise ValueError(f"k_out and v_out must have the same strides, got {strides} and {v_out.stride()}")
-    index = _one_device(slots, k_pages, v_pages, k_scale_pages, v_scale_pages, k_out, v_out)
+    tensors = (slots, k_pages, v_pages, k_scale_pages, v_scale_pages, k_out, v_out)
+    index = _one_device(*tensors)
     if T == 0:
         return k_out, v_out
     p = SlotReadParams(T, Hkv, d, page, P_, code, slots.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                        k_scale_pages.data_ptr(), v_scale_pages.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
                        strides[0], strides[1])
-    _call(lib().kvq_slot_read_launch, "kvq_slot_read_launch", (ctypes.byref(p),), index, stream)
+    _call(lib().kvq_slot_read_launch, "kvq_slot_read_launch", (ctypes.byref(p),), index, stream, tensors)
     return k_out, v_out
 
 
@@ -791,10 +809,11 @@ def page_bounds(k_pages, k_scale_pages, block_table, lengths, bounds, bound_scal
     for t, n in ((start, "start"), (lengths, "lengths")):
         if t is not None:
             _needs((t, torch.int32, (B,), n))
-    index = _one_device(k_pages, k_scale_pages, block_table, lengths, bounds, bound_scale, start)
+    tensors = (k_pages, k_scale_pages, block_table, lengths, bounds, bound_scale, start)
+    index = _one_device(*tensors)
     p = PageBoundsParams(B, Hkv, d, page, P_, per, int(max_seq_len), block_table.data_ptr(), _ptr(start), _ptr(lengths),
                          k_pages.data_ptr(), k_scale_pages.data_ptr(), bounds.data_ptr(), bound_scale.data_ptr())
-    _call(lib().kvq_page_bounds_launch, "kvq_page_bounds_launch", (ctypes.byref(p),), index, stream)
+    _call(lib().kvq_page_bounds_launch, "kvq_page_bounds_launch", (ctypes.byref(p),), index, stream, tensors)
 
 
 class SparseDecoder:
@@ -829,7 +848,8 @@ class SparseDecoder:
         self._args = (ctypes.byref(self.params), _ptr(self.ws), self.ws_bytes)
 
     def __call__(self, stream=None) -> None:
-        _call(lib().kvq_sparse_decode_launch, "kvq_sparse_decode_launch", self._args, self.device, stream)
+        _call(lib().kvq_sparse_decode_launch, "kvq_sparse_decode_launch", self._args, self.device, stream,
+              self.keep + (self.ws,))
 
 
 def sparse_decode_plan(p: SparseDecodeParams) -> PlanInfo:

@@ -30,6 +30,9 @@ bool heads_ok(int num_kv_heads, int head_dim) {
 // The tuned bounds kernels address a page's keys with 32-bit offsets.
 bool page_fits(int page_size, int head_dim) { return static_cast<long long>(page_size) * head_dim < (1LL << 30); }
 
+// n rows `stride` elements apart lie within an address space.
+bool spans(int64_t n, int64_t stride) { return n <= 1 || stride <= (1LL << 46) / n; }
+
 bool dtype_ok(int dtype) { return dtype == KVQ_DTYPE_F32 || dtype == KVQ_DTYPE_BF16; }
 
 kvq::PageMap page_map(const int32_t* table, int size, int max_pages, int num_pages) {
@@ -161,7 +164,7 @@ hipError_t kvq_slot_write_launch(const kvq_slot_write_params* p, hipStream_t str
     if (static_cast<long long>(p->tokens) * p->num_kv_heads >= (1LL << 31)) return hipErrorInvalidValue;
     const int64_t row = static_cast<int64_t>(p->num_kv_heads) * p->head_dim;
     if ((p->k_stride != 0 && p->k_stride < row) || (p->v_stride != 0 && p->v_stride < row)) return hipErrorInvalidValue;
-    if (p->k_stride > (1LL << 40) || p->v_stride > (1LL << 40)) return hipErrorInvalidValue;
+    if (!spans(p->tokens, p->k_stride) || !spans(p->tokens, p->v_stride)) return hipErrorInvalidValue;
     const bool bf16 = p->dtype == KVQ_DTYPE_BF16;
     kvq::SlotArgs a{};
     a.slots = p->slots;
@@ -195,7 +198,7 @@ hipError_t kvq_slot_read_launch(const kvq_slot_read_params* p, hipStream_t strea
     if (static_cast<long long>(p->tokens) * p->num_kv_heads >= (1LL << 31)) return hipErrorInvalidValue;
     // Rows apart: the tokens of a head within a token's heads, or the other way round.
     const int64_t ts = p->token_stride, hs = p->head_stride, d = p->head_dim, T = p->tokens, H = p->num_kv_heads;
-    if (ts < 0 || hs < 0 || ts > (1LL << 40) || hs > (1LL << 40)) return hipErrorInvalidValue;
+    if (ts < 0 || hs < 0 || !spans(T, ts) || !spans(H, hs)) return hipErrorInvalidValue;
     const bool by_token = (H == 1 || hs >= d) && (T <= 1 || ts >= (H > 1 ? (H - 1) * hs : 0) + d);
     const bool by_head = (T <= 1 || ts >= d) && (H == 1 || hs >= (T > 1 ? (T - 1) * ts : 0) + d);
     if (!by_token && !by_head) return hipErrorInvalidValue;

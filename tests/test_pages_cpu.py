@@ -101,7 +101,7 @@ ROWS = [dict(tokens=-1), dict(num_kv_heads=0), dict(head_dim=0), dict(head_dim=4
         dict(tokens=1 << 30, num_kv_heads=2)]
 
 
-@pytest.mark.parametrize("bad", BAD_POOL + ROWS + [dict(k_stride=127), dict(v_stride=-1), dict(k_stride=1 << 41)] +
+@pytest.mark.parametrize("bad", BAD_POOL + ROWS + [dict(k_stride=127), dict(v_stride=-1), dict(k_stride=1 << 45)] +
                          [{n: None} for n in ("k_new", "v_new", "slots", "k_pages", "v_pages", "k_scale_pages", "v_scale_pages")])
 def test_slot_write_refuses(bad):
     assert launch("kvq_slot_write_launch", write_params(**bad)) == INVALID
@@ -109,7 +109,7 @@ def test_slot_write_refuses(bad):
 
 @pytest.mark.parametrize("bad", BAD_POOL + ROWS + [
     dict(token_stride=127), dict(token_stride=-128), dict(head_stride=63), dict(head_stride=0), dict(token_stride=0, head_stride=64),
-    dict(token_stride=64, head_stride=319), dict(token_stride=63, head_stride=320), dict(token_stride=1 << 41)] +
+    dict(token_stride=64, head_stride=319), dict(token_stride=63, head_stride=320), dict(token_stride=1 << 45)] +
     [{n: None} for n in ("k_out", "v_out", "slots", "k_pages", "v_pages", "k_scale_pages", "v_scale_pages")])
 def test_slot_read_refuses(bad):
     assert launch("kvq_slot_read_launch", read_params(**bad)) == INVALID

@@ -254,7 +254,7 @@ __device__ inline void write_kept(const SelectArgs& a, const Unit& u, int unit) 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr int kSelTile = 16;                      // pages a wave scores at a time
 constexpr int kSelStep = kSelTile * kSelWaves;    // pages a workgroup does
-constexpr int kSelLdsKeys = 12288;                // ranks kept in LDS, at most
+constexpr int kSelLdsKeys = 6144;                 // ranks kept in LDS, at most
 
 template <int CTRL>
 __device__ __forceinline__ int dpp_max(int x) {
@@ -270,7 +270,7 @@ __device__ __forceinline__ int row16_max(int x) {
 
 template <int ND>
 __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))) void select_kernel(const SelectArgs a, int lds_keys) {
-    extern __shared__ __align__(16) unsigned char s_dyn[];  // columns [passes][ND][64] x 16 bytes, then lds_keys ranks
+    extern __shared__ __align__(16) unsigned char s_dyn[];  // columns [passes][ND][64] x 16 bytes, lds_keys ranks, their pool rows
     __shared__ RankScratch s;
     __shared__ float s_max[kSelWaves];
     __shared__ int s_last;
@@ -283,6 +283,11 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
     const int d = a.b.d;
     const int passes = (a.G + 15) / 16;
     unsigned* s_keys = reinterpret_cast<unsigned*>(s_dyn + static_cast<size_t>(passes) * ND * 1024);
+    int* s_rows = reinterpret_cast<int*>(s_keys + lds_keys);
+    // q is on its way while the length and the page ids are waited for.
+    const float4* q = reinterpret_cast<const float4*>(a.q + static_cast<size_t>(unit) * a.G * d);
+    const int quads = a.G * d / 4;
+    const float4 mine = q[min(t, quads - 1)];
     const Unit u = unit_of(a, unit);
 
     // This workgroup's pages, and how many workgroups have any.
@@ -321,16 +326,13 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
     float next_scale = 0.0f;
     int base = i0 + wave * kSelTile;
     const size_t row0 = row_of(base + r);
+    size_t next_row = row0;  // of the pages in `next`
     size_t row = row_of(base + kSelStep + r);
     const bool renews = u.renewed >= 0 && split == active - 1;
     if (!renews) load(row0, next, next_scale);
 
     // The heads' codes: four of one head a thread, once into the highs' half of
     // its column (those above zero) and once into the lows' half (those below).
-    const float4* q = reinterpret_cast<const float4*>(a.q + static_cast<size_t>(unit) * a.G * d);
-    const int quads = a.G * d / 4;
-    const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const float4 mine = t < quads ? q[t] : zero;
     auto largest = [](const float4& x) { return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))); };
     float amax = largest(mine);
     for (int i = t + kSelThreads; i < quads; i += kSelThreads) amax = fmaxf(amax, largest(q[i]));
@@ -371,7 +373,9 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
 #pragma unroll
         for (int j = 0; j < ND; j++) x[j] = next[j];
         const float scale = next_scale;
+        const size_t now = next_row;
         load(row, next, next_scale);
+        next_row = row;
         row = row_of(base + 2 * kSelStep + r);
         i32x4 top = {INT_MIN, INT_MIN, INT_MIN, INT_MIN};
         for (int pass = 0; pass < passes; pass++) {
@@ -392,6 +396,7 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
         const int best = (r & 2) ? ((r & 1) ? top[3] : top[2]) : ((r & 1) ? top[1] : top[0]);
         const int page = 4 * (lane >> 4) + (r & 3);
         const float sc = __shfl(scale, page);
+        if (!shared && lane < kSelTile && base + r < i1) s_rows[base + r] = static_cast<int>(now);
         const int i = base + page;
         if (r < 4 && i < i1) {
             const unsigned key = rank_key(static_cast<float>(best) * sc);
@@ -413,8 +418,10 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
     }
     if (shared && n <= lds_keys) {
         for (int i = t; i < n; i += kSelThreads) {
+            const int place = pool_row(a, u, a.keep_first + i);
             const unsigned key = __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             s_keys[i] = key;
+            s_rows[i] = place;
             lo = min(lo, key);
             hi = max(hi, key);
         }
@@ -424,12 +431,13 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
     }
     __syncthreads();
     int32_t* out = a.selected + static_cast<size_t>(unit) * a.max_selected + a.keep_first;
-    auto finish = [&](const auto& key) {
+    auto finish = [&](const auto& key, const auto& place_of) {
         const Cut cut = rank_cut(key, n, u.wanted, lo, hi, s);
-        rank_emit(key, n, cut, s, [&](int place, int i) { out[place] = pool_row(a, u, a.keep_first + i); });
+        rank_emit(key, n, cut, s, [&](int place, int i) { out[place] = place_of(i); });
     };
-    if (n <= lds_keys) finish([&](int i) { return s_keys[i]; });
-    else finish([&](int i) { return __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
+    if (n <= lds_keys) finish([&](int i) { return s_keys[i]; }, [&](int i) { return s_rows[i]; });
+    else finish([&](int i) { return __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); },
+                [&](int i) { return pool_row(a, u, a.keep_first + i); });
 }
 
 // Any head dim or alignment: a workgroup a unit, a wave a page, keys in global memory.
@@ -514,7 +522,7 @@ hipError_t launch_select(const SelectArgs& a, const SelectPlan& p, bool vec_ok, 
     }
     const int nd = (2 * a.b.d + 63) / 64;
     const dim3 grid(units * static_cast<unsigned>(p.splits));
-    const size_t lds = static_cast<size_t>((a.G + 15) / 16) * nd * 1024 + static_cast<size_t>(p.lds_keys) * sizeof(unsigned);
+    const size_t lds = static_cast<size_t>((a.G + 15) / 16) * nd * 1024 + static_cast<size_t>(p.lds_keys) * 2 * sizeof(unsigned);
 #define KVQ_SELECT_CASE(ND) \
     case ND: hipLaunchKernelGGL(select_kernel<ND>, grid, block, lds, stream, a, p.lds_keys); break;
     switch (nd) {

@@ -496,7 +496,9 @@ typedef struct kvq_page_bounds_params {
  * codes, S = max |s_t|, highs ceil(max_t k_t r_t) and lows floor(min_t k_t r_t)
  * per dim for r_t = s_t / S (quotient and product rounded in fp32), so every key
  * lies in S * [low, high] but for those roundings.  S = 0: bounds 0.  S not
- * finite: bounds 127 and -127 under the scale +inf, which rank first. */
+ * finite: bounds 127 and -127 under the scale +inf, which rank first.  Codes lie
+ * in [-127, 127], as every quantiser here writes them.  A page in two tables must
+ * hold the same tokens below both lengths. */
 hipError_t kvq_page_bounds_launch(const kvq_page_bounds_params* p, hipStream_t stream);
 
 typedef struct kvq_sparse_decode_params {

@@ -533,19 +533,18 @@ __global__ __launch_bounds__(kBoundsWaves* kWave) void page_bounds_generic(const
 
 }  // namespace
 
-// Workgroups of 1024 threads, two rows a thread, up to 64 (each scans the whole
-// batch).  Without arrays of rows the pages are what there is to do.
-#ifndef KVQ_MAP_ROWS
-#define KVQ_MAP_ROWS 2048
-#endif
-#ifndef KVQ_MAP_GROUPS
-#define KVQ_MAP_GROUPS 64
-#endif
+// Each workgroup scans the whole batch, so more of them only share out what comes
+// after, of which the releases of a decode step are not known here: one for each
+// 32 rows, up to 128 (steps of 1000 sequences 7.6 us, with one for each 256 rows
+// 9.6, each 2048 16.4; of 256 sequences 7.8 / 8.1 / 8.1; of 64 6.4 / 6.2 / 6.2;
+// 131008 rows of 64 prompts 6.0 in 128, 6.4 in 64, 7.9 in 32 workgroups).
+// Without arrays of rows the pages are what there is to do.
+constexpr int kMapRows = 32, kMapGroups = 128;
 int page_map_groups(const PageMapArgs& a) {
     const long long work = a.slot_map || a.token_seq || a.token_pos
                                ? a.T
                                : min(static_cast<long long>(a.T / static_cast<int>(a.page.d)) + a.B, static_cast<long long>(a.num_pages));
-    return static_cast<int>(max(1LL, min(static_cast<long long>(KVQ_MAP_GROUPS), (work + KVQ_MAP_ROWS - 1) / KVQ_MAP_ROWS)));
+    return static_cast<int>(max(1LL, min(static_cast<long long>(kMapGroups), (work + kMapRows - 1) / kMapRows)));
 }
 
 hipError_t launch_page_map(const PageMapArgs& a, hipStream_t stream) {

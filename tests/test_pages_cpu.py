@@ -94,7 +94,7 @@ def test_page_map_workspace_is_wanted():
     if n:
         assert launch("kvq_page_map_launch", p, None, n) == INVALID
         assert launch("kvq_page_map_launch", p, 4096, n - 1) == INVALID
-    assert kvq.lib().kvq_page_map_workspace_size(ctypes.byref(map_params())) == 0
+    assert kvq.lib().kvq_page_map_workspace_size(ctypes.byref(map_params(max_tokens=20))) == 0
 
 
 ROWS = [dict(tokens=-1), dict(num_kv_heads=0), dict(head_dim=0), dict(head_dim=4097), dict(dtype=2), dict(dtype=-1),

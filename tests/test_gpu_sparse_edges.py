@@ -203,3 +203,44 @@ def test_plan_and_workspace_agree():
     assert info.workspace_bytes == dec.ws_bytes
     assert info.kernel == kvq.KERNEL_DECODE_MFMA
     assert kvq.lib().kvq_sparse_decode_launch(ctypes.byref(dec.params), None, 0, None) == (kvq.HIP_ERROR_INVALID_VALUE if dec.ws_bytes else 0)
+
+
+@pytest.mark.parametrize("G", [64, 65])
+def test_many_heads_over_many_pages(G):
+    """The most columns and ranks that a workgroup keeps, and one head more (which takes the generic selection)."""
+    rng = np.random.default_rng(11)
+    p = Problem(rng, [5900, 64], G, 1, 256, 1)
+    g = p.gpu()
+    dec, out, sel, n = decoder(p, g, 300)
+    dec()
+    torch.cuda.synchronize()
+    verify(p, out, sel, n, 300, 1, 1)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("d", [64, 20])
+def test_queries_that_are_not_finite(d, bad):
+    """Their own heads give NaN; whatever is selected are pages of the sequence, and the other heads attend those."""
+    rng = np.random.default_rng(12)
+    p = Problem(rng, [16 * 50 + 3, 16 * 40], 4, 2, d, 16)
+    p.q[0, 1, 3] = bad     # head 1 of the first kv head
+    p.q[1, 4:] = bad       # all of the second kv head
+    g = p.gpu()
+    dec, out, sel, n = decoder(p, g, 9)
+    dec()
+    torch.cuda.synchronize()
+    picked, out, n = down(sel), down(out), down(n)
+    for b, length in enumerate(p.lens):
+        of_page = {int(x): i for i, x in enumerate(p.table[b, :ref.pages_of(length, 16)])}
+        for h in range(2):
+            entries = [of_page[int(x) // 2] for x in picked[b, h]]
+            assert (picked[b, h] % 2 == h).all() and entries == sorted(set(entries))
+            assert entries[0] == 0 and entries[-1] == len(of_page) - 1 and n[b, h] == 8 * 16 + (length - 1) % 16 + 1
+            rows = p.rows(b, h, entries)
+            for i in range(4):
+                q = p.q[b, 4 * h + i:4 * h + i + 1]
+                if not np.isfinite(q).all():
+                    assert np.isnan(out[b, 4 * h + i]).all()
+                    continue
+                exact = ref.attend(q, *rows, 1 / np.sqrt(d))
+                assert np.abs(out[b, 4 * h + i] - exact[0]).max() <= ref.attend_tolerance(q, *rows, 1 / np.sqrt(d))

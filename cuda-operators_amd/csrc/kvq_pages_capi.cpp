@@ -119,10 +119,11 @@ SparsePlan sparse_plan(const kvq_sparse_decode_params* p) {
     if (s.num_splits == 0) {
         // Nearly every sequence attends the same number of tokens, so the split
         // count of a uniform batch, over at least two tiles a wave, beats the
-        // plans for ragged ones: 8 heads of 4096 tokens 28.3 us a step with
-        // those, 24.2 in 16 splits (26.0 in 32, 46.6 unsplit); 128 units of 4096
-        // tokens 53.5 / 47.8 us; 256 units of 2048 tokens, whose ragged plan has
-        // a launch of its own, 93.5 / 50.3 us.
+        // plans for ragged ones: 8 heads of 4096 tokens 24.0 us a step with
+        // those, 20.3 in 16 splits (21.0 in 8, 21.7 in 32, 41.4 unsplit); 128 units
+        // of 4096 tokens 47.3 us, 41.2 in 2 splits (55.0 unsplit, 42.5 in 4); 256
+        // units of 2048 tokens, whose ragged plan has a launch of its own, 85.0 us,
+        // 43.5 unsplit.
         kvq_paged_decode_params u = s;
         u.lengths = nullptr;
         kvq_plan_info info;

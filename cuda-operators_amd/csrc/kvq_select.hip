@@ -541,9 +541,9 @@ SelectPlan select_plan(int units, int G, int d, bool vec_ok, int max_pages, int 
     if (vec_ok && select_tuned(G, d)) {
         // About two workgroups a CU, each with at least one step of pages; units
         // that fill the CUs alone are not split (whole steps: 2048 pages of 8
-        // units 22.1 us in 16 parts, 24.2 in 4, 28.3 in 2; 1024 pages of 128 units
-        // 42.6 us in 4 parts, 43.5 in 2, 44.8 in one; of 256 units 45.6 in 2, 44.4 in
-        // one).
+        // units 20.4 us in 16 parts, 22.8 in 4, 26.8 in 2; 1024 pages of 128 units
+        // 42.6 us in 4 parts, 42.5 in 2, 44.1 in one; of 256 units 45.3 in 2, 43.5
+        // in one).
         const long steps = (static_cast<long>(max_pages) + kSelStep - 1) / kSelStep;
         if (units < 256) p.splits = static_cast<int>(std::min(steps, 512L / units));
         p.lds_keys = max_pages <= kSelLdsKeys ? max_pages : 0;

@@ -244,3 +244,24 @@ def test_queries_that_are_not_finite(d, bad):
                     continue
                 exact = ref.attend(q, *rows, 1 / np.sqrt(d))
                 assert np.abs(out[b, 4 * h + i] - exact[0]).max() <= ref.attend_tolerance(q, *rows, 1 / np.sqrt(d))
+
+
+@pytest.mark.parametrize("length", [16 * 40 + 1, 16 * 40 + 9])
+def test_uniform_steps_append_as_those_with_lengths(length):
+    """Without a lengths array, every sequence of max_seq_len tokens: the same pages, bits, bounds and appended rows."""
+    rng = np.random.default_rng(13)
+    p = Problem(rng, [length] * 3, 4, 2, 64, 16)
+    new = [up(rng.standard_normal((3, 2, 64)).astype(np.float32)) for _ in "kv"]
+    got = []
+    for lengths in (True, False):
+        g = p.gpu()
+        dec, out, sel, n = decoder(p, g, 7, lengths=lengths, max_seq_len=length, k_new=new[0], v_new=new[1])
+        dec()
+        torch.cuda.synchronize()
+        got.append([out, sel, n] + [g[x] for x in ("k", "v", "ks", "vs", "bounds", "scale")])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    at = p.table[:, (length - 1) // 16], (length - 1) % 16
+    want, scale = ref.quantise(down(new[0]))
+    assert np.array_equal(down(got[1][3])[at[0], :, at[1]], want)
+    assert np.array_equal(down(got[1][5])[at[0], :, at[1]], scale)

@@ -833,8 +833,9 @@ class SparseDecoder:
     """Decode over the pages that rank highest (kvq_sparse_decode_launch), with its own workspace.
 
     The arguments of PagedDecoder; bounds and bound_scale as page_bounds writes them; selected [B, Hkv, max_selected]
-    and selected_lengths [B, Hkv], both int32, receive the pages attended and the tokens in them.  workspace: as
-    PageMapper's."""
+    and selected_lengths [B, Hkv], both int32, receive the pages attended and the tokens in them.  k_new/v_new overwrite
+    token lengths[b] - 1 of every sequence: after a page map give length 0 to those that were granted no token, or write
+    the rows with slot_write.  workspace: as PageMapper's."""
 
     def __init__(self, q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, lengths, bounds, bound_scale, out,
                  selected, selected_lengths, max_seq_len=0, keep_first=1, keep_last=1, softmax_scale=0.0, num_splits=0,

@@ -37,6 +37,8 @@ allocates nothing once its workspace exists.
                               max_seq_len, softmax_scale, num_splits, k_new, v_new)
                               -> (out, selected, selected_lengths)
       kvq_sparse_decode_launch (mutates the pool with k_new/v_new, and the bounds).
+      k_new/v_new of decode, paged_decode and sparse_decode go to every sequence
+      of length 1 or more; one without a new token in the step has length 0.
 
 Workspaces are cached per (operator, device, stream) and grown on demand:
 launches on one stream are ordered, so they may share one; launches on

@@ -110,7 +110,9 @@ typedef struct kvq_decode_params {
     /* Fused append (both NULL = off).  When set, token length_b - 1 of every
      * (b, kv_head) is first quantised from k_new/v_new [B, Hkv, d] fp32 into the
      * cache (int8 values + scale, the same bits as kvq_append_launch), then
-     * attended over; the caller's lengths already count the new token. */
+     * attended over; the caller's lengths already count the new token.  This
+     * holds for every sequence: one that has no new token in this step is given
+     * length 0, or its last token is overwritten. */
     const float* k_new;
     const float* v_new;
 } kvq_decode_params;
@@ -432,6 +434,10 @@ typedef struct kvq_page_map_params {
  *   rows have slot -1; rows behind the last have -1 in all three.  A row whose
  *   page id lies outside the pool has slot -1.
  * - Pages belong to one sequence; a page in two tables is given up twice.
+ * - A decode step's fused append (k_new, v_new) writes token length_b - 1 of every
+ *   sequence, granted or not: of one that was refused, waits or shrank that is a
+ *   token it holds.  Rows written through slot_map skip those sequences; a step
+ *   with a fused append is given length 0 for them (where granted[b] <= 0).
  * Workspace: kvq_page_map_workspace_size bytes (0 for small batches), zero-filled
  * once (kvq_workspace_init) and left zeroed.  Calls on one pool must be ordered. */
 size_t kvq_page_map_workspace_size(const kvq_page_map_params* p);

@@ -254,6 +254,10 @@ __global__ __launch_bounds__(kMapThreads) void page_map_kernel(const PageMapArgs
 // Packed rows into and out of their slots.
 // ---------------------------------------------------------------------------
 constexpr int kSlotWaves = 4;
+// Workgroups along a grid's x: a dimension of 2^32 threads or more is not
+// launched, which short rows reach (fp32 of up to 32 elements, four threads a
+// row, at 2^30 rows).  Further workgroups lie along y.
+constexpr unsigned kSlotGroups = 1u << 20;
 
 // Pool row of token t's row for kv head h; -1: the slot lies outside the pool.
 __device__ __forceinline__ long long slot_row(const SlotArgs& a, int t, int h) {
@@ -295,9 +299,11 @@ struct SlotGeom {
     static_assert(LPR >= 1 && LPR <= kWave && kWave % LPR == 0, "row geometry");
 };
 
-// The wave's unit (token block, head): false past the last one.
+// The wave's unit (token block, head) and plane (blockIdx.y's last bit: K or V):
+// false past the last unit.  Units number at most T * Hkv, below 2^31.
 __device__ __forceinline__ bool slot_unit(const SlotArgs& a, int tb, int& t0, int& h) {
-    const unsigned unit = blockIdx.x * kSlotWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const unsigned group = (blockIdx.y >> 1) * kSlotGroups + blockIdx.x;
+    const unsigned unit = group * kSlotWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const unsigned blk = fastdiv(unit, a.heads);
     h = static_cast<int>(unit - blk * a.Hkv);
     const long long first = static_cast<long long>(blk) * tb;
@@ -317,7 +323,7 @@ __global__ __launch_bounds__(kSlotWaves* kWave) void slot_write_kernel(const Slo
     const int d = PAD ? a.d : D;
     const int ls = PAD ? min(lane % LPR, d / EPL - 1) : lane % LPR;  // 16-byte piece of the row
     const bool owner = !PAD || ls == lane % LPR;
-    const int kv = blockIdx.y;
+    const int kv = blockIdx.y & 1;
     const int64_t stride = kv ? a.v_stride : a.k_stride;
     const char* x = static_cast<const char*>(kv ? a.v_rows : a.k_rows) +
                     (static_cast<int64_t>(h) * a.head_stride + ls * EPL) * (BF16 ? 2 : 4);
@@ -371,7 +377,7 @@ __global__ __launch_bounds__(kSlotWaves* kWave) void slot_read_kernel(const Slot
     const int d = PAD ? a.d : D;
     const int ls = PAD ? min(lane % LPR, d / EPL - 1) : lane % LPR;
     const bool owner = !PAD || ls == lane % LPR;
-    const int kv = blockIdx.y;
+    const int kv = blockIdx.y & 1;
     const int64_t stride = kv ? a.v_stride : a.k_stride;
     char* x = static_cast<char*>(kv ? a.v_rows : a.k_rows) +
               (static_cast<int64_t>(h) * a.head_stride + ls * EPL) * (BF16 ? 2 : 4);
@@ -558,7 +564,7 @@ hipError_t launch_page_map(const PageMapArgs& a, hipStream_t stream) {
 namespace {
 dim3 slot_grid(unsigned rows, unsigned rows_per_group) {
     const unsigned groups = (rows + rows_per_group - 1) / rows_per_group;
-    return dim3(groups < (1u << 20) ? groups : (1u << 20), 2);
+    return dim3(groups < kSlotGroups ? groups : kSlotGroups, 2);
 }
 }  // namespace
 
@@ -571,7 +577,10 @@ hipError_t launch_slots(const SlotArgs& a, bool write, bool vec_ok, hipStream_t 
     // ones, go to the generic kernels.
     if (vec_ok && a.d <= 256 && a.d % (BF16 ? 8 : 4) == 0) {
         auto units = [&](int tb) { return (static_cast<long long>(a.T) + tb - 1) / tb * a.Hkv; };  // waves of K or of V
-        auto grid = [&](int tb) { return dim3(static_cast<unsigned>((units(tb) + kSlotWaves - 1) / kSlotWaves), 2); };
+        auto grid = [&](int tb) {
+            const unsigned groups = static_cast<unsigned>((units(tb) + kSlotWaves - 1) / kSlotWaves);
+            return dim3(groups < kSlotGroups ? groups : kSlotGroups, 2 * ((groups + kSlotGroups - 1) / kSlotGroups));
+        };
 #define KVQ_SLOT_LAUNCH(KERNEL, LOADS) \
     hipLaunchKernelGGL(KERNEL, grid(SlotGeom<DD, BF16, LOADS>::TB), block, 0, stream, a)
 #define KVQ_SLOT_CASE(DIM)                                                                                             \

@@ -30,6 +30,10 @@ bool heads_ok(int num_kv_heads, int head_dim) {
 // The tuned bounds kernels address a page's keys with 32-bit offsets.
 bool page_fits(int page_size, int head_dim) { return static_cast<long long>(page_size) * head_dim < (1LL << 30); }
 
+// Sequences of a bounds launch and (sequence, kv head)s of a selection lie along
+// the grid's x in workgroups of 256 and 512 threads: below 2^32 of them.
+constexpr long long kMaxBoundsBatch = (1LL << 24) - 1, kMaxSelectUnits = (1LL << 23) - 1;
+
 // n rows `stride` elements apart lie within an address space.
 bool spans(int64_t n, int64_t stride) { return n <= 1 || stride <= (1LL << 46) / n; }
 
@@ -99,6 +103,7 @@ bool sparse_params_ok(const kvq_sparse_decode_params* p) {
     if (!p->bounds || !p->bound_scale || !p->selected || !p->selected_lengths) return false;
     const kvq_paged_decode_params& s = p->decode;
     const long long units = static_cast<long long>(s.batch) * s.num_kv_heads;
+    if (units > kMaxSelectUnits) return false;
     if (static_cast<long long>(s.num_pages) * s.num_kv_heads > INT_MAX || units * p->max_selected > INT_MAX) return false;
     return static_cast<long long>(p->max_selected) * s.page_size <= INT_MAX;
 }
@@ -227,8 +232,8 @@ hipError_t kvq_slot_read_launch(const kvq_slot_read_params* p, hipStream_t strea
 }
 
 hipError_t kvq_page_bounds_launch(const kvq_page_bounds_params* p, hipStream_t stream) {
-    if (!p || p->batch <= 0 || !heads_ok(p->num_kv_heads, p->head_dim) || p->page_size <= 0 || p->num_pages <= 0 ||
-        p->max_pages_per_seq <= 0 || p->max_seq_len < 0 || (!p->lengths && p->max_seq_len == 0))
+    if (!p || p->batch <= 0 || p->batch > kMaxBoundsBatch || !heads_ok(p->num_kv_heads, p->head_dim) ||
+        p->page_size <= 0 || p->num_pages <= 0 || p->max_pages_per_seq <= 0 || p->max_seq_len < 0 || (!p->lengths && p->max_seq_len == 0))
         return hipErrorInvalidValue;
     const long long cap = static_cast<long long>(p->max_pages_per_seq) * p->page_size;
     if (cap > INT_MAX || p->max_seq_len > cap || (p->max_seq_len > 0 ? p->max_seq_len : cap) > KVQ_MAX_SEQ_LEN ||

@@ -485,7 +485,7 @@ typedef struct kvq_slot_read_params {
 hipError_t kvq_slot_read_launch(const kvq_slot_read_params* p, hipStream_t stream);
 
 typedef struct kvq_page_bounds_params {
-    int batch, num_kv_heads, head_dim;
+    int batch, num_kv_heads, head_dim; /* batch < 2^24 */
     int page_size, num_pages, max_pages_per_seq; /* max_pages_per_seq * num_kv_heads must fit an int */
     int max_seq_len;            /* as kvq_paged_decode_params */
     const int32_t* block_table; /* device [B, max_pages_per_seq] */
@@ -539,7 +539,7 @@ typedef struct kvq_sparse_decode_params {
  * selected_lengths tokens.
  * Workspace as for kvq_paged_decode_launch: kvq_sparse_decode_workspace_size
  * bytes, zero-filled once, left ready by every completed launch.  num_pages * Hkv
- * and B * Hkv * max_selected must fit an int. */
+ * and B * Hkv * max_selected must fit an int, and B * Hkv must be below 2^23. */
 size_t kvq_sparse_decode_workspace_size(const kvq_sparse_decode_params* p);
 hipError_t kvq_sparse_decode_launch(const kvq_sparse_decode_params* p, void* workspace, size_t workspace_bytes,
                                     hipStream_t stream);

@@ -80,9 +80,12 @@ def _workspace(key, nbytes: int, device) -> Tensor:
         if ws is not None and ws.numel() >= nbytes:
             return ws
         size = max(nbytes, 2 * ws.numel() if ws is not None else 0, 1)
-        new = torch.empty(size, dtype=torch.uint8, device=device)
-        kvq.workspace_init(new, size)
-        if torch.cuda.is_current_stream_capturing():
+        # Both speak of the current device's stream, which need not be this one's.
+        with torch.cuda.device(device):
+            new = torch.empty(size, dtype=torch.uint8, device=device)
+            kvq.workspace_init(new, size)
+            capturing = torch.cuda.is_current_stream_capturing()
+        if capturing:
             # Allocated from the graph's private pool; the zero-fill kernel is
             # part of the graph and has not run yet.  Only this graph may use
             # it (kept alive for its replays).

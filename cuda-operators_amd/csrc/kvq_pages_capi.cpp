@@ -122,13 +122,25 @@ SparsePlan sparse_plan(const kvq_sparse_decode_params* p) {
     s.block_table = p->selected;
     s.lengths = p->selected_lengths;
     if (s.num_splits == 0) {
-        // Nearly every sequence attends the same number of tokens, so the split
-        // count of a uniform batch, over at least two tiles a wave, beats the
-        // plans for ragged ones: 8 heads of 4096 tokens 24.0 us a step with
-        // those, 20.3 in 16 splits (21.0 in 8, 21.7 in 32, 41.4 unsplit); 128 units
-        // of 4096 tokens 47.3 us, 41.2 in 2 splits (55.0 unsplit, 42.5 in 4); 256
-        // units of 2048 tokens, whose ragged plan has a launch of its own, 85.0 us,
-        // 43.5 unsplit.
+        // Sequences longer than the selection attend the same number of tokens,
+        // so the split count of a uniform batch, over at least two tiles a wave,
+        // beats the plans for ragged ones: 8 heads of 4096 tokens 24.0 us a step
+        // with those, 20.3 in 16 splits (21.0 in 8, 21.7 in 32, 41.4 unsplit); 128
+        // units of 4096 tokens 47.3 us, 41.2 in 2 splits (55.0 unsplit, 42.5 in 4);
+        // 256 units of 2048 tokens, whose ragged plan has a launch of its own, 85.0
+        // us, 43.5 unsplit.  It is not the best count of long selections (8192
+        // tokens: 192 units 95.8 us unsplit, 88.4 in 4; 96 units 55.9 in 2, 53.2
+        // in 8).
+        // It is taken where the sequences fit the selection as well, whose lengths
+        // may be anything; there the dense step, planned for ragged lengths, is the
+        // faster one (G = 4, d = 128, sparse / dense step: 16 sequences of 512 to
+        // 8192 tokens 42.8 / 28.5 us, 2048 to 32768 131.6 / 79, 64 of 512 to 8192
+        // 129 / 82; all of 8192 48.8 / 52 and 169 / 181).
+        // The count goes on as a request, which the planner's rules for small steps
+        // leave alone; with them (the uniform plan's kernel too) 3 to 7 heads over
+        // 512 tokens take 15.4-18.2 us for 16.6-18.4, but twelve heads over 32
+        // tokens of 2048 units 58.8 for 44.7, and the generic kernel over 2112
+        // tokens, in 7 splits instead of 8, 288 for 247.
         kvq_paged_decode_params u = s;
         u.lengths = nullptr;
         kvq_plan_info info;

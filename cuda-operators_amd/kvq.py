@@ -153,6 +153,50 @@ class SparseDecodeParams(ctypes.Structure):
     ]
 
 
+CHUNK_MAX_BATCH = 4096  # KVQ_CHUNK_MAX_BATCH
+FORK_MAX_BATCH = 4096   # KVQ_FORK_MAX_BATCH
+
+
+class ChunkAttentionParams(ctypes.Structure):
+    """struct kvq_chunk_attention_params (include/kvq.h)."""
+    _fields_ = [
+        ("batch", _int), ("num_q_heads", _int), ("num_kv_heads", _int), ("head_dim", _int), ("page_size", _int),
+        ("num_pages", _int), ("max_pages_per_seq", _int), ("max_seq_len", _int), ("tokens", _int), ("dtype", _int),
+        ("causal", _int), ("token_offsets", _vp), ("lengths", _vp), ("granted", _vp), ("block_table", _vp), ("q", _vp),
+        ("q_stride", _i64), ("k_pages", _vp), ("v_pages", _vp), ("k_scale_pages", _vp), ("v_scale_pages", _vp),
+        ("out", _vp), ("out_stride", _i64), ("softmax_scale", ctypes.c_float),
+    ]
+
+
+class PageForkParams(ctypes.Structure):
+    """struct kvq_page_fork_params (include/kvq.h)."""
+    _fields_ = [
+        ("batch", _int), ("page_size", _int), ("num_pages", _int), ("max_pages_per_seq", _int), ("parents", _vp),
+        ("keep", _vp), ("lengths", _vp), ("block_table", _vp), ("shares", _vp), ("free_pages", _vp), ("free_count", _vp),
+        ("new_lengths", _vp), ("new_block_table", _vp), ("new_shares", _vp), ("new_free_count", _vp), ("copy_src", _vp),
+        ("copy_dst", _vp),
+    ]
+
+
+class PageCopyParams(ctypes.Structure):
+    """struct kvq_page_copy_params (include/kvq.h)."""
+    _fields_ = [
+        ("copies", _int), ("layers", _int), ("num_kv_heads", _int), ("head_dim", _int), ("page_size", _int),
+        ("num_pages", _int), ("src", _vp), ("dst", _vp), ("k_pages", _vp), ("v_pages", _vp), ("k_scale_pages", _vp),
+        ("v_scale_pages", _vp), ("bounds", _vp), ("bound_scale", _vp),
+    ]
+
+
+class PageCompactParams(ctypes.Structure):
+    """struct kvq_page_compact_params (include/kvq.h)."""
+    _fields_ = [
+        ("batch", _int), ("page_size", _int), ("num_pages", _int), ("max_pages_per_seq", _int), ("max_moves", _int),
+        ("lengths", _vp), ("block_table", _vp), ("shares", _vp), ("free_pages", _vp), ("free_count", _vp),
+        ("new_block_table", _vp), ("new_shares", _vp), ("new_free_pages", _vp), ("copy_src", _vp), ("copy_dst", _vp),
+        ("moved", _vp),
+    ]
+
+
 class PlanInfo(ctypes.Structure):
     """struct kvq_plan_info (include/kvq.h part 6)."""
     _fields_ = [
@@ -174,7 +218,9 @@ EXPORTS = ("solve", "kv_int8_split_launch", "kv_int8_simple_launch", "kvq_decode
            "kvq_diagnostics", "kvq_decode_launch_noalloc", "kvq_paged_decode_plan",
            "kvq_page_map_workspace_size", "kvq_page_map_launch", "kvq_slot_write_launch", "kvq_slot_read_launch",
            "kvq_page_bounds_launch", "kvq_sparse_decode_workspace_size", "kvq_sparse_decode_launch",
-           "kvq_sparse_decode_plan")
+           "kvq_sparse_decode_plan", "kvq_chunk_attention_workspace_size", "kvq_chunk_attention_launch",
+           "kvq_page_fork_workspace_size", "kvq_page_fork_launch", "kvq_page_copy_launch",
+           "kvq_page_compact_workspace_size", "kvq_page_compact_launch")
 
 
 class KvqError(RuntimeError):
@@ -248,6 +294,13 @@ def lib() -> ctypes.CDLL:
         L.kvq_sparse_decode_launch.restype = _int
         L.kvq_sparse_decode_plan.argtypes = [ctypes.POINTER(SparseDecodeParams), ctypes.POINTER(PlanInfo)]
         L.kvq_sparse_decode_plan.restype = _int
+        for fn, cls in (("kvq_chunk_attention", ChunkAttentionParams), ("kvq_page_fork", PageForkParams),
+                        ("kvq_page_compact", PageCompactParams)):
+            size, launch = getattr(L, fn + "_workspace_size"), getattr(L, fn + "_launch")
+            size.argtypes, size.restype = [ctypes.POINTER(cls)], ctypes.c_size_t
+            launch.argtypes, launch.restype = [ctypes.POINTER(cls), _vp, ctypes.c_size_t, _vp], _int
+        L.kvq_page_copy_launch.argtypes = [ctypes.POINTER(PageCopyParams), _vp]
+        L.kvq_page_copy_launch.restype = _int
         _lib = L
         return L
 
@@ -873,6 +926,209 @@ def sparse_decode_plan(p: SparseDecodeParams) -> PlanInfo:
     return info
 
 
+# ---------------------------------------------------------------------------
+# chunks of new tokens, shared pages (include/kvq.h part 8)
+# ---------------------------------------------------------------------------
+def _token_stride(t, dtype, shape, name):
+    """Elements from a token to the next of a [T, H, d] tensor whose tokens' heads lie together (0: one token)."""
+    s = _check_rows(t, dtype, shape, name)
+    T, H, d = shape
+    if (s[1] != d and H > 1) or (s[0] < H * d and T > 1):
+        raise ValueError(f"{name}: a token's heads must lie together, got strides {s}")
+    return s[0] if T > 1 else 0
+
+
+def _table_of(t, B, name="block_table"):
+    if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.shape[0] != B:
+        raise ValueError(f"{name}: want [B, max_pages_per_seq]")
+    _needs((t, torch.int32, t.shape, name))
+    return int(t.shape[1])
+
+
+class _Planned:
+    """A call with its parameters and workspace: checked once, launched as often as one likes."""
+
+    def _plan(self, name, params, tensors, stream, workspace):
+        self.params, self.device = params, _one_device(*tensors)
+        fn = getattr(lib(), name + "_workspace_size")
+        self.ws_bytes = int(fn(ctypes.byref(params)))
+        self.ws = workspace(self.ws_bytes) if workspace and self.ws_bytes else _new_workspace(self.ws_bytes, self.device, stream)
+        self._keep = tuple(tensors) + (self.ws,)
+        self._name, self._launch = name + "_launch", getattr(lib(), name + "_launch")
+        self._args = (ctypes.byref(params), _ptr(self.ws), self.ws_bytes)
+
+    def __call__(self, stream=None) -> None:
+        """Launch on `stream` (a torch stream or a raw hipStream_t handle; default: torch's current stream)."""
+        _call(self._launch, self._name, self._args, self.device, stream, self._keep)
+
+
+class ChunkAttention(_Planned):
+    """kvq_chunk_attention_launch with its workspace: build once, launch for every batch of the same tensors.
+
+    q and out [T, Hq, d] fp32 or bf16, tokens any stride apart; token_offsets [B + 1], lengths [B] and granted [B] (or
+    None) int32, as a PageMapper writes them: sequence b's new tokens are rows token_offsets[b] to token_offsets[b + 1],
+    the last of its lengths[b] tokens, which its pages hold already.  causal: each attends the tokens up to itself, else
+    all of its sequence (an encoder's states).  Rows of refused sequences, and without a token to attend, become zeros;
+    rows behind the last sequence stay.  workspace: as PageMapper's."""
+
+    def __init__(self, q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, lengths, token_offsets, out,
+                 granted=None, causal=True, max_seq_len=0, softmax_scale=0.0, stream=None, workspace=None):
+        P_, Hkv, page, d = _check_pool(k_pages, v_pages, k_scale_pages, v_scale_pages)
+        if q.dim() != 3 or q.shape[2] != d or q.shape[1] % Hkv:
+            raise ValueError(f"q: want [T, a multiple of {Hkv}, {d}], got {tuple(q.shape)}")
+        code = _dtype_code(q, "q")
+        T, Hq, _ = shape = q.shape
+        strides = [_token_stride(t, q.dtype, shape, n) for t, n in ((q, "q"), (out, "out"))]
+        B = _rows_of(lengths, "lengths")
+        per = _table_of(block_table, B)
+        _rows_of(token_offsets, "token_offsets", B + 1)
+        if granted is not None:
+            _rows_of(granted, "granted", B)
+        tensors = (q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, lengths, token_offsets, out, granted)
+        p = ChunkAttentionParams(B, Hq, Hkv, d, page, P_, per, int(max_seq_len), T, code, int(bool(causal)),
+                                 _ptr(token_offsets), _ptr(lengths), _ptr(granted), _ptr(block_table), _pad_ptr(q),
+                                 strides[0], _ptr(k_pages), _ptr(v_pages), _ptr(k_scale_pages), _ptr(v_scale_pages),
+                                 _pad_ptr(out), strides[1], float(softmax_scale))
+        self.out = out
+        self._plan("kvq_chunk_attention", p, tensors, stream, workspace)
+
+
+def _pad_ptr(t):
+    """A tensor's address; of an empty one some address that is not null (nothing there is read or written)."""
+    return t.data_ptr() or 4096
+
+
+def chunk_attention(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, lengths, token_offsets, out=None,
+                    stream=None, **options) -> torch.Tensor:
+    """One chunk attention (ChunkAttention's arguments); returns out (default: a new tensor, zero where no sequence has
+    a row)."""
+    if out is None:
+        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    ChunkAttention(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, lengths, token_offsets, out,
+                   stream=stream, **options)(stream)
+    return out
+
+
+class PageForker(_Planned):
+    """kvq_page_fork_launch with its outputs and workspace: build once, launch whenever rows go on from other rows.
+
+    parents [B] (the row each goes on from; outside [0, B): none), keep [B] (tokens of it to keep) or None, lengths [B],
+    block_table [B, max_pages], shares [num_pages] (holders beyond the first: new_shares), free_pages [num_pages] (a
+    stack) and free_count [1], all int32.  lengths, block_table, shares and free_count are updated in place unless the
+    new_ tensors are given; free_pages always is.  copy_src and copy_dst [B] name the pages to copy (page_copy) before
+    anything else is written.  Every output is an attribute.  workspace: as PageMapper's."""
+
+    def __init__(self, parents, lengths, block_table, shares, free_pages, free_count, page_size, keep=None,
+                 new_lengths=None, new_block_table=None, new_shares=None, new_free_count=None, copy_src=None,
+                 copy_dst=None, stream=None, workspace=None):
+        B = _rows_of(parents, "parents")
+        per = _table_of(block_table, B)
+        num = _rows_of(free_pages, "free_pages")
+        for name, t, n in (("lengths", lengths, B), ("shares", shares, num), ("free_count", free_count, 1)):
+            _rows_of(t, name, n)
+        for name, t, n in (("keep", keep, B), ("new_lengths", new_lengths, B), ("new_shares", new_shares, num),
+                           ("new_free_count", new_free_count, 1), ("copy_src", copy_src, B), ("copy_dst", copy_dst, B)):
+            if t is not None:
+                _rows_of(t, name, n)
+        if new_block_table is not None and _table_of(new_block_table, B, "new_block_table") != per:
+            raise ValueError("new_block_table: want block_table's shape")
+        empty = lambda n: torch.empty(n, dtype=torch.int32, device=parents.device)  # noqa: E731
+        self.new_lengths = lengths if new_lengths is None else new_lengths
+        self.new_block_table = block_table if new_block_table is None else new_block_table
+        self.new_shares = shares if new_shares is None else new_shares
+        self.new_free_count = free_count if new_free_count is None else new_free_count
+        self.free_pages = free_pages
+        self.copy_src = empty(B) if copy_src is None else copy_src
+        self.copy_dst = empty(B) if copy_dst is None else copy_dst
+        tensors = (parents, keep, lengths, block_table, shares, free_pages, free_count, self.new_lengths,
+                   self.new_block_table, self.new_shares, self.new_free_count, self.copy_src, self.copy_dst)
+        self._plan("kvq_page_fork", PageForkParams(B, int(page_size), num, per, *(_ptr(t) for t in tensors)), tensors,
+                   stream, workspace)
+
+
+def page_fork(parents, lengths, block_table, shares, free_pages, free_count, page_size, stream=None, **outputs) -> PageForker:
+    """One fork (PageForker's arguments); returns the PageForker, whose attributes are the outputs."""
+    f = PageForker(parents, lengths, block_table, shares, free_pages, free_count, page_size, stream=stream, **outputs)
+    f(stream)
+    return f
+
+
+def new_shares(free_pages) -> torch.Tensor:
+    """Holders beyond the first for a pool of free_pages' size in which no page is shared."""
+    return torch.zeros_like(free_pages)
+
+
+def page_copy(copy_src, copy_dst, k_pages, v_pages, k_scale_pages, v_scale_pages, bounds=None, bound_scale=None,
+              stream=None) -> None:
+    """Copy pages copy_src[i] to copy_dst[i] (int32; -1: none) within a pool (kvq_page_copy_launch).
+
+    A pool is [num_pages, Hkv, page_size, d], or [layers, num_pages, ...] for all layers at once (scales and bounds
+    alike)."""
+    if k_pages.dim() not in (4, 5):
+        raise ValueError("k_pages: want [num_pages, Hkv, page_size, d] or [layers, num_pages, Hkv, page_size, d]")
+    shape = tuple(k_pages.shape)
+    *lead, Hkv, page, d = shape
+    scales = shape[:-1]
+    _needs((k_pages, _I8, shape, "k_pages"), (v_pages, _I8, shape, "v_pages"),
+           (k_scale_pages, _F32, scales, "k_scale_pages"), (v_scale_pages, _F32, scales, "v_scale_pages"))
+    if (bounds is None) != (bound_scale is None):
+        raise ValueError("bounds and bound_scale must be given together")
+    if bounds is not None:
+        _needs((bounds, _I8, (*lead, Hkv, 2, d), "bounds"), (bound_scale, _F32, (*lead, Hkv), "bound_scale"))
+    n = _rows_of(copy_src, "copy_src")
+    _rows_of(copy_dst, "copy_dst", n)
+    tensors = (copy_src, copy_dst, k_pages, v_pages, k_scale_pages, v_scale_pages, bounds, bound_scale)
+    index = _one_device(*tensors)
+    if n == 0:
+        return
+    p = PageCopyParams(n, lead[0] if len(lead) == 2 else 1, Hkv, d, page, lead[-1], *(_ptr(t) for t in tensors))
+    _call(lib().kvq_page_copy_launch, "kvq_page_copy_launch", (ctypes.byref(p),), index, stream, tensors)
+
+
+class PageCompactor(_Planned):
+    """kvq_page_compact_launch with its outputs and workspace: moves pages in use to the front of a pool.
+
+    lengths [B], block_table [B, max_pages], shares [num_pages] (or None where no page is shared), free_pages
+    [num_pages] (a stack) and free_count [1], all int32; the table, shares and the stack are updated in place unless the
+    new_ tensors are given.  At most max_moves pages move: copy_src and copy_dst [max_moves] name them (page_copy), moved
+    [1] says how many.  Every output is an attribute.  workspace: as PageMapper's."""
+
+    def __init__(self, lengths, block_table, shares, free_pages, free_count, page_size, max_moves=None,
+                 new_block_table=None, new_shares=None, new_free_pages=None, copy_src=None, copy_dst=None, moved=None,
+                 stream=None, workspace=None):
+        B = _rows_of(lengths, "lengths")
+        per = _table_of(block_table, B)
+        num = _rows_of(free_pages, "free_pages")
+        _rows_of(free_count, "free_count", 1)
+        max_moves = num if max_moves is None else int(max_moves)
+        if shares is None and new_shares is not None:
+            raise ValueError("new_shares without shares")
+        for name, t, n in (("shares", shares, num), ("new_shares", new_shares, num), ("new_free_pages", new_free_pages, num),
+                           ("copy_src", copy_src, max_moves), ("copy_dst", copy_dst, max_moves), ("moved", moved, 1)):
+            if t is not None:
+                _rows_of(t, name, n)
+        if new_block_table is not None and _table_of(new_block_table, B, "new_block_table") != per:
+            raise ValueError("new_block_table: want block_table's shape")
+        empty = lambda n: torch.empty(max(n, 0), dtype=torch.int32, device=lengths.device)  # noqa: E731
+        self.new_block_table = block_table if new_block_table is None else new_block_table
+        self.new_shares = shares if new_shares is None else new_shares
+        self.new_free_pages = free_pages if new_free_pages is None else new_free_pages
+        self.copy_src = empty(max_moves) if copy_src is None else copy_src
+        self.copy_dst = empty(max_moves) if copy_dst is None else copy_dst
+        self.moved = empty(1) if moved is None else moved
+        tensors = (lengths, block_table, shares, free_pages, free_count, self.new_block_table, self.new_shares,
+                   self.new_free_pages, self.copy_src, self.copy_dst, self.moved)
+        self._plan("kvq_page_compact", PageCompactParams(B, int(page_size), num, per, max_moves, *(_ptr(t) for t in tensors)),
+                   tensors, stream, workspace)
+
+
+def page_compact(lengths, block_table, shares, free_pages, free_count, page_size, stream=None, **outputs) -> PageCompactor:
+    """One compaction (PageCompactor's arguments); returns the PageCompactor, whose attributes are the outputs."""
+    c = PageCompactor(lengths, block_table, shares, free_pages, free_count, page_size, stream=stream, **outputs)
+    c(stream)
+    return c
+
+
 def _attention_shapes(q, k, v, out):
     M, d = q.shape
     N = k.shape[0]
@@ -982,4 +1238,7 @@ __all__ = ["lib", "version", "solve", "kv_int8_split_launch", "DecodeParams", "A
            "attention", "PlanInfo", "reference_plan", "decode_plan", "paged_decode_plan", "attention_plan", "diagnostics",
            "attention_lib", "attention_solve", "decode_launch_noalloc", "NOALLOC_SCRATCH_BYTES", "PAGE_MAP_MAX_BATCH",
            "PageMapParams", "SlotWriteParams", "SlotReadParams", "PageBoundsParams", "SparseDecodeParams", "PageMapper",
-           "page_map", "slot_write", "slot_read", "new_bounds", "page_bounds", "SparseDecoder", "sparse_decode_plan"]
+           "page_map", "slot_write", "slot_read", "new_bounds", "page_bounds", "SparseDecoder", "sparse_decode_plan",
+           "CHUNK_MAX_BATCH", "FORK_MAX_BATCH", "ChunkAttentionParams", "PageForkParams", "PageCopyParams",
+           "PageCompactParams", "ChunkAttention", "chunk_attention", "PageForker", "page_fork", "new_shares", "page_copy",
+           "PageCompactor", "page_compact"]

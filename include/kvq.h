@@ -547,6 +547,162 @@ hipError_t kvq_sparse_decode_launch(const kvq_sparse_decode_params* p, void* wor
  * whole call's.  Host-only (as part 6). */
 hipError_t kvq_sparse_decode_plan(const kvq_sparse_decode_params* p, kvq_plan_info* info);
 
+/* ============ Part 8: chunks of new tokens, shared pages (no counterpart in the reference) ============
+ *
+ *   kvq_chunk_attention_launch  attention of a packed batch of new tokens over their sequences' pages
+ *   kvq_page_fork_launch        rows that go on from other rows' tokens on pages they share; cuts and ends
+ *   kvq_page_copy_launch        pages copied within a pool
+ *   kvq_page_compact_launch     pages in use moved to the front of a pool
+ * Layouts, block tables and slots are those of parts 3 and 7.  Every entry point
+ * returns hipErrorInvalidValue before any HIP call on a bad argument, is
+ * asynchronous on `stream`, allocates nothing and can be captured. */
+
+/* Most sequences of one chunk attention, and most rows of one fork or compaction. */
+#define KVQ_CHUNK_MAX_BATCH 4096
+#define KVQ_FORK_MAX_BATCH 4096
+
+typedef struct kvq_chunk_attention_params {
+    int batch;               /* B in [1, KVQ_CHUNK_MAX_BATCH] */
+    int num_q_heads;         /* Hq >= 1, a multiple of num_kv_heads */
+    int num_kv_heads;        /* Hkv >= 1 */
+    int head_dim;            /* d in [1, KVQ_MAX_HEAD_DIM] */
+    int page_size, num_pages, max_pages_per_seq;
+    int max_seq_len;         /* a bound on every lengths[b] (0: max_pages_per_seq * page_size) */
+    int tokens;              /* T >= 0: rows of q and out; T * num_q_heads < 2^31 */
+    int dtype;               /* of q and out: KVQ_DTYPE_F32 or KVQ_DTYPE_BF16 */
+    int causal;              /* not 0: a token attends the tokens up to itself; 0: all of its sequence */
+    const int32_t* token_offsets; /* device [B + 1], ascending: sequence b's new tokens are rows
+                                [token_offsets[b], token_offsets[b + 1]) (kvq_page_map_launch's) */
+    const int32_t* lengths;  /* device [B]: tokens held, the new ones among them; clamped on device to [0, max_seq_len] */
+    const int32_t* granted;  /* device [B] or NULL: a sequence with granted[b] <= 0 gets zero rows */
+    const int32_t* block_table; /* device [B, max_pages_per_seq] */
+    const void* q;           /* [T, Hq, d]: a token's heads lie together */
+    int64_t q_stride;        /* elements from a token to the next, >= Hq * d (0: Hq * d) */
+    const int8_t* k_pages;   /* [num_pages, Hkv, page_size, d] */
+    const int8_t* v_pages;
+    const float* k_scale_pages; /* [num_pages, Hkv, page_size] */
+    const float* v_scale_pages;
+    void* out;               /* [T, Hq, d] */
+    int64_t out_stride;      /* as q_stride */
+    float softmax_scale;     /* <= 0 selects 1/sqrtf(d) */
+} kvq_chunk_attention_params;
+
+/* Attention of new tokens (prompt chunks, drafts to verify, single tokens, in one
+ * batch) over the pages of their sequences, which already hold them (write them
+ * with kvq_slot_write_launch first).  New token i of sequence b, of n_b, stands at
+ * position lengths[b] - n_b + i; with `causal` it attends the tokens up to that
+ * position, without (the states of an encoder, say) all lengths[b] of them.  A row
+ * with no token to attend is zero; rows at or behind token_offsets[B] are left as
+ * they are.  The math is part 1's for each row; bf16 outputs are rounded once.
+ * A contiguous cache [B, Hkv, capacity, d] is a pool of B pages of `capacity`
+ * tokens with the block table 0, 1, .., B - 1.
+ * Workspace: kvq_chunk_attention_workspace_size bytes, zero-filled once
+ * (kvq_workspace_init) and left ready by every completed launch; calls that may
+ * overlap in time need separate ones. */
+size_t kvq_chunk_attention_workspace_size(const kvq_chunk_attention_params* p);
+hipError_t kvq_chunk_attention_launch(const kvq_chunk_attention_params* p, void* workspace, size_t workspace_bytes,
+                                      hipStream_t stream);
+
+typedef struct kvq_page_fork_params {
+    int batch;               /* B in [1, KVQ_FORK_MAX_BATCH] */
+    int page_size;           /* >= 1 */
+    int num_pages;           /* num_pages * page_size <= INT_MAX */
+    int max_pages_per_seq;   /* row stride of both tables */
+    const int32_t* parents;  /* device [B]: the row that row b goes on from; outside [0, B): none, row b ends */
+    const int32_t* keep;     /* device [B]: tokens of the parent to keep (clamped to [0, what it has]), or NULL: all */
+    const int32_t* lengths;  /* device [B]: tokens held, each clamped to [0, capacity] */
+    const int32_t* block_table; /* device [B, max_pages_per_seq] */
+    const int32_t* shares;   /* device [num_pages]: holders of a page beyond the first (0: one holder, or free) */
+    int32_t* free_pages;     /* device [num_pages]: the free stack, updated in place */
+    const int32_t* free_count; /* device [1]: its entries, clamped to [0, num_pages] */
+    int32_t* new_lengths;    /* device [B]; may be `lengths` */
+    int32_t* new_block_table; /* device [B, max_pages_per_seq]; may be `block_table` */
+    int32_t* new_shares;     /* device [num_pages], wholly written; may be `shares` */
+    int32_t* new_free_count; /* device [1]; may be `free_count` */
+    int32_t* copy_src;       /* device [B]: the page to copy for row b, or -1 */
+    int32_t* copy_dst;       /* device [B]: to this page, or -1 */
+} kvq_page_fork_params;
+
+/* Every row of a batch goes on from the first tokens of a row (itself, another,
+ * none): copies of a conversation, beams of a search, cuts, ends, a batch put into
+ * another order.
+ * - Row b gets the first n_b = min(keep[b], length of its parent) tokens of its
+ *   parent and shares the pages that hold them.
+ * - shares counts a page's holders, every table row and whatever else holds it
+ *   (a prefix kept by the caller: one more in shares); a page that loses its last
+ *   holder is free.  Pages that have become free go onto the stack in ascending order.
+ * - A row that ends inside a page will write there.  If others hold the page, the
+ *   row gets a page of its own and the pair to copy in copy_src[b], copy_dst[b]
+ *   (kvq_page_copy_launch, before anything else is written); if all its holders
+ *   end inside it, the first row of them keeps it.  The i-th such row takes the
+ *   i-th page from the stack's top, those freed by this call first; a row for
+ *   which none is left keeps its whole pages only: new_lengths[b] says how many
+ *   tokens that are, and the caller writes the others again.
+ * - A row's entries behind its last page, and the stack behind its end, have no
+ *   meaning and are left as they were (so in a new_block_table of its own too).
+ *   Table entries outside the pool are carried along, not counted.
+ * - kvq_page_map_launch gives pages up without a look at shares: where pages are
+ *   shared, rows are cut and ended here and grow there.
+ * Workspace: kvq_page_fork_workspace_size bytes, zero-filled once and left ready.
+ * Calls on one pool must be ordered. */
+size_t kvq_page_fork_workspace_size(const kvq_page_fork_params* p);
+hipError_t kvq_page_fork_launch(const kvq_page_fork_params* p, void* workspace, size_t workspace_bytes,
+                                hipStream_t stream);
+
+typedef struct kvq_page_copy_params {
+    int copies;               /* n >= 0 pairs */
+    int layers;               /* pools of the same shape one behind the other, >= 1 */
+    int num_kv_heads, head_dim;
+    int page_size, num_pages; /* of one layer's pool; num_pages * page_size <= INT_MAX */
+    const int32_t* src;       /* device [n] */
+    const int32_t* dst;       /* device [n]; a pair with a page outside the pool copies nothing */
+    int8_t* k_pages;          /* [layers, num_pages, Hkv, page_size, d] */
+    int8_t* v_pages;
+    float* k_scale_pages;     /* [layers, num_pages, Hkv, page_size] */
+    float* v_scale_pages;
+    int8_t* bounds;           /* [layers, num_pages, Hkv, 2, d] with bound_scale, or both NULL */
+    float* bound_scale;       /* [layers, num_pages, Hkv] */
+} kvq_page_copy_params;
+
+/* Copies whole pages, in every layer.  The pages of dst are distinct and none of
+ * them is a src (kvq_page_fork_launch's and kvq_page_compact_launch's are); a src
+ * may be copied several times. */
+hipError_t kvq_page_copy_launch(const kvq_page_copy_params* p, hipStream_t stream);
+
+typedef struct kvq_page_compact_params {
+    int batch;               /* B in [1, KVQ_FORK_MAX_BATCH] */
+    int page_size;           /* >= 1 */
+    int num_pages;           /* num_pages * page_size <= INT_MAX */
+    int max_pages_per_seq;   /* row stride of both tables */
+    int max_moves;           /* >= 1: most pages moved by this call */
+    const int32_t* lengths;  /* device [B]: tokens held, each clamped to [0, capacity] */
+    const int32_t* block_table; /* device [B, max_pages_per_seq] */
+    const int32_t* shares;   /* device [num_pages] (as kvq_page_fork_params), or NULL with new_shares */
+    const int32_t* free_pages; /* device [num_pages]: the free stack, distinct pages of the pool */
+    const int32_t* free_count; /* device [1]: its entries, clamped to [0, num_pages]; stays what it is */
+    int32_t* new_block_table; /* device [B, max_pages_per_seq]; may be `block_table` */
+    int32_t* new_shares;     /* device [num_pages], wholly written (a free page: 0); may be `shares` */
+    int32_t* new_free_pages; /* device [num_pages]; may be `free_pages` */
+    int32_t* copy_src;       /* device [max_moves]: pages to copy, then -1 */
+    int32_t* copy_dst;       /* device [max_moves] */
+    int32_t* moved;          /* device [1]: pages moved */
+} kvq_page_compact_params;
+
+/* Moves pages in use to the front of the pool.  With U pages not on the free
+ * stack, whoever holds them, the i-th highest of those at or behind U moves to the
+ * i-th lowest free page before U, for the first max_moves i; after a call that
+ * moves fewer than max_moves, the pages in use are 0 .. U - 1.  Tables (entries of
+ * pages that a row holds), shares and the free stack say so afterwards, the stack
+ * with the lowest page on top; the pages themselves are copied with
+ * kvq_page_copy_launch before anything is written or read.  A holder that is no
+ * table row learns the new numbers from copy_src and copy_dst.  Entries behind the
+ * ends of rows and of the stack are left as they were.
+ * Workspace: kvq_page_compact_workspace_size bytes, zero-filled once and left
+ * ready.  Calls on one pool must be ordered. */
+size_t kvq_page_compact_workspace_size(const kvq_page_compact_params* p);
+hipError_t kvq_page_compact_launch(const kvq_page_compact_params* p, void* workspace, size_t workspace_bytes,
+                                   hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

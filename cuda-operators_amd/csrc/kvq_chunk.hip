@@ -2,6 +2,8 @@
 #include <limits.h>
 #include <math.h>
 
+#include <algorithm>
+
 #include "kvq_chunk.hpp"
 #include "kvq_device.hpp"
 
@@ -95,9 +97,66 @@ __global__ __launch_bounds__(kWave) void chunk_generic(const ChunkArgs a) {
 }
 
 }  // namespace
+}  // namespace kvq
 
-hipError_t launch_chunk(const ChunkArgs& a, bool, void*, hipStream_t stream) {
+#include "kvq_chunk_mfma.hpp"
+
+namespace kvq {
+namespace {
+
+template <int D, int LIMBS>
+hipError_t launch_mfma(const ChunkArgs& a, unsigned items, hipStream_t stream) {
+    hipLaunchKernelGGL((chunk_mfma<D, LIMBS>), dim3(items), dim3(kChunkThreads), 0, stream, a);
+    return hipGetLastError();
+}
+
+int chunk_dim(int d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : d <= 192 ? 192 : 256; }
+
+constexpr size_t kChunkCounters = 256 * 1024;
+
+}  // namespace
+
+ChunkPlan chunk_plan(const ChunkArgs& a, bool vec_ok) {
+    ChunkPlan p{};
+    p.mfma = vec_ok && a.d <= 256 && a.d % 8 == 0 && a.G <= kChunkRows;
+    if (!p.mfma || a.T == 0) return p;
+    p.D = chunk_dim(a.d);
+    p.tile_tokens = kChunkRows / a.G;
+    const long long tiles = std::min<long long>(a.T, a.T / p.tile_tokens + a.B);
+    const long long units = tiles * a.Hkv;
+    const int blocks = (a.max_len + kChunkKeys - 1) / kChunkKeys;
+    p.max_tiles = static_cast<int>(tiles);
+    p.slots = p.D <= 128 ? 512 : 256;
+    p.max_splits = units < p.slots && a.B <= kChunkThreads ? std::min(p.slots, (blocks + 3) / 4) : 1;
+    p.items = static_cast<unsigned>(p.max_splits > 1 ? std::max<long long>(units, std::min<long long>(p.slots, units * p.max_splits)) : units);
+    p.records = p.max_splits > 1 ? p.items : 0;
+    if (p.records) p.bytes = kChunkCounters + p.records * kChunkRows * (p.D + 2) * sizeof(float);
+    return p;
+}
+
+hipError_t launch_chunk(ChunkArgs a, const ChunkPlan& p, void* workspace, hipStream_t stream) {
     if (a.T == 0) return hipSuccess;
+    if (p.mfma) {
+        a.tile_tokens = p.tile_tokens;
+        a.slots = p.slots;
+        a.max_splits = p.max_splits;
+        a.max_tiles = p.max_tiles;
+        a.heads = make_fastdiv(static_cast<uint32_t>(a.Hkv));
+        a.group = make_fastdiv(static_cast<uint32_t>(a.G));
+        a.counters = static_cast<int*>(workspace);
+        a.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + (p.records ? kChunkCounters : 0));
+        a.part_ml = a.part_acc + p.records * kChunkRows * p.D;
+#define KVQ_CHUNK_CASE(DIM) \
+    case DIM: return a.bf16 ? launch_mfma<DIM, 1>(a, p.items, stream) : launch_mfma<DIM, 2>(a, p.items, stream);
+        switch (p.D) {
+            KVQ_CHUNK_CASE(64)
+            KVQ_CHUNK_CASE(96)
+            KVQ_CHUNK_CASE(128)
+            KVQ_CHUNK_CASE(192)
+            KVQ_CHUNK_CASE(256)
+        }
+#undef KVQ_CHUNK_CASE
+    }
     const long long rows = static_cast<long long>(a.T) * a.Hq;
     const unsigned groups = static_cast<unsigned>(rows < (1 << 20) ? rows : (1 << 20));
     const size_t lds = sizeof(float) * (2 * static_cast<size_t>(a.d) + kWave) + sizeof(size_t) * kWave;

@@ -72,11 +72,20 @@ kvq::ChunkArgs chunk_args(const kvq_chunk_attention_params* p) {
     a.d = p->head_dim;
     a.T = p->tokens;
     a.max_len = p->max_seq_len > 0 ? p->max_seq_len : p->max_pages_per_seq * p->page_size;
+    a.page = kvq::make_fastdiv(static_cast<uint32_t>(size));
     a.bf16 = p->dtype == KVQ_DTYPE_BF16;
     a.causal = p->causal != 0;
-    const float scale = p->softmax_scale > 0.0f ? p->softmax_scale : 1.0f / sqrtf(static_cast<float>(p->head_dim));
-    a.scale_log2 = scale * 1.4426950408889634f;
+    // Rounded once: a relative error of it is one of every score.
+    const double scale = p->softmax_scale > 0.0f ? static_cast<double>(p->softmax_scale) : 1.0 / sqrt(static_cast<double>(p->head_dim));
+    a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
     return a;
+}
+
+// Rows of 16-byte pieces, caches of 8-byte ones.
+bool chunk_vec_ok(const kvq_chunk_attention_params* p, const kvq::ChunkArgs& a) {
+    const int64_t size = a.bf16 ? 2 : 4;
+    return ((bits(p->q) | bits(p->out)) & 15u) == 0 && ((bits(p->k_pages) | bits(p->v_pages)) & 7u) == 0 &&
+           a.q_stride * size % 16 == 0 && a.out_stride * size % 16 == 0;
 }
 
 bool fork_params_ok(const kvq_page_fork_params* p) {
@@ -145,16 +154,18 @@ kvq::CompactArgs compact_args(const kvq_page_compact_params* p) {
 extern "C" {
 
 size_t kvq_chunk_attention_workspace_size(const kvq_chunk_attention_params* p) {
-    (void)p;
-    return 0;
+    if (!chunk_params_ok(p)) return 0;
+    const kvq::ChunkArgs a = chunk_args(p);
+    return kvq::chunk_plan(a, chunk_vec_ok(p, a)).bytes;
 }
 
 hipError_t kvq_chunk_attention_launch(const kvq_chunk_attention_params* p, void* workspace, size_t workspace_bytes,
                                       hipStream_t stream) {
     if (!chunk_params_ok(p)) return hipErrorInvalidValue;
-    (void)workspace_bytes;
     const kvq::ChunkArgs a = chunk_args(p);
-    return checked_call(stream, [&] { return kvq::launch_chunk(a, false, workspace, stream); });
+    const kvq::ChunkPlan plan = kvq::chunk_plan(a, chunk_vec_ok(p, a));
+    if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes)) return hipErrorInvalidValue;
+    return checked_call(stream, [&] { return kvq::launch_chunk(a, plan, workspace, stream); });
 }
 
 size_t kvq_page_fork_workspace_size(const kvq_page_fork_params* p) {

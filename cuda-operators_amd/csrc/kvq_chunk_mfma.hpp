@@ -21,6 +21,7 @@ constexpr int kChunkThreads = kChunkWaves * kWave;
 constexpr int kChunkCoherent = 16;  // buffer cache policy sc1: device-coherent
 constexpr float kWeightTop = 15.0f;   // log2 of the largest f16 weight that is let grow,
 constexpr float kWeightReset = 12.0f; // and of what a row's weights are set to when they pass it
+constexpr float kKsMax = 0x1p80f;     // |k scale|s above overflow as scores of q scaled to 2^15
 constexpr float kVsMax = 0x1p40f, kVsMin = 0x1p-40f;  // |v scale|s outside take fp32 weights, as does a
 template <int LIMBS>                                  // tile set whose scales differ by more than this
 constexpr float kVsRatio = LIMBS == 1 ? 0x1p24f : 0x1p14f;
@@ -272,7 +273,7 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
 
     int2 kraw[NP], vraw[NP];
     float ksr = 0.0f, vsr = 0.0f;
-    float vmax = 0.0f, vmin = INFINITY;
+    float vmax = 0.0f, vmin = INFINITY, kmax = 0.0f;
     bool vbad = false;
     auto load_tile = [&](int tile) {
         const long long* rows = s_row[tile & 3];
@@ -305,6 +306,7 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
             buf.ks[lane] = ksr;
             buf.vs[lane] = vsr;
             const float v = fabsf(vsr);
+            kmax = fmaxf(kmax, fabsf(ksr));
             vbad |= !(v < INFINITY);
             vmax = fmaxf(vmax, v);
             if (v > 0.0f) vmin = fminf(vmin, v);
@@ -484,10 +486,10 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
         __syncthreads();
     }
 
-    // V scales that f16 weights do not cover.
+    // Scales that f16 weights, or q scaled to 2^15, do not cover.
     if (wave == 0) {
         const float top = wave_max(vmax), low = -wave_max(-vmin);
-        const bool bad = __builtin_amdgcn_ballot_w64(vbad) != 0 ||
+        const bool bad = __builtin_amdgcn_ballot_w64(vbad || kmax > kKsMax) != 0 ||
                          (top > 0.0f && (top > kVsMax || low < kVsMin || top > low * kVsRatio<LIMBS>));
         if (lane == 0) s_flag = bad;
     }

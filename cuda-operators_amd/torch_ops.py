@@ -39,6 +39,18 @@ allocates nothing once its workspace exists.
       kvq_sparse_decode_launch (mutates the pool with k_new/v_new, and the bounds).
       k_new/v_new of decode, paged_decode and sparse_decode go to every sequence
       of length 1 or more; one without a new token in the step has length 0.
+  torch.ops.kvq.chunk_attention(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, lengths,
+                                token_offsets, granted, causal, max_seq_len, softmax_scale) -> out
+      kvq_chunk_attention_launch of packed rows [T, Hq, d]; rows behind the last sequence are zero.
+  torch.ops.kvq.page_fork(parents, keep, lengths, block_table, shares, free_pages, free_count,
+                          page_size) -> (copy_src, copy_dst)
+      kvq_page_fork_launch in place (mutates all from lengths on).
+  torch.ops.kvq.page_copy(copy_src, copy_dst, k_pages, v_pages, k_scale_pages, v_scale_pages, bounds,
+                          bound_scale) -> ()
+      kvq_page_copy_launch (mutates the pool and the bounds).
+  torch.ops.kvq.page_compact(lengths, block_table, shares, free_pages, free_count, page_size,
+                             max_moves) -> (copy_src, copy_dst, moved)
+      kvq_page_compact_launch in place (mutates block_table, shares and free_pages).
 
 Workspaces are cached per (operator, device, stream) and grown on demand:
 launches on one stream are ordered, so they may share one; launches on
@@ -307,5 +319,62 @@ def _sparse_decode_fake(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block
     return _sparse_outputs(q, k_pages, max_selected)
 
 
+@torch.library.custom_op("kvq::chunk_attention", mutates_args=())
+def chunk_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, k_scale_pages: Tensor, v_scale_pages: Tensor,
+                    block_table: Tensor, lengths: Tensor, token_offsets: Tensor, granted: Optional[Tensor], causal: bool,
+                    max_seq_len: int, softmax_scale: float) -> Tensor:
+    out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    kvq.ChunkAttention(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, lengths, token_offsets, out,
+                       granted=granted, causal=causal, max_seq_len=max_seq_len, softmax_scale=softmax_scale,
+                       workspace=_workspace_for("chunk", q.device))()
+    return out
+
+
+@chunk_attention.register_fake
+def _chunk_attention_fake(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, lengths, token_offsets, granted,
+                          causal, max_seq_len, softmax_scale):
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+
+@torch.library.custom_op("kvq::page_fork", mutates_args=("lengths", "block_table", "shares", "free_pages", "free_count"))
+def page_fork(parents: Tensor, keep: Optional[Tensor], lengths: Tensor, block_table: Tensor, shares: Tensor,
+              free_pages: Tensor, free_count: Tensor, page_size: int) -> Tuple[Tensor, Tensor]:
+    f = kvq.PageForker(parents, lengths, block_table, shares, free_pages, free_count, page_size, keep=keep,
+                       workspace=_workspace_for("page_fork", lengths.device))
+    f()
+    return f.copy_src, f.copy_dst
+
+
+@page_fork.register_fake
+def _page_fork_fake(parents, keep, lengths, block_table, shares, free_pages, free_count, page_size):
+    return torch.empty_like(parents), torch.empty_like(parents)
+
+
+@torch.library.custom_op("kvq::page_copy", mutates_args=_POOL + ("bounds", "bound_scale"))
+def page_copy(copy_src: Tensor, copy_dst: Tensor, k_pages: Tensor, v_pages: Tensor, k_scale_pages: Tensor,
+              v_scale_pages: Tensor, bounds: Optional[Tensor], bound_scale: Optional[Tensor]) -> None:
+    kvq.page_copy(copy_src, copy_dst, k_pages, v_pages, k_scale_pages, v_scale_pages, bounds, bound_scale)
+
+
+@page_copy.register_fake
+def _page_copy_fake(copy_src, copy_dst, k_pages, v_pages, k_scale_pages, v_scale_pages, bounds, bound_scale):
+    return None
+
+
+@torch.library.custom_op("kvq::page_compact", mutates_args=("block_table", "shares", "free_pages"))
+def page_compact(lengths: Tensor, block_table: Tensor, shares: Optional[Tensor], free_pages: Tensor, free_count: Tensor,
+                 page_size: int, max_moves: int) -> Tuple[Tensor, Tensor, Tensor]:
+    c = kvq.PageCompactor(lengths, block_table, shares, free_pages, free_count, page_size, max_moves=max_moves,
+                          workspace=_workspace_for("page_compact", lengths.device))
+    c()
+    return c.copy_src, c.copy_dst, c.moved
+
+
+@page_compact.register_fake
+def _page_compact_fake(lengths, block_table, shares, free_pages, free_count, page_size, max_moves):
+    e = lambda n: torch.empty(n, dtype=torch.int32, device=lengths.device)  # noqa: E731
+    return e(max_moves), e(max_moves), e(1)
+
+
 __all__ = ["decode", "paged_decode", "append", "prefill", "attention", "page_map", "slot_write", "slot_read",
-           "page_bounds", "sparse_decode"]
+           "page_bounds", "sparse_decode", "chunk_attention", "page_fork", "page_copy", "page_compact"]

@@ -24,15 +24,15 @@ constexpr float kWeightReset = 12.0f; // and of what a row's weights are set to 
 constexpr float kKsMax = 0x1p80f;     // |k scale|s above overflow as scores of q scaled to 2^15
 constexpr float kVsMax = 0x1p40f, kVsMin = 0x1p-40f;  // |v scale|s outside take fp32 weights, as does a
 template <int LIMBS>                                  // tile set whose scales differ by more than this
-constexpr float kVsRatio = LIMBS == 1 ? 0x1p24f : 0x1p14f;
+constexpr float kVsRatio = LIMBS == 1 ? 0x1p18f : 0x1p14f;
 
-// Eight int8 as f16: each byte, made unsigned, under the exponent of 1024; less 1152.
-__device__ __forceinline__ h16x8 codes_to_f16(int2 w) {
-    const h16x2 bias = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+// Eight int8 as f16: each byte, made unsigned, under the exponent of 1024, so
+// kCodeBias + code; then f of each pair.
+constexpr float kCodeBias = 1152.0f;
+template <class F>
+__device__ __forceinline__ h16x8 codes_to_f16(int2 w, F&& f) {
     const unsigned x = static_cast<unsigned>(w.x) ^ 0x80808080u, y = static_cast<unsigned>(w.y) ^ 0x80808080u;
-    auto pair = [&](unsigned z, unsigned sel) {
-        return __builtin_bit_cast(h16x2, __builtin_amdgcn_perm(0x64646464u, z, sel)) - bias;
-    };
+    auto pair = [&](unsigned z, unsigned sel) { return f(__builtin_bit_cast(h16x2, __builtin_amdgcn_perm(0x64646464u, z, sel))); };
     const h16x2 a = pair(x, 0x04010400u), b = pair(x, 0x04030402u), c = pair(y, 0x04010400u), e = pair(y, 0x04030402u);
     return h16x8{a[0], a[1], b[0], b[1], c[0], c[1], e[0], e[1]};
 }
@@ -40,7 +40,7 @@ __device__ __forceinline__ h16x8 codes_to_f16(int2 w) {
 // x times lane I's y of the 16-lane row.
 template <int I>
 __device__ __forceinline__ float times_lane(float x, float y) {
-    return x * __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(y), 0x150 + I, 0xF, 0xF, true));
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(y), 0x150 + I, 0xF, 0xF, true)) * x;
 }
 template <int I = 0>
 __device__ __forceinline__ void times_lanes(f32x16& x, float y) {
@@ -221,11 +221,17 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
     struct alignas(16) Buf {
         _Float16 k[kChunkKeys * KS];
         _Float16 v[kChunkKeys * VS];
-        float ks[kChunkKeys], vs[kChunkKeys];
-        float lv;
+    };
+    // A tile's scales, in the slot of its number: kept four, as rows and scales
+    // are fetched up to three tiles ahead.
+    struct Scales {
+        long long row[kChunkKeys];  // pool rows
+        float ks[kChunkKeys];
+        float vs[kChunkKeys];       // LIMBS == 1: two f16 of vs / 2^lv
+        float lv, unit;             // |vs| <= 2^lv; 2^-lv
     };
     __shared__ __align__(16) Buf s_buf[2];
-    __shared__ long long s_row[4][kChunkKeys];
+    __shared__ __align__(16) Scales s_scale[4];
     __shared__ ChunkPlanLds s_plan;
     __shared__ int s_flag;
 
@@ -276,7 +282,7 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
     float vmax = 0.0f, vmin = INFINITY, kmax = 0.0f;
     bool vbad = false;
     auto load_tile = [&](int tile) {
-        const long long* rows = s_row[tile & 3];
+        const long long* rows = s_scale[tile & 3].row;
 #pragma unroll
         for (int i = 0; i < NP; i++) {
             const int piece = i * kChunkThreads + t;
@@ -286,45 +292,62 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
             kraw[i] = in ? *reinterpret_cast<const int2*>(a.k + at) : make_int2(0, 0);
             vraw[i] = in ? *reinterpret_cast<const int2*>(a.v + at) : make_int2(0, 0);
         }
-        if (wave == 0) {
-            const long long at = rows[lane];
-            ksr = a.ks[at];
-            vsr = a.vs[at];
-            if (k0 + tile * kChunkKeys + lane >= k1) ksr = vsr = 0.0f;
-        }
     };
+    // Codes become f16 here, once a workgroup.  bf16: K keeps its bias (taken off
+    // in the accumulators' start), V is scaled by vs / 2^lv, rounded to f16; fp32:
+    // codes are exact.
     auto store_tile = [&](int tile) {
         Buf& buf = s_buf[tile & 1];
+        const h16x2 bias = {static_cast<_Float16>(kCodeBias), static_cast<_Float16>(kCodeBias)};
 #pragma unroll
         for (int i = 0; i < NP; i++) {
             const int piece = i * kChunkThreads + t;
             const int kr = piece / PPR, c = (piece - kr * PPR) * 8;
-            *reinterpret_cast<h16x8*>(buf.k + kr * KS + c) = codes_to_f16(kraw[i]);
-            *reinterpret_cast<h16x8*>(buf.v + kr * VS + c) = codes_to_f16(vraw[i]);
-        }
-        if (wave == 0) {
-            buf.ks[lane] = ksr;
-            buf.vs[lane] = vsr;
-            const float v = fabsf(vsr);
-            kmax = fmaxf(kmax, fabsf(ksr));
-            vbad |= !(v < INFINITY);
-            vmax = fmaxf(vmax, v);
-            if (v > 0.0f) vmin = fminf(vmin, v);
-            const float top = wave_max(v);
-            if (lane == 0) buf.lv = fminf(fmaxf(static_cast<float>(__builtin_amdgcn_frexp_expf(top)), -60.0f), 60.0f);
+            *reinterpret_cast<h16x8*>(buf.k + kr * KS + c) =
+                codes_to_f16(kraw[i], [&](h16x2 x) { return LIMBS == 1 ? x : x - bias; });
+            const h16x2 f = LIMBS == 1 ? __builtin_bit_cast(h16x2, s_scale[tile & 3].vs[kr]) : bias;
+            *reinterpret_cast<h16x8*>(buf.v + kr * VS + c) =
+                codes_to_f16(vraw[i], [&](h16x2 x) { return LIMBS == 1 ? (x - bias) * f : x - bias; });
         }
     };
-    if (tiles > 0 && wave == 0) {
-        s_row[0][lane] = pool_row(0, table[page_of(0)]);
-        s_row[1][lane] = pool_row(1, table[page_of(1)]);
-        s_row[2][lane] = pool_row(2, table[page_of(2)]);
-    }
+    // Wave 0 looks after rows and scales, a key a lane.
+    auto load_scales = [&](int tile, long long at) {
+        s_scale[tile & 3].row[lane] = at;
+        ksr = a.ks[at];
+        vsr = a.vs[at];
+        if (k0 + tile * kChunkKeys + lane >= k1) ksr = vsr = 0.0f;
+    };
+    auto store_scales = [&](int tile) {
+        Scales& x = s_scale[tile & 3];
+        const float v = fabsf(vsr);
+        kmax = fmaxf(kmax, fabsf(ksr));
+        vbad |= !(v < INFINITY);
+        vmax = fmaxf(vmax, v);
+        if (v > 0.0f) vmin = fminf(vmin, v);
+        const int e = min(max(__builtin_amdgcn_frexp_expf(lanes_max<kWave>(v)), -60), 60);
+        x.ks[lane] = ksr;
+        const _Float16 h = static_cast<_Float16>(ldexpf(vsr, -e));
+        x.vs[lane] = LIMBS == 1 ? __builtin_bit_cast(float, h16x2{h, h}) : vsr;
+        if (lane == 0) {
+            x.lv = static_cast<float>(e);
+            x.unit = ldexpf(1.0f, -e);
+        }
+    };
     int next_id = 0;
-    if (tiles > 0 && wave == 0) next_id = table[page_of(3)];
+    if (tiles > 0 && wave == 0) {
+        const int id0 = table[page_of(0)], id1 = table[page_of(1)], id2 = table[page_of(2)];
+        next_id = table[page_of(3)];
+        load_scales(0, pool_row(0, id0));
+        store_scales(0);
+        load_scales(1, pool_row(1, id1));
+        store_scales(1);
+        load_scales(2, pool_row(2, id2));
+    }
 
     // q^T operands: lane has dims 16 s + 8 h + [0, 8) of its row, scaled to 2^15.
     h16x8 q[LIMBS][NS];
     float c_row;
+    float start = 0.0f;  // of a score's sum: minus the codes' bias times the sum of q
     {
         float x[NS][8];
         float top = 0.0f;
@@ -369,10 +392,15 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
             for (int j = 0; j < 8; j++) {
                 const float y = bad ? 0.0f : ldexpf(x[n][j], -e);
                 q[0][n][j] = static_cast<_Float16>(y);
+                if (LIMBS == 1) start -= static_cast<float>(q[0][n][j]);
                 if (LIMBS == 2) q[LIMBS - 1][n][j] = static_cast<_Float16>(y - static_cast<float>(q[0][n][j]));
             }
     }
 
+    f32x16 sum0;
+    if (LIMBS == 1) start = (start + __shfl_xor(start, 32)) * kCodeBias;
+#pragma unroll
+    for (int i = 0; i < 16; i++) sum0[i] = start;
     f32x16 o[NB];
 #pragma unroll
     for (int c = 0; c < NB; c++)
@@ -384,13 +412,14 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
     const int scale_at = 8 * (c16 >> 2) + 4 * h + (c16 & 3);
     auto compute = [&](int tile) {
         const Buf& buf = s_buf[tile & 1];
+        const Scales& sc = s_scale[tile & 3];
         const int t0 = k0 + tile * kChunkKeys;
         f32x16 p[2];
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
-            f32x16 acc, low;
+            f32x16 acc = sum0, low;
 #pragma unroll
-            for (int i = 0; i < 16; i++) acc[i] = low[i] = 0.0f;
+            for (int i = 0; i < 16; i++) low[i] = 0.0f;
             const _Float16* kp = buf.k + (32 * kb + c32) * KS + 8 * h;
 #pragma unroll
             for (int n = 0; n < NS; n++) {
@@ -399,10 +428,11 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
                 if (LIMBS == 2) low = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q[LIMBS - 1][n], low, 0, 0, 0);
             }
             if (LIMBS == 2) acc += low;
-            times_lanes(acc, buf.ks[32 * kb + scale_at]);
+            times_lanes(acc, sc.ks[32 * kb + scale_at]);
             p[kb] = acc;
         }
         if (t0 + kChunkKeys > keys_all) {
+            asm volatile("");  // a branch, not selects: most tiles need no mask (95 of 575 VALU slots of a tile)
 #pragma unroll
             for (int kb = 0; kb < 2; kb++)
 #pragma unroll
@@ -412,7 +442,7 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
         float top = p[0][0];
 #pragma unroll
         for (int i = 1; i < 32; i++) top = fmaxf(top, p[i / 16][i % 16]);
-        const float u = fmaf(top, c_row, buf.lv);
+        const float u = fmaf(top, c_row, sc.lv);
         if (__builtin_amdgcn_ballot_w64(u > m + kWeightTop) != 0) {
             const float un = fmaxf(u, __shfl_xor(u, 32)) - kWeightReset;
             const float mn = un > m ? un : m;
@@ -424,7 +454,7 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[c][i] *= alpha;
         }
-        const float ms = m == -INFINITY ? 0.0f : m;
+        const float ms = (m == -INFINITY ? 0.0f : m) - (LIMBS == 1 ? sc.lv : 0.0f);
         h16x8 wt[LIMBS][4];
         // Summed by itself, so l rounds once a tile (2000 keys in fp32: error 2.0e-6 with a sum key by key).
         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -435,7 +465,7 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
                 p[kb][i] = fast_exp2(fmaf(p[kb][i], c_row, -ms));
                 part[i % 4] += p[kb][i];
             }
-            times_lanes(p[kb], buf.vs[32 * kb + scale_at]);
+            if (LIMBS == 2) times_lanes(p[kb], sc.vs[32 * kb + scale_at]);
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 if (LIMBS == 2) {
@@ -450,7 +480,7 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
                 if (LIMBS == 2) wt[LIMBS - 1][2 * kb + i / 8][i % 8] = static_cast<_Float16>(p[kb][i] - static_cast<float>(hi));
             }
         }
-        l += (part[0] + part[1]) + (part[2] + part[3]);
+        l = fmaf((part[0] + part[1]) + (part[2] + part[3]), LIMBS == 1 ? sc.unit : 1.0f, l);
         // Keys 16 n + 8 j + 4 h + [0, 4), j = 0, 1, are the lane's 8 slots of step n.
         const _Float16* vp = buf.v + (4 * h + (c16 >> 2)) * VS + 16 * ((lane >> 4) & 1) + 4 * (c16 & 3);
 #pragma unroll
@@ -474,12 +504,16 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
         if (tiles > 1) load_tile(1);
     }
     __syncthreads();
+    // Iteration i: tile i + 1 becomes f16 in the buffer that was last read before
+    // the last barrier, codes of tile i + 2 are on their way, scales of tile i + 2
+    // are stored, and rows and scales of tile i + 3 fetched; the slot of those held
+    // tile i - 1's.
     for (int i = 0; i < tiles; i++) {
         if (i + 1 < tiles) store_tile(i + 1);
         if (i + 2 < tiles) load_tile(i + 2);
-        // Rows of tile i + 3; its slot's last readers loaded tile i - 1, two barriers ago.
-        if (i + 3 < tiles && wave == 0) {
-            s_row[(i + 3) & 3][lane] = pool_row(i + 3, next_id);
+        if (wave == 0 && i + 2 < tiles) {
+            store_scales(i + 2);
+            if (i + 3 < tiles) load_scales(i + 3, pool_row(i + 3, next_id));
             next_id = table[page_of(i + 4)];
         }
         if (k0 + i * kChunkKeys < keys_any) compute(i);

@@ -106,7 +106,7 @@ namespace {
 
 template <int D, int LIMBS>
 hipError_t launch_mfma(const ChunkArgs& a, unsigned items, hipStream_t stream) {
-    hipLaunchKernelGGL((chunk_mfma<D, LIMBS>), dim3(items), dim3(kChunkThreads), 0, stream, a);
+    hipLaunchKernelGGL((chunk_mfma<D, LIMBS>), dim3(items), dim3(chunk_waves(D, LIMBS) * kWave), 0, stream, a);
     return hipGetLastError();
 }
 
@@ -118,19 +118,21 @@ constexpr size_t kChunkCounters = 256 * 1024;
 
 ChunkPlan chunk_plan(const ChunkArgs& a, bool vec_ok) {
     ChunkPlan p{};
-    p.mfma = vec_ok && a.d <= 256 && a.d % 8 == 0 && a.G <= kChunkRows;
+    p.mfma = vec_ok && a.d <= 256 && a.d % 8 == 0 && a.G <= 128;
     if (!p.mfma || a.T == 0) return p;
     p.D = chunk_dim(a.d);
-    p.tile_tokens = kChunkRows / a.G;
+    const int waves = chunk_waves(p.D, a.bf16 ? 1 : 2);
+    p.rows = 32 * waves;
+    p.tile_tokens = p.rows / a.G;
     const long long tiles = std::min<long long>(a.T, a.T / p.tile_tokens + a.B);
     const long long units = tiles * a.Hkv;
     const int blocks = (a.max_len + kChunkKeys - 1) / kChunkKeys;
     p.max_tiles = static_cast<int>(tiles);
-    p.slots = p.D <= 128 ? 512 : 256;
-    p.max_splits = units < p.slots && a.B <= kChunkThreads ? std::min(p.slots, (blocks + 3) / 4) : 1;
+    p.slots = 256;  // a workgroup a CU
+    p.max_splits = units < p.slots && a.B <= waves * kWave ? std::min(p.slots, (blocks + 3) / 4) : 1;
     p.items = static_cast<unsigned>(p.max_splits > 1 ? std::max<long long>(units, std::min<long long>(p.slots, units * p.max_splits)) : units);
     p.records = p.max_splits > 1 ? p.items : 0;
-    if (p.records) p.bytes = kChunkCounters + p.records * kChunkRows * (p.D + 2) * sizeof(float);
+    if (p.records) p.bytes = kChunkCounters + p.records * p.rows * (p.D + 2) * sizeof(float);
     return p;
 }
 
@@ -145,7 +147,7 @@ hipError_t launch_chunk(ChunkArgs a, const ChunkPlan& p, void* workspace, hipStr
         a.group = make_fastdiv(static_cast<uint32_t>(a.G));
         a.counters = static_cast<int*>(workspace);
         a.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + (p.records ? kChunkCounters : 0));
-        a.part_ml = a.part_acc + p.records * kChunkRows * p.D;
+        a.part_ml = a.part_acc + p.records * p.rows * p.D;
 #define KVQ_CHUNK_CASE(DIM) \
     case DIM: return a.bf16 ? launch_mfma<DIM, 1>(a, p.items, stream) : launch_mfma<DIM, 2>(a, p.items, stream);
         switch (p.D) {

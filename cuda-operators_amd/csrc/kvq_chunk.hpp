@@ -29,16 +29,15 @@ struct ChunkArgs {
     int max_splits;          // most splits of a sequence's keys
     int max_tiles;           // query tiles that the launch has room for
     int* counters;           // [units] arrivals of a split tile's workgroups; left at 0
-    float* part_acc;         // [items, kChunkRows, D] partial records of split tiles
-    float* part_ml;          // [items, kChunkRows, 2]
+    float* part_acc;         // [items, rows of a tile, D] partial records of split tiles
+    float* part_ml;          // [items, rows of a tile, 2]
 };
 
-constexpr int kChunkRows = 128;  // query rows (token, head) of a workgroup
 constexpr int kChunkKeys = 64;   // keys of a tile
 
 struct ChunkPlan {
     bool mfma;       // the matrix-core kernel
-    int D;           // its padded head dim
+    int D, rows;     // its padded head dim and a tile's query rows
     int tile_tokens, slots, max_splits, max_tiles;
     unsigned items;  // workgroups
     size_t records;  // partial records (0: nothing is split)

@@ -4,6 +4,8 @@
 #include <limits.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "kvq_chunk.hpp"
 #include "kvq_device.hpp"
 
@@ -16,8 +18,9 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-constexpr int kChunkWaves = 4;
-constexpr int kChunkThreads = kChunkWaves * kWave;
+// Waves of a workgroup, 32 query rows each.  Eight run in two phases a tile, which
+// takes two waves a SIMD; where the state needs a SIMD's registers, four run.
+constexpr int chunk_waves(int D, int limbs) { return D <= (limbs == 1 ? 128 : 96) ? 8 : 4; }
 constexpr int kChunkCoherent = 16;  // buffer cache policy sc1: device-coherent
 constexpr float kWeightTop = 15.0f;   // log2 of the largest f16 weight that is let grow,
 constexpr float kWeightReset = 12.0f; // and of what a row's weights are set to when they pass it
@@ -25,6 +28,10 @@ constexpr float kKsMax = 0x1p80f;     // |k scale|s above overflow as scores of 
 constexpr float kVsMax = 0x1p40f, kVsMin = 0x1p-40f;  // |v scale|s outside take fp32 weights, as does a
 template <int LIMBS>                                  // tile set whose scales differ by more than this
 constexpr float kVsRatio = LIMBS == 1 ? 0x1p18f : 0x1p14f;
+
+// Dims that lane half h contracts in step n: steps 2 j and 2 j + 1 take the halves
+// of one 16-byte piece, so that a row's codes can come straight from memory.
+__device__ __forceinline__ constexpr int chunk_dim_of(int n, int h) { return 32 * (n >> 1) + 16 * h + 8 * (n & 1); }
 
 // Eight int8 as f16: each byte, made unsigned, under the exponent of 1024, so
 // kCodeBias + code; then f of each pair.
@@ -69,11 +76,13 @@ __device__ __forceinline__ void chunk_counts(const ChunkArgs& a, const ChunkSeq&
 // chunks of the fewest blocks (in steps) with which the items are at most a.slots;
 // all tiles of a sequence have the same number of splits.
 struct ChunkPlanLds {
-    int part[kChunkWaves], best[kChunkWaves];
-    int tiles[kChunkThreads], blocks[kChunkThreads];
+    int part[8], best[8];
+    int tiles[512], blocks[512];
     int found[6];
 };
+template <int W>
 __device__ inline bool chunk_locate(const ChunkArgs& a, ChunkPlanLds& s, int r, ChunkItem& w) {
+    constexpr int kChunkWaves = W, kChunkThreads = W * kWave;
     const int t = threadIdx.x;
     const int lane = t & (kWave - 1), wave = t / kWave;
     const int per = (a.B + kChunkThreads - 1) / kChunkThreads;
@@ -210,29 +219,33 @@ __device__ __forceinline__ void chunk_row_f32(const ChunkArgs& a, int b, int kvh
 }
 
 template <int D, int LIMBS>
-__global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void chunk_mfma(
-    const ChunkArgs a) {
+__global__ __launch_bounds__(chunk_waves(D, LIMBS) * kWave) __attribute__((amdgpu_waves_per_eu(chunk_waves(D, LIMBS) / 4))) void
+chunk_mfma(const ChunkArgs a) {
+    constexpr int W = chunk_waves(D, LIMBS);
+    constexpr bool kPhased = W == 8;
+    constexpr int kChunkThreads = W * kWave;
+    constexpr int kChunkRows = 32 * W;
     constexpr int KS = D + 8, VS = D + 16;     // LDS row strides in f16
     constexpr int NS = D / 16;                 // QK contraction steps
     constexpr int NB = D / 32;                 // output blocks
     constexpr int PPR = D / 8;                 // 8-code pieces of a row
-    constexpr int NP = kChunkKeys * PPR / kChunkThreads;  // a thread's, of K and of V
-    static_assert(D % 32 == 0 && kChunkKeys * PPR % kChunkThreads == 0, "whole pieces");
-    struct alignas(16) Buf {
-        _Float16 k[kChunkKeys * KS];
-        _Float16 v[kChunkKeys * VS];
-    };
-    // A tile's scales, in the slot of its number: kept four, as rows and scales
-    // are fetched up to three tiles ahead.
+    constexpr int NP = kChunkKeys * PPR / 256;  // a thread's: of K and of V, or (phased) of one of them
+    static_assert(D % 32 == 0 && kChunkKeys * PPR % 256 == 0, "whole pieces");
+    // A tile's scales, in the slot of its number.
     struct Scales {
-        long long row[kChunkKeys];  // pool rows
+        long long at[kChunkKeys];   // byte offsets of the pool rows
         float ks[kChunkKeys];
         float vs[kChunkKeys];       // LIMBS == 1: two f16 of vs / 2^lv
         float lv, unit;             // |vs| <= 2^lv; 2^-lv
     };
-    __shared__ __align__(16) Buf s_buf[2];
-    __shared__ __align__(16) Scales s_scale[4];
-    __shared__ ChunkPlanLds s_plan;
+    constexpr int kKTile = kChunkKeys * KS, kVTile = kChunkKeys * VS;
+    __shared__ __align__(16) _Float16 s_buf[2 * (kKTile + kVTile)];
+    auto s_k = [&](int tile) { return s_buf + (tile & 1) * kKTile; };
+    auto s_v = [&](int tile) { return s_buf + 2 * kKTile + (tile & 1) * kVTile; };
+    constexpr int kSlots = kPhased ? 8 : 4;
+    __shared__ __align__(16) Scales s_scale[kSlots];
+    static_assert(sizeof(ChunkPlanLds) <= sizeof(s_buf), "the plan's scratch lies where tiles come later");
+    ChunkPlanLds& s_plan = *reinterpret_cast<ChunkPlanLds*>(s_buf);
     __shared__ int s_flag;
 
     const int t = threadIdx.x;
@@ -242,7 +255,7 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
     const int r = static_cast<int>(fastdiv(blockIdx.x, a.heads));
     const int kvh = static_cast<int>(blockIdx.x) - r * a.Hkv;
     ChunkItem w;
-    if (!chunk_locate(a, s_plan, r, w)) return;
+    if (!chunk_locate<W>(a, s_plan, r, w)) return;
     const ChunkSeq s = chunk_seq(a, w.b);
     const int i0 = w.tile * a.tile_tokens;                       // the tile's new tokens
     const int tokens = min(a.tile_tokens, s.n - i0);
@@ -253,19 +266,20 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
     const int k1 = min(min((w.split + 1) * share, nblocks) * kChunkKeys, kend);
     const int tiles = k1 > k0 ? (k1 - k0 + kChunkKeys - 1) / kChunkKeys : 0;
 
+    // Tiles of up to 32 rows are computed by all waves, each with the same rows and
+    // keys of its own.
+    const bool narrow = tokens * a.G <= 32;
     // This lane's query row: (token, head) = divmod(row, G).
-    const int row = wave * 32 + c32;
+    const int row = (narrow ? 0 : wave * 32) + c32;
     const int tok = static_cast<int>(fastdiv(row, a.group));
     const int head = kvh * a.G + row - tok * a.G;
-    const bool live = tok < tokens;
+    bool live = tok < tokens;
     const int keys = live ? chunk_keys(a, s, i0 + tok) : 0;
     const int64_t q_at = static_cast<int64_t>(s.row0 + i0 + tok) * a.q_stride + static_cast<int64_t>(head) * a.d;
-    const int wave_rows = min(max(tokens * a.G - wave * 32, 0), 32);  // live rows of this wave
-    // Keys that every live row of the wave attends, and that any does.
-    const int first_tok = static_cast<int>(fastdiv(wave * 32, a.group));
-    const int last_tok = static_cast<int>(fastdiv(wave * 32 + max(wave_rows, 1) - 1, a.group));
+    int wave_rows = min(max(tokens * a.G - (narrow ? 0 : wave * 32), 0), 32);  // live rows of this wave
+    // Keys that every live row of the wave attends.
+    const int first_tok = narrow ? 0 : static_cast<int>(fastdiv(wave * 32, a.group));
     const int keys_all = __builtin_amdgcn_readfirstlane(wave_rows > 0 ? chunk_keys(a, s, i0 + first_tok) : 0);
-    const int keys_any = __builtin_amdgcn_readfirstlane(wave_rows > 0 ? chunk_keys(a, s, i0 + last_tok) : 0);
 
     // Pool row of key t0 + (t % 64) (past the end: the last key's again).
     const int32_t* table = a.pages.table + static_cast<size_t>(w.b) * a.pages.max_pages;
@@ -277,54 +291,82 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
         return (static_cast<long long>(id) * a.Hkv + kvh) * a.pages.size + (key - page * a.pages.size);
     };
 
-    int2 kraw[NP], vraw[NP];
+    // Phased: the first four waves fetch and convert K, the others V.
+    const bool is_v = kPhased && wave >= 4;
+    const int t256 = t & 255;
+    int2 kraw[NP], vraw[kPhased ? 1 : NP];
     float ksr = 0.0f, vsr = 0.0f;
     float vmax = 0.0f, vmin = INFINITY, kmax = 0.0f;
     bool vbad = false;
-    auto load_tile = [&](int tile) {
-        const long long* rows = s_scale[tile & 3].row;
+    // Places of a tile's codes, read ahead of the loads that need them.
+    long long at[NP];
+    auto read_places = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < NP; i++) at[i] = s_scale[tile & (kSlots - 1)].at[(i * 256 + t256) / PPR];
+    };
+    auto load_codes = [&](const int8_t* src, int2* raw) {
 #pragma unroll
         for (int i = 0; i < NP; i++) {
-            const int piece = i * kChunkThreads + t;
-            const int kr = piece / PPR, c = (piece - kr * PPR) * 8;
-            const long long at = rows[kr] * a.d + c;
-            const bool in = c < a.d;
-            kraw[i] = in ? *reinterpret_cast<const int2*>(a.k + at) : make_int2(0, 0);
-            vraw[i] = in ? *reinterpret_cast<const int2*>(a.v + at) : make_int2(0, 0);
+            const int c = (i * 256 + t256) % PPR * 8;
+            raw[i] = c < a.d ? *reinterpret_cast<const int2*>(src + at[i] + c) : make_int2(0, 0);
         }
     };
-    // Codes become f16 here, once a workgroup.  bf16: K keeps its bias (taken off
-    // in the accumulators' start), V is scaled by vs / 2^lv, rounded to f16; fp32:
-    // codes are exact.
-    auto store_tile = [&](int tile) {
-        Buf& buf = s_buf[tile & 1];
-        const h16x2 bias = {static_cast<_Float16>(kCodeBias), static_cast<_Float16>(kCodeBias)};
+    // Codes become f16 here, once a workgroup: K exactly; V too for fp32, for bf16
+    // times vs / 2^lv, rounded to f16.
+    const h16x2 bias = {static_cast<_Float16>(kCodeBias), static_cast<_Float16>(kCodeBias)};
+    auto store_k = [&](const int2* raw, int tile) {
 #pragma unroll
         for (int i = 0; i < NP; i++) {
-            const int piece = i * kChunkThreads + t;
+            const int piece = i * 256 + t256;
             const int kr = piece / PPR, c = (piece - kr * PPR) * 8;
-            *reinterpret_cast<h16x8*>(buf.k + kr * KS + c) =
-                codes_to_f16(kraw[i], [&](h16x2 x) { return LIMBS == 1 ? x : x - bias; });
-            const h16x2 f = LIMBS == 1 ? __builtin_bit_cast(h16x2, s_scale[tile & 3].vs[kr]) : bias;
-            *reinterpret_cast<h16x8*>(buf.v + kr * VS + c) =
-                codes_to_f16(vraw[i], [&](h16x2 x) { return LIMBS == 1 ? (x - bias) * f : x - bias; });
+            *reinterpret_cast<h16x8*>(s_k(tile) + kr * KS + c) =
+                codes_to_f16(raw[i], [&](h16x2 x) { return x - bias; });
+        }
+    };
+    auto store_v = [&](const int2* raw, int tile) {
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+            const int piece = i * 256 + t256;
+            const int kr = piece / PPR, c = (piece - kr * PPR) * 8;
+            const h16x2 f = LIMBS == 1 ? __builtin_bit_cast(h16x2, s_scale[tile & (kSlots - 1)].vs[kr]) : bias;
+            *reinterpret_cast<h16x8*>(s_v(tile) + kr * VS + c) =
+                codes_to_f16(raw[i], [&](h16x2 x) { return LIMBS == 1 ? (x - bias) * f : x - bias; });
+        }
+    };
+    auto load_tile = [&]() {
+        if constexpr (kPhased) {
+            load_codes(is_v ? a.v : a.k, kraw);
+        } else {
+            load_codes(a.k, kraw);
+            load_codes(a.v, vraw);
+        }
+    };
+    auto store_tile = [&](int tile) {
+        if constexpr (kPhased) {
+            if (is_v) store_v(kraw, tile);
+            else store_k(kraw, tile);
+        } else {
+            store_k(kraw, tile);
+            store_v(vraw, tile);
         }
     };
     // Wave 0 looks after rows and scales, a key a lane.
-    auto load_scales = [&](int tile, long long at) {
-        s_scale[tile & 3].row[lane] = at;
-        ksr = a.ks[at];
-        vsr = a.vs[at];
+    auto load_scales = [&](int tile, long long row) {
+        s_scale[tile & (kSlots - 1)].at[lane] = row * a.d;
+        ksr = a.ks[row];
+        vsr = a.vs[row];
         if (k0 + tile * kChunkKeys + lane >= k1) ksr = vsr = 0.0f;
     };
     auto store_scales = [&](int tile) {
-        Scales& x = s_scale[tile & 3];
+        Scales& x = s_scale[tile & (kSlots - 1)];
         const float v = fabsf(vsr);
         kmax = fmaxf(kmax, fabsf(ksr));
         vbad |= !(v < INFINITY);
         vmax = fmaxf(vmax, v);
         if (v > 0.0f) vmin = fminf(vmin, v);
-        const int e = min(max(__builtin_amdgcn_frexp_expf(lanes_max<kWave>(v)), -60), 60);
+        // (bits of a float >= 0 order as integers)
+        const float top = __int_as_float(__builtin_amdgcn_readlane(wave_inclusive_max_nonneg(__float_as_int(v)), kWave - 1));
+        const int e = min(max(__builtin_amdgcn_frexp_expf(top), -60), 60);
         x.ks[lane] = ksr;
         const _Float16 h = static_cast<_Float16>(ldexpf(vsr, -e));
         x.vs[lane] = LIMBS == 1 ? __builtin_bit_cast(float, h16x2{h, h}) : vsr;
@@ -334,7 +376,7 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
         }
     };
     int next_id = 0;
-    if (tiles > 0 && wave == 0) {
+    if (tiles > 0 && wave == 0 && !narrow) {
         const int id0 = table[page_of(0)], id1 = table[page_of(1)], id2 = table[page_of(2)];
         next_id = table[page_of(3)];
         load_scales(0, pool_row(0, id0));
@@ -344,17 +386,16 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
         load_scales(2, pool_row(2, id2));
     }
 
-    // q^T operands: lane has dims 16 s + 8 h + [0, 8) of its row, scaled to 2^15.
+    // q^T operands: lane has dims chunk_dim_of(n, h) + [0, 8) of its row, scaled to 2^15.
     h16x8 q[LIMBS][NS];
     float c_row;
-    float start = 0.0f;  // of a score's sum: minus the codes' bias times the sum of q
     {
         float x[NS][8];
         float top = 0.0f;
         bool bad = false;
 #pragma unroll
         for (int n = 0; n < NS; n++) {
-            const int dim = 16 * n + 8 * h;
+            const int dim = chunk_dim_of(n, h);
             const bool in = live && dim < a.d;
             if (LIMBS == 1) {
                 uint4 raw = make_uint4(0, 0, 0, 0);
@@ -392,15 +433,10 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
             for (int j = 0; j < 8; j++) {
                 const float y = bad ? 0.0f : ldexpf(x[n][j], -e);
                 q[0][n][j] = static_cast<_Float16>(y);
-                if (LIMBS == 1) start -= static_cast<float>(q[0][n][j]);
                 if (LIMBS == 2) q[LIMBS - 1][n][j] = static_cast<_Float16>(y - static_cast<float>(q[0][n][j]));
             }
     }
 
-    f32x16 sum0;
-    if (LIMBS == 1) start = (start + __shfl_xor(start, 32)) * kCodeBias;
-#pragma unroll
-    for (int i = 0; i < 16; i++) sum0[i] = start;
     f32x16 o[NB];
 #pragma unroll
     for (int c = 0; c < NB; c++)
@@ -410,29 +446,60 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
 
     // Keys of this lane's score registers: block 32 kb, register i: 32 kb + 8 (i / 4) + 4 h + i % 4.
     const int scale_at = 8 * (c16 >> 2) + 4 * h + (c16 & 3);
-    auto compute = [&](int tile) {
-        const Buf& buf = s_buf[tile & 1];
-        const Scales& sc = s_scale[tile & 3];
-        const int t0 = k0 + tile * kChunkKeys;
-        f32x16 p[2];
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++) {
-            f32x16 acc = sum0, low;
-#pragma unroll
-            for (int i = 0; i < 16; i++) low[i] = 0.0f;
-            const _Float16* kp = buf.k + (32 * kb + c32) * KS + 8 * h;
-#pragma unroll
-            for (int n = 0; n < NS; n++) {
-                const h16x8 x = *reinterpret_cast<const h16x8*>(kp + 16 * n);
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q[0][n], acc, 0, 0, 0);
-                if (LIMBS == 2) low = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q[LIMBS - 1][n], low, 0, 0, 0);
+    f32x16 p[2];        // scores, then weights, of a tile
+    h16x8 wt[LIMBS][4]; // weights as the operands of PV
+    // PV of tile `pv` (O^T += V^T P^T) and QK of tile `qk` (S^T = K q^T), as one
+    // sequence of A operands that are read kAhead of their MFMA: 8 keys of V (16 n +
+    // 8 j + 4 h + [0, 4), j = 0, 1, are the lane's slots of step n) by two transposing
+    // reads, 8 dims of K by one.
+    auto matrix = [&](auto do_pv, auto do_qk, int pv, int qk) {
+        constexpr int kPv = decltype(do_pv)::value ? 4 * NB : 0, kQk = decltype(do_qk)::value ? 2 * NS : 0;
+        constexpr int kAll = kPv + kQk, kAhead = LIMBS == 1 ? 6 : 4;
+        const _Float16* kp = s_k(qk) + c32 * KS;
+        const _Float16* vp = s_v(pv) + (4 * h + (c16 >> 2)) * VS + 16 * ((lane >> 4) & 1) + 4 * (c16 & 3);
+        auto read = [&](int n) {
+            if (n < kPv) {
+                const _Float16* x = vp + 16 * (n / NB) * VS + 32 * (n % NB);
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(const_cast<_Float16*>(x)));
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(const_cast<_Float16*>(x + 8 * VS)));
+                return __builtin_bit_cast(h16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
             }
-            if (LIMBS == 2) acc += low;
-            times_lanes(acc, sc.ks[32 * kb + scale_at]);
-            p[kb] = acc;
+            n -= kPv;
+            return *reinterpret_cast<const h16x8*>(kp + 32 * (n & 1) * KS + chunk_dim_of(n >> 1, h));
+        };
+        h16x8 x[kAll];
+        f32x16 low[2];
+#pragma unroll
+        for (int n = 0; n < kAhead && n < kAll; n++) x[n] = read(n);
+#pragma unroll
+        for (int n = 0; n < kAll; n++) {
+            if (n + kAhead < kAll) x[n + kAhead] = read(n + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+            if (n < kPv) {
+                const int c = n % NB, step = n / NB;
+                o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[n], wt[0][step], o[c], 0, 0, 0);
+                if (LIMBS == 2) o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[n], wt[LIMBS - 1][step], o[c], 0, 0, 0);
+            } else {
+                const int kb = (n - kPv) & 1, step = (n - kPv) >> 1;
+                if (step == 0) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) p[kb][i] = low[kb][i] = 0.0f;
+                }
+                p[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[n], q[0][step], p[kb], 0, 0, 0);
+                if (LIMBS == 2) low[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[n], q[LIMBS - 1][step], low[kb], 0, 0, 0);
+                if (LIMBS == 2 && step == NS - 1) p[kb] += low[kb];
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
+    };
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    auto softmax = [&](int tile) {
+        const Scales& sc = s_scale[tile & (kSlots - 1)];
+        const int t0 = k0 + tile * kChunkKeys;
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) times_lanes(p[kb], sc.ks[32 * kb + scale_at]);
         if (t0 + kChunkKeys > keys_all) {
-            asm volatile("");  // a branch, not selects: most tiles need no mask (95 of 575 VALU slots of a tile)
 #pragma unroll
             for (int kb = 0; kb < 2; kb++)
 #pragma unroll
@@ -442,6 +509,8 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
         float top = p[0][0];
 #pragma unroll
         for (int i = 1; i < 32; i++) top = fmaxf(top, p[i / 16][i % 16]);
+        // m is a reference that weights pass by up to 2^kWeightTop: it moves, with the
+        // state, only when some row's could pass by more.
         const float u = fmaf(top, c_row, sc.lv);
         if (__builtin_amdgcn_ballot_w64(u > m + kWeightTop) != 0) {
             const float un = fmaxf(u, __shfl_xor(u, 32)) - kWeightReset;
@@ -455,8 +524,7 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
                 for (int i = 0; i < 16; i++) o[c][i] *= alpha;
         }
         const float ms = (m == -INFINITY ? 0.0f : m) - (LIMBS == 1 ? sc.lv : 0.0f);
-        h16x8 wt[LIMBS][4];
-        // Summed by itself, so l rounds once a tile (2000 keys in fp32: error 2.0e-6 with a sum key by key).
+        // Summed by themselves, so l rounds once a tile (2000 keys in fp32: error 2.0e-6 with a sum key by key).
         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
@@ -468,55 +536,298 @@ __global__ __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(D
             if (LIMBS == 2) times_lanes(p[kb], sc.vs[32 * kb + scale_at]);
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                if (LIMBS == 2) {
-                    // One value for both limbs: contracted into one of them, the product would be
-                    // rounded once there and twice here, 2^-10 apart in one weight of some thousand.
-                    float x = p[kb][i];
-                    asm("" : "+v"(x));
-                    p[kb][i] = x;
-                }
-                const _Float16 hi = static_cast<_Float16>(p[kb][i]);
+                float y = p[kb][i];
+                // One value for both limbs: contracted into one of them, the product would be
+                // rounded once there and twice here, 2^-10 apart in one weight of some thousand.
+                if (LIMBS == 2) asm("" : "+v"(y));
+                const _Float16 hi = static_cast<_Float16>(y);
                 wt[0][2 * kb + i / 8][i % 8] = hi;
-                if (LIMBS == 2) wt[LIMBS - 1][2 * kb + i / 8][i % 8] = static_cast<_Float16>(p[kb][i] - static_cast<float>(hi));
+                if (LIMBS == 2) wt[LIMBS - 1][2 * kb + i / 8][i % 8] = static_cast<_Float16>(y - static_cast<float>(hi));
             }
         }
         l = fmaf((part[0] + part[1]) + (part[2] + part[3]), LIMBS == 1 ? sc.unit : 1.0f, l);
-        // Keys 16 n + 8 j + 4 h + [0, 4), j = 0, 1, are the lane's 8 slots of step n.
-        const _Float16* vp = buf.v + (4 * h + (c16 >> 2)) * VS + 16 * ((lane >> 4) & 1) + 4 * (c16 & 3);
-#pragma unroll
-        for (int n = 0; n < 4; n++) {
-#pragma unroll
-            for (int c = 0; c < NB; c++) {
-                const _Float16* x = vp + 16 * n * VS + 32 * c;
-                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(const_cast<_Float16*>(x)));
-                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(const_cast<_Float16*>(x + 8 * VS)));
-                const h16x8 v = __builtin_bit_cast(h16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-                o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, wt[0][n], o[c], 0, 0, 0);
-                if (LIMBS == 2) o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, wt[LIMBS - 1][n], o[c], 0, 0, 0);
-            }
-        }
     };
-
-    __syncthreads();
-    if (tiles > 0) {
-        load_tile(0);
-        store_tile(0);
-        if (tiles > 1) load_tile(1);
-    }
-    __syncthreads();
-    // Iteration i: tile i + 1 becomes f16 in the buffer that was last read before
-    // the last barrier, codes of tile i + 2 are on their way, scales of tile i + 2
-    // are stored, and rows and scales of tile i + 3 fetched; the slot of those held
-    // tile i - 1's.
-    for (int i = 0; i < tiles; i++) {
-        if (i + 1 < tiles) store_tile(i + 1);
-        if (i + 2 < tiles) load_tile(i + 2);
+    // Rows and scales ahead of tile i's: scales of tile i + 2 are stored, rows and
+    // scales of tile i + 3 fetched into the slot of tile i - 1.
+    auto ahead = [&](int i) {
         if (wave == 0 && i + 2 < tiles) {
             store_scales(i + 2);
             if (i + 3 < tiles) load_scales(i + 3, pool_row(i + 3, next_id));
             next_id = table[page_of(i + 4)];
         }
-        if (k0 + i * kChunkKeys < keys_any) compute(i);
+    };
+
+    if (narrow) {
+        // Each wave takes every W-th block of 32 keys, with nothing to wait for but its
+        // own loads: K codes come as A operands straight from memory, V codes through a
+        // part of LDS of the wave's own, read transposed.  The waves' states are joined
+        // at the end.
+        constexpr int VS8 = D + 16;   // LDS row stride of V codes
+        constexpr int NK = D / 32;    // 16-byte pieces of K a lane,
+        constexpr int LPV = D / 16;   // lanes a row of V,
+        static_assert(W * 32 * VS8 <= sizeof(s_buf) && W / 2 * 32 * D * 4 <= sizeof(s_buf), "LDS");
+        typedef int i32x2 __attribute__((ext_vector_type(2)));
+        typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+        int8_t* const vl = reinterpret_cast<int8_t*>(s_buf) + wave * 32 * VS8;
+        struct Block {
+            int4 k[NK], v[NK];
+            float ks, vs;
+        };
+        const int blocks = (k1 - k0 + 31) / 32;
+        auto key_of = [&](int blk, int r) { return min(k0 + blk * 32 + r, max(k1 - 1, 0)); };
+        auto id_of = [&](int blk) { return table[fastdiv(key_of(blk, c32), a.page)]; };
+        auto piece = [&](const int8_t* src, long long at, int c) {  // codes c .. c + 15 of a row, zeros past its end
+            int4 x = make_int4(0, 0, 0, 0);
+            if (c + 16 <= a.d) {
+                x = *reinterpret_cast<const int4*>(src + at + c);
+            } else if (c < a.d) {
+                const int2 y = *reinterpret_cast<const int2*>(src + at + c);
+                x.x = y.x, x.y = y.y;
+            }
+            return x;
+        };
+        auto load = [&](Block& x, int blk, int id) __attribute__((always_inline)) {
+            const int key = key_of(blk, c32);
+            const int page = static_cast<int>(fastdiv(key, a.page));
+            id = min(max(id, 0), a.pages.num_pages - 1);
+            const long long mine = (static_cast<long long>(id) * a.Hkv + kvh) * a.pages.size + (key - page * a.pages.size);
+#pragma unroll
+            for (int j = 0; j < NK; j++) x.k[j] = piece(a.k, mine * a.d, 32 * j + 16 * h);
+#pragma unroll
+            for (int j = 0; j < NK; j++) {
+                const int n = j * kWave + lane;
+                x.v[j] = piece(a.v, __shfl(mine, n / LPV) * a.d, n % LPV * 16);
+            }
+            const bool in = k0 + blk * 32 + c32 < k1;
+            x.ks = in ? a.ks[mine] : 0.0f;
+            x.vs = in ? a.vs[mine] : 0.0f;
+        };
+        const int scale_key = 8 * (c16 >> 2) + 4 * h + (c16 & 3);
+        auto compute = [&](const Block& x, int blk) __attribute__((always_inline)) {
+            wave_sync();
+#pragma unroll
+            for (int j = 0; j < NK; j++) {
+                const int n = j * kWave + lane;
+                *reinterpret_cast<int4*>(vl + n / LPV * VS8 + n % LPV * 16) = x.v[j];
+            }
+            const h16x2 bias = {static_cast<_Float16>(kCodeBias), static_cast<_Float16>(kCodeBias)};
+            auto exact = [&](int2 w) { return codes_to_f16(w, [&](h16x2 y) { return y - bias; }); };
+            f32x16 p, low;
+#pragma unroll
+            for (int i = 0; i < 16; i++) p[i] = low[i] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NS; n++) {
+                const int4 w = x.k[n / 2];
+                const h16x8 y = exact(n & 1 ? make_int2(w.z, w.w) : make_int2(w.x, w.y));
+                p = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, q[0][n], p, 0, 0, 0);
+                if (LIMBS == 2) low = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, q[LIMBS - 1][n], low, 0, 0, 0);
+            }
+            if (LIMBS == 2) p += low;
+            kmax = fmaxf(kmax, fabsf(x.ks));
+            const float v = fabsf(x.vs);
+            vbad |= !(v < INFINITY);
+            vmax = fmaxf(vmax, v);
+            if (v > 0.0f) vmin = fminf(vmin, v);
+            const float vtop = __int_as_float(__builtin_amdgcn_readlane(wave_inclusive_max_nonneg(__float_as_int(v)), kWave - 1));
+            const float lv = static_cast<float>(min(max(__builtin_amdgcn_frexp_expf(vtop), -60), 60));
+            times_lanes(p, __shfl(x.ks, scale_key));
+            const int t0 = k0 + blk * 32;
+            if (t0 + 32 > keys_all) {
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (t0 + 8 * (i / 4) + 4 * h + i % 4 >= keys) p[i] = -INFINITY;
+            }
+            float top = p[0];
+#pragma unroll
+            for (int i = 1; i < 16; i++) top = fmaxf(top, p[i]);
+            const float u = fmaf(top, c_row, lv);
+            if (__builtin_amdgcn_ballot_w64(u > m + kWeightTop) != 0) {
+                const float un = fmaxf(u, __shfl_xor(u, 32)) - kWeightReset;
+                const float mn = un > m ? un : m;
+                const float alpha = mn == -INFINITY ? 1.0f : fast_exp2(m - mn);
+                m = mn;
+                l *= alpha;
+#pragma unroll
+                for (int c = 0; c < NB; c++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[c][i] *= alpha;
+            }
+            const float ms = m == -INFINITY ? 0.0f : m;
+            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                p[i] = fast_exp2(fmaf(p[i], c_row, -ms));
+                part[i % 4] += p[i];
+            }
+            l += (part[0] + part[1]) + (part[2] + part[3]);
+            times_lanes(p, __shfl(x.vs, scale_key));
+            h16x8 w[LIMBS][2];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                float y = p[i];
+                if (LIMBS == 2) asm("" : "+v"(y));  // one value for both limbs, as in softmax()
+                const _Float16 hi = static_cast<_Float16>(y);
+                w[0][i / 8][i % 8] = hi;
+                if (LIMBS == 2) w[LIMBS - 1][i / 8][i % 8] = static_cast<_Float16>(y - static_cast<float>(hi));
+            }
+            wave_sync();
+            // Lanes 2 r and 2 r + 1 of each 16 address row r of eight; lane i gets column i.
+            const int r8 = c16 >> 1;
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int c = 0; c < NB; c++) {
+                    const int8_t* src = vl + (16 * n + 8 * (r8 >> 2) + 4 * h + (r8 & 3)) * VS8 + 32 * c + 16 * ((lane >> 4) & 1) + 8 * (c16 & 1);
+                    const i32x2 b = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(const_cast<int8_t*>(src)));
+                    const h16x8 y = exact(make_int2(b[0], b[1]));
+                    o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, w[0][n], o[c], 0, 0, 0);
+                    if (LIMBS == 2) o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, w[LIMBS - 1][n], o[c], 0, 0, 0);
+                }
+        };
+        __syncthreads();
+        if (wave < blocks) {
+            Block cur;
+            load(cur, wave, id_of(wave));
+            int id = id_of(wave + W);
+            for (int b = wave; b < blocks; b += W) {
+                Block next;
+                load(next, b + W, id);  // (past the end: the last key's again)
+                id = id_of(b + 2 * W);
+                compute(cur, b);
+                cur = next;
+            }
+        }
+        // The waves' states: every wave finds the common reference, then the upper half
+        // of the waves hands its sums to the lower one, and so on.
+        __shared__ float s_ml[W][32][2];
+        l += __shfl_xor(l, 32);
+        if (h == 0) s_ml[wave][c32][0] = m, s_ml[wave][c32][1] = l;
+        const bool odd = __builtin_amdgcn_ballot_w64(vbad || kmax > kKsMax) != 0;
+        const float vtop = wave_max(vmax), vlow = -wave_max(-vmin);
+        __shared__ float s_range[W][3];
+        if (lane == 0) s_range[wave][0] = vtop, s_range[wave][1] = vlow, s_range[wave][2] = odd ? 1.0f : 0.0f;
+        __syncthreads();
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int i = 0; i < W; i++) M = fmaxf(M, s_ml[i][c32][0]);
+        const float Ms = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+        for (int i = 0; i < W; i++) L = fmaf(s_ml[i][c32][1], fast_exp2(s_ml[i][c32][0] - Ms), L);
+        const float f = fast_exp2(m - Ms);
+#pragma unroll
+        for (int c = 0; c < NB; c++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[c][i] *= f;
+        float* const s_o = reinterpret_cast<float*>(s_buf);
+#pragma unroll
+        for (int half = W / 2; half >= 1; half /= 2) {
+            __syncthreads();
+            float* const at = s_o + (wave % half) * (32 * D) + lane * 4;
+            if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                for (int c = 0; c < NB; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        *reinterpret_cast<float4*>(at + (4 * c + i) * 256) =
+                            make_float4(o[c][4 * i], o[c][4 * i + 1], o[c][4 * i + 2], o[c][4 * i + 3]);
+            }
+            __syncthreads();
+            if (wave < half) {
+#pragma unroll
+                for (int c = 0; c < NB; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float4 y = *reinterpret_cast<const float4*>(at + (4 * c + i) * 256);
+                        o[c][4 * i] += y.x, o[c][4 * i + 1] += y.y, o[c][4 * i + 2] += y.z, o[c][4 * i + 3] += y.w;
+                    }
+            }
+        }
+        m = M;
+        l = 0.5f * L;  // (the halves of the lanes are added below)
+        if (wave != 0) live = false, wave_rows = 0;
+        // One wave's ranges for all.
+        vmax = 0.0f, vmin = INFINITY, vbad = false;
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+            vmax = fmaxf(vmax, s_range[i][0]);
+            vmin = fminf(vmin, s_range[i][1]);
+            vbad |= s_range[i][2] != 0.0f;
+        }
+        __syncthreads();
+    } else {
+        __syncthreads();
+        if (tiles > 0) {
+            read_places(0);
+            load_tile();
+            read_places(1);
+            store_tile(0);
+            if (tiles > 1) load_tile();
+        }
+        __syncthreads();
+        if constexpr (kPhased) {
+            // Two phases a tile, a barrier after each: matrix cores (PV of tile i - 1, QK
+            // of tile i), then vector ALU (softmax of tile i, codes of tile i + 1).  The
+            // V waves are one phase behind the K waves, so a SIMD's two waves, one of
+            // each, use different units.  K waves are in phases 2 i and 2 i + 1, V waves
+            // in 2 i + 1 and 2 i + 2.
+            // * K of tile i + 1 is stored in phase 2 i + 1: its buffer's last readers (QK
+            //   of i - 1) were V waves in phase 2 i - 1, its first is a K wave in 2 i + 2.
+            // * V of tile i + 1 is stored in phase 2 i + 2: last read (PV of i - 1) by V
+            //   waves in phase 2 i + 1, first by K waves in 2 i + 4.
+            // * Wave 0 writes places of tile i + 3 and scales of tile i + 2 in phase 2 i, where
+            //   V waves may still read those of tile i - 1: there are eight slots.
+            // Every wave passes 2 tiles + 1 barriers.
+            if (is_v) __syncthreads();
+            auto stage = [&](int i) {
+                if (i + 1 < tiles) {
+                    store_tile(i + 1);
+                    if (i + 2 < tiles) load_tile();
+                }
+                __syncthreads();
+            };
+            if (wave_rows > 0 && tiles > 0) {
+                read_places(2);
+                matrix(no, yes, 0, 0);
+                ahead(0);
+                __syncthreads();
+                softmax(0);
+                stage(0);
+                for (int i = 1; i < tiles; i++) {
+                    read_places(i + 2);
+                    matrix(yes, yes, i - 1, i);
+                    ahead(i);
+                    __syncthreads();
+                    softmax(i);
+                    stage(i);
+                }
+                matrix(yes, no, tiles - 1, 0);
+            } else {
+                for (int i = 0; i < tiles; i++) {
+                    read_places(i + 2);
+                    ahead(i);
+                    __syncthreads();
+                    stage(i);
+                }
+            }
+            if (!is_v) __syncthreads();
+        } else {
+            // Tile i + 1 becomes f16 in the buffer that was last read before the last
+            // barrier; codes of tile i + 2 are on their way.
+            for (int i = 0; i < tiles; i++) {
+                if (i + 1 < tiles) {
+                    read_places(i + 2);
+                    store_tile(i + 1);
+                    if (i + 2 < tiles) load_tile();
+                }
+                ahead(i);
+                if (wave_rows > 0) {
+                    matrix(no, yes, 0, i);
+                    softmax(i);
+                    matrix(yes, no, i, 0);
+                }
+                __syncthreads();
+            }
+        }
         __syncthreads();
     }
 

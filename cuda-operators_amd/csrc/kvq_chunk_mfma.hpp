@@ -61,8 +61,8 @@ __device__ __forceinline__ void times_lanes(f32x16& x, float y) {
 // over key blocks [k0, k1) of the tile's, as split `split` of nsplit.
 struct ChunkItem {
     int b, tile, split, nsplit;
-    int unit;  // split tiles' counter
     int rec;   // first of the tile's records
+    ChunkSeq seq;
 };
 
 // Sequence b's query tiles and key blocks.
@@ -78,7 +78,7 @@ __device__ __forceinline__ void chunk_counts(const ChunkArgs& a, const ChunkSeq&
 struct ChunkPlanLds {
     int part[8], best[8];
     int tiles[512], blocks[512];
-    int found[6];
+    int found[8];
 };
 template <int W>
 __device__ inline bool chunk_locate(const ChunkArgs& a, ChunkPlanLds& s, int r, ChunkItem& w) {
@@ -106,10 +106,15 @@ __device__ inline bool chunk_locate(const ChunkArgs& a, ChunkPlanLds& s, int r, 
         return before + incl - v;
     };
     int mine = 0, first_tiles = 0, first_blocks = 0;
-    for (int i = 0; i < per; i++) {
+    ChunkSeq first{};
+    if (b0 < a.B) {
+        first = chunk_seq(a, b0);
+        chunk_counts(a, first, first_tiles, first_blocks);
+        mine = first_tiles;
+    }
+    for (int i = 1; i < per; i++) {
         int tiles, blocks;
         counts(b0 + i, tiles, blocks);
-        if (i == 0) first_tiles = tiles, first_blocks = blocks;
         mine += tiles;
     }
     int all;
@@ -151,6 +156,10 @@ __device__ inline bool chunk_locate(const ChunkArgs& a, ChunkPlanLds& s, int r, 
                 s.found[2] = local - tile * nsplit;
                 s.found[3] = nsplit;
                 s.found[4] = at + tile * nsplit;
+                const ChunkSeq q = i > 0 ? chunk_seq(a, b0 + i) : first;
+                s.found[5] = q.row0;
+                s.found[6] = q.n;
+                s.found[7] = q.len;
                 break;
             }
             at += tiles * nsplit;
@@ -162,6 +171,9 @@ __device__ inline bool chunk_locate(const ChunkArgs& a, ChunkPlanLds& s, int r, 
     w.split = __builtin_amdgcn_readfirstlane(s.found[2]);
     w.nsplit = __builtin_amdgcn_readfirstlane(s.found[3]);
     w.rec = __builtin_amdgcn_readfirstlane(s.found[4]);
+    w.seq.row0 = __builtin_amdgcn_readfirstlane(s.found[5]);
+    w.seq.n = __builtin_amdgcn_readfirstlane(s.found[6]);
+    w.seq.len = __builtin_amdgcn_readfirstlane(s.found[7]);
     return true;
 }
 
@@ -256,7 +268,7 @@ chunk_mfma(const ChunkArgs a) {
     const int kvh = static_cast<int>(blockIdx.x) - r * a.Hkv;
     ChunkItem w;
     if (!chunk_locate<W>(a, s_plan, r, w)) return;
-    const ChunkSeq s = chunk_seq(a, w.b);
+    const ChunkSeq s = w.seq;
     const int i0 = w.tile * a.tile_tokens;                       // the tile's new tokens
     const int tokens = min(a.tile_tokens, s.n - i0);
     const int kend = chunk_keys(a, s, i0 + tokens - 1);          // keys that any of them attends
@@ -375,16 +387,63 @@ chunk_mfma(const ChunkArgs a) {
             x.unit = ldexpf(1.0f, -e);
         }
     };
-    int next_id = 0;
+    int far_id = 0;
     if (tiles > 0 && wave == 0 && !narrow) {
         const int id0 = table[page_of(0)], id1 = table[page_of(1)], id2 = table[page_of(2)];
-        next_id = table[page_of(3)];
+        far_id = table[page_of(3)];
         load_scales(0, pool_row(0, id0));
         store_scales(0);
         load_scales(1, pool_row(1, id1));
         store_scales(1);
         load_scales(2, pool_row(2, id2));
     }
+
+    // Narrow tiles: a block's codes and scales.
+    constexpr int NK = D / 32;    // 16-byte pieces of K, and of V, a lane,
+    constexpr int LPV = D / 16;   // lanes a row of V
+    struct Block {
+        int4 k[NK], v[NK];
+        float ks, vs;
+    };
+    const int blocks = (k1 - k0 + 31) / 32;
+    auto key_of = [&](int blk, int r) { return min(k0 + blk * 32 + r, max(k1 - 1, 0)); };
+    auto id_of = [&](int blk) { return table[fastdiv(key_of(blk, c32), a.page)]; };
+    auto piece = [&](const int8_t* src, long long at, int c) {  // codes c .. c + 15 of a row, zeros past its end
+        int4 x = make_int4(0, 0, 0, 0);
+        if (c + 16 <= a.d) {
+            x = *reinterpret_cast<const int4*>(src + at + c);
+        } else if (c < a.d) {
+            const int2 y = *reinterpret_cast<const int2*>(src + at + c);
+            x.x = y.x, x.y = y.y;
+        }
+        return x;
+    };
+    auto load = [&](Block& x, int blk, int id) __attribute__((always_inline)) {
+        const int key = key_of(blk, c32);
+        const int page = static_cast<int>(fastdiv(key, a.page));
+        id = min(max(id, 0), a.pages.num_pages - 1);
+        const long long mine = (static_cast<long long>(id) * a.Hkv + kvh) * a.pages.size + (key - page * a.pages.size);
+#pragma unroll
+        for (int j = 0; j < NK; j++) x.k[j] = piece(a.k, mine * a.d, 32 * j + 16 * h);
+#pragma unroll
+        for (int j = 0; j < NK; j++) {
+            const int n = j * kWave + lane;
+            x.v[j] = piece(a.v, __shfl(mine, n / LPV) * a.d, n % LPV * 16);
+        }
+        const bool in = k0 + blk * 32 + c32 < k1;
+        x.ks = in ? a.ks[mine] : 0.0f;
+        x.vs = in ? a.vs[mine] : 0.0f;
+    };
+    // The first block is on its way while q is fetched, where registers allow.
+    constexpr bool kEarly = LIMBS == 1 && D <= 192;
+    Block cur;
+    int next_id = 0;
+    auto load_first = [&]() __attribute__((always_inline)) {
+        const int id = id_of(wave);
+        next_id = id_of(wave + W);
+        load(cur, wave, id);
+    };
+    if (kEarly && narrow && wave < blocks) load_first();
 
     // q^T operands: lane has dims chunk_dim_of(n, h) + [0, 8) of its row, scaled to 2^15.
     h16x8 q[LIMBS][NS];
@@ -552,56 +611,60 @@ chunk_mfma(const ChunkArgs a) {
     auto ahead = [&](int i) {
         if (wave == 0 && i + 2 < tiles) {
             store_scales(i + 2);
-            if (i + 3 < tiles) load_scales(i + 3, pool_row(i + 3, next_id));
-            next_id = table[page_of(i + 4)];
+            if (i + 3 < tiles) load_scales(i + 3, pool_row(i + 3, far_id));
+            far_id = table[page_of(i + 4)];
         }
     };
 
+    const bool whole = w.nsplit == 1;
+    const size_t item = static_cast<size_t>(w.rec + w.split) * a.Hkv + kvh;
+    const buf_rsrc acc_rs = make_rsrc(a.part_acc + (whole ? 0 : item * kChunkRows * D), kChunkRows * D * 4u);
+    const buf_rsrc ml_rs = make_rsrc(a.part_ml + (whole ? 0 : item * kChunkRows * 2), kChunkRows * 8u);
+    const int64_t o_at = static_cast<int64_t>(s.row0 + i0 + tok) * a.out_stride + static_cast<int64_t>(head) * a.d;
+    auto put4 = [&](int64_t at, float x, float y, float z, float u) {
+        if (LIMBS == 1) {
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) =
+                make_uint2(bf16_of(x) | static_cast<unsigned>(bf16_of(y)) << 16, bf16_of(z) | static_cast<unsigned>(bf16_of(u)) << 16);
+        } else {
+            *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(x, y, z, u);
+        }
+    };
+    // Four sums of this lane's row, dims 32 (g / 4) + 8 (g % 4) + 4 h: the output, or a
+    // record of a split.
+    auto store_group = [&](int g, float4 x, float l_row) __attribute__((always_inline)) {
+        const int dim = 32 * (g >> 2) + 8 * (g & 3) + 4 * h;
+        if (!live) return;
+        if (whole) {
+            if (dim >= a.d) return;
+            const float inv = 1.0f / l_row;
+            if (keys > 0) put4(o_at + dim, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+            else put4(o_at + dim, 0.0f, 0.0f, 0.0f, 0.0f);
+        } else {
+            const v4i_t y = {__float_as_int(x.x), __float_as_int(x.y), __float_as_int(x.z), __float_as_int(x.w)};
+            __builtin_amdgcn_raw_buffer_store_b128(y, acc_rs, (row * D + dim) * 4, 0, kChunkCoherent);
+        }
+    };
+    auto store_state = [&](float m_row, float l_row) __attribute__((always_inline)) {
+        typedef int v2i_t __attribute__((ext_vector_type(2)));
+        __builtin_amdgcn_raw_buffer_store_b64(v2i_t{__float_as_int(m_row), __float_as_int(l_row)}, ml_rs, row * 8, 0, kChunkCoherent);
+    };
+
+    // Whether the scales that this wave knows of are beyond f16 weights, or q scaled to 2^15.
+    auto out_of_range = [&]() {
+        const float top = wave_max(vmax), low = -wave_max(-vmin);
+        return __builtin_amdgcn_ballot_w64(vbad || kmax > kKsMax) != 0 ||
+               (top > 0.0f && (top > kVsMax || low < kVsMin || top > low * kVsRatio<LIMBS>));
+    };
     if (narrow) {
         // Each wave takes every W-th block of 32 keys, with nothing to wait for but its
         // own loads: K codes come as A operands straight from memory, V codes through a
         // part of LDS of the wave's own, read transposed.  The waves' states are joined
         // at the end.
         constexpr int VS8 = D + 16;   // LDS row stride of V codes
-        constexpr int NK = D / 32;    // 16-byte pieces of K a lane,
-        constexpr int LPV = D / 16;   // lanes a row of V,
         static_assert(W * 32 * VS8 <= sizeof(s_buf) && W / 2 * 32 * D * 4 <= sizeof(s_buf), "LDS");
         typedef int i32x2 __attribute__((ext_vector_type(2)));
         typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
         int8_t* const vl = reinterpret_cast<int8_t*>(s_buf) + wave * 32 * VS8;
-        struct Block {
-            int4 k[NK], v[NK];
-            float ks, vs;
-        };
-        const int blocks = (k1 - k0 + 31) / 32;
-        auto key_of = [&](int blk, int r) { return min(k0 + blk * 32 + r, max(k1 - 1, 0)); };
-        auto id_of = [&](int blk) { return table[fastdiv(key_of(blk, c32), a.page)]; };
-        auto piece = [&](const int8_t* src, long long at, int c) {  // codes c .. c + 15 of a row, zeros past its end
-            int4 x = make_int4(0, 0, 0, 0);
-            if (c + 16 <= a.d) {
-                x = *reinterpret_cast<const int4*>(src + at + c);
-            } else if (c < a.d) {
-                const int2 y = *reinterpret_cast<const int2*>(src + at + c);
-                x.x = y.x, x.y = y.y;
-            }
-            return x;
-        };
-        auto load = [&](Block& x, int blk, int id) __attribute__((always_inline)) {
-            const int key = key_of(blk, c32);
-            const int page = static_cast<int>(fastdiv(key, a.page));
-            id = min(max(id, 0), a.pages.num_pages - 1);
-            const long long mine = (static_cast<long long>(id) * a.Hkv + kvh) * a.pages.size + (key - page * a.pages.size);
-#pragma unroll
-            for (int j = 0; j < NK; j++) x.k[j] = piece(a.k, mine * a.d, 32 * j + 16 * h);
-#pragma unroll
-            for (int j = 0; j < NK; j++) {
-                const int n = j * kWave + lane;
-                x.v[j] = piece(a.v, __shfl(mine, n / LPV) * a.d, n % LPV * 16);
-            }
-            const bool in = k0 + blk * 32 + c32 < k1;
-            x.ks = in ? a.ks[mine] : 0.0f;
-            x.vs = in ? a.vs[mine] : 0.0f;
-        };
         const int scale_key = 8 * (c16 >> 2) + 4 * h + (c16 & 3);
         auto compute = [&](const Block& x, int blk) __attribute__((always_inline)) {
             wave_sync();
@@ -686,13 +749,11 @@ chunk_mfma(const ChunkArgs a) {
         };
         __syncthreads();
         if (wave < blocks) {
-            Block cur;
-            load(cur, wave, id_of(wave));
-            int id = id_of(wave + W);
+            if (!kEarly) load_first();
             for (int b = wave; b < blocks; b += W) {
                 Block next;
-                load(next, b + W, id);  // (past the end: the last key's again)
-                id = id_of(b + 2 * W);
+                load(next, b + W, next_id);  // (past the end: the last key's again)
+                next_id = id_of(b + 2 * W);
                 compute(cur, b);
                 cur = next;
             }
@@ -707,6 +768,16 @@ chunk_mfma(const ChunkArgs a) {
         __shared__ float s_range[W][3];
         if (lane == 0) s_range[wave][0] = vtop, s_range[wave][1] = vlow, s_range[wave][2] = odd ? 1.0f : 0.0f;
         __syncthreads();
+        // One wave's ranges for all.
+        vmax = 0.0f, vmin = INFINITY, vbad = false;
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+            vmax = fmaxf(vmax, s_range[i][0]);
+            vmin = fminf(vmin, s_range[i][1]);
+            vbad |= s_range[i][2] != 0.0f;
+        }
+        // (rows that are computed again are not stored here)
+        const bool stored = !out_of_range();
         float M = -INFINITY, L = 0.0f;
 #pragma unroll
         for (int i = 0; i < W; i++) M = fmaxf(M, s_ml[i][c32][0]);
@@ -718,41 +789,35 @@ chunk_mfma(const ChunkArgs a) {
         for (int c = 0; c < NB; c++)
 #pragma unroll
             for (int i = 0; i < 16; i++) o[c][i] *= f;
-        float* const s_o = reinterpret_cast<float*>(s_buf);
+        // Sums go through LDS in groups of 64 lanes' four values; wave g % W adds up
+        // group g of all waves, and stores it.
+        constexpr int kGroups = 4 * NB;
+        constexpr int kRound = kGroups % 16 == 0 && W * 16 * 1024 <= sizeof(s_buf) ? 16 : kGroups % 8 == 0 && W * 8 * 1024 <= sizeof(s_buf) ? 8 : 4;
+        static_assert(kGroups % kRound == 0 && W * kRound * 1024 <= sizeof(s_buf), "LDS");
+        float4* const s_o = reinterpret_cast<float4*>(s_buf);
 #pragma unroll
-        for (int half = W / 2; half >= 1; half /= 2) {
+        for (int g0 = 0; g0 < kGroups; g0 += kRound) {
             __syncthreads();
-            float* const at = s_o + (wave % half) * (32 * D) + lane * 4;
-            if (wave >= half && wave < 2 * half) {
 #pragma unroll
-                for (int c = 0; c < NB; c++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        *reinterpret_cast<float4*>(at + (4 * c + i) * 256) =
-                            make_float4(o[c][4 * i], o[c][4 * i + 1], o[c][4 * i + 2], o[c][4 * i + 3]);
-            }
+            for (int g = g0; g < g0 + kRound; g++)
+                s_o[(wave * kRound + g - g0) * kWave + lane] =
+                    make_float4(o[g / 4][4 * (g % 4)], o[g / 4][4 * (g % 4) + 1], o[g / 4][4 * (g % 4) + 2], o[g / 4][4 * (g % 4) + 3]);
             __syncthreads();
-            if (wave < half) {
 #pragma unroll
-                for (int c = 0; c < NB; c++)
+            for (int n = 0; n < (kRound + W - 1) / W; n++) {
+                const int g = g0 + n * W + wave;
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (n * W + wave < kRound) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float4 y = *reinterpret_cast<const float4*>(at + (4 * c + i) * 256);
-                        o[c][4 * i] += y.x, o[c][4 * i + 1] += y.y, o[c][4 * i + 2] += y.z, o[c][4 * i + 3] += y.w;
+                    for (int i = 0; i < W; i++) {
+                        const float4 y = s_o[(i * kRound + n * W + wave) * kWave + lane];
+                        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
                     }
+                    if (stored) store_group(g, x, L);
+                }
             }
         }
-        m = M;
-        l = 0.5f * L;  // (the halves of the lanes are added below)
-        if (wave != 0) live = false, wave_rows = 0;
-        // One wave's ranges for all.
-        vmax = 0.0f, vmin = INFINITY, vbad = false;
-#pragma unroll
-        for (int i = 0; i < W; i++) {
-            vmax = fmaxf(vmax, s_range[i][0]);
-            vmin = fminf(vmin, s_range[i][1]);
-            vbad |= s_range[i][2] != 0.0f;
-        }
+        if (stored && !whole && live && h == 0 && wave == 0) store_state(M, L);
         __syncthreads();
     } else {
         __syncthreads();
@@ -833,51 +898,21 @@ chunk_mfma(const ChunkArgs a) {
 
     // Scales that f16 weights, or q scaled to 2^15, do not cover.
     if (wave == 0) {
-        const float top = wave_max(vmax), low = -wave_max(-vmin);
-        const bool bad = __builtin_amdgcn_ballot_w64(vbad || kmax > kKsMax) != 0 ||
-                         (top > 0.0f && (top > kVsMax || low < kVsMin || top > low * kVsRatio<LIMBS>));
+        const bool bad = out_of_range();
         if (lane == 0) s_flag = bad;
     }
     __syncthreads();
-    l += __shfl_xor(l, 32);
     const bool exact = s_flag != 0;
-    const bool whole = w.nsplit == 1;
-    const size_t item = static_cast<size_t>(w.rec + w.split) * a.Hkv + kvh;
-    const buf_rsrc acc_rs = make_rsrc(a.part_acc + (whole ? 0 : item * kChunkRows * D), kChunkRows * D * 4u);
-    const buf_rsrc ml_rs = make_rsrc(a.part_ml + (whole ? 0 : item * kChunkRows * 2), kChunkRows * 8u);
-    const int64_t o_at = static_cast<int64_t>(s.row0 + i0 + tok) * a.out_stride + static_cast<int64_t>(head) * a.d;
-    auto put4 = [&](int64_t at, float x, float y, float z, float u) {
-        if (LIMBS == 1) {
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) =
-                make_uint2(bf16_of(x) | static_cast<unsigned>(bf16_of(y)) << 16, bf16_of(z) | static_cast<unsigned>(bf16_of(u)) << 16);
-        } else {
-            *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(x, y, z, u);
-        }
-    };
     if (!exact) {
-        if (live) {
-            const float inv = keys > 0 ? 1.0f / l : 0.0f;
+        if (live && !narrow) {
+            l += __shfl_xor(l, 32);
 #pragma unroll
-            for (int c = 0; c < NB; c++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int dim = 32 * c + 8 * j + 4 * h;
-                    if (whole) {
-                        if (dim >= a.d) continue;
-                        if (keys > 0) put4(o_at + dim, o[c][4 * j] * inv, o[c][4 * j + 1] * inv, o[c][4 * j + 2] * inv, o[c][4 * j + 3] * inv);
-                        else put4(o_at + dim, 0.0f, 0.0f, 0.0f, 0.0f);
-                    } else {
-                        const v4i_t x = {__float_as_int(o[c][4 * j]), __float_as_int(o[c][4 * j + 1]),
-                                         __float_as_int(o[c][4 * j + 2]), __float_as_int(o[c][4 * j + 3])};
-                        __builtin_amdgcn_raw_buffer_store_b128(x, acc_rs, (row * D + dim) * 4, 0, kChunkCoherent);
-                    }
-                }
-            if (!whole && h == 0) {
-                typedef int v2i_t __attribute__((ext_vector_type(2)));
-                __builtin_amdgcn_raw_buffer_store_b64(v2i_t{__float_as_int(m), __float_as_int(l)}, ml_rs, row * 8, 0, kChunkCoherent);
-            }
+            for (int g = 0; g < 4 * NB; g++)
+                store_group(g, make_float4(o[g / 4][4 * (g % 4)], o[g / 4][4 * (g % 4) + 1], o[g / 4][4 * (g % 4) + 2], o[g / 4][4 * (g % 4) + 3]), l);
+            if (!whole && h == 0) store_state(m, l);
         }
     } else {
+        if (narrow && wave > 0) wave_rows = 0;
         float* const scratch = reinterpret_cast<float*>(s_buf) + wave * (2 * D + kWave + 2 * kWave);
         const float* s_acc = scratch + D;
         for (int j = 0; j < wave_rows; j++) {
@@ -917,28 +952,44 @@ chunk_mfma(const ChunkArgs a) {
     constexpr int LPR = D / 4;                   // lanes a row
     constexpr int RPP = kChunkThreads / LPR;     // rows a pass
     const int live_rows = tokens * a.G;
+    // Records of eight splits are on their way together.
+    constexpr int kDeep = 8;
+    const unsigned step_acc = a.Hkv * kChunkRows * D * 4u, step_ml = a.Hkv * kChunkRows * 8u;
+    const unsigned span = static_cast<unsigned>(w.nsplit - 1);
+    const buf_rsrc accs = make_rsrc(a.part_acc + rec0 * kChunkRows * D, span * step_acc + kChunkRows * D * 4u);
+    const buf_rsrc mls = make_rsrc(a.part_ml + rec0 * kChunkRows * 2, span * step_ml + kChunkRows * 8u);
     for (int jr = t / LPR; jr < live_rows; jr += RPP) {
         if (t / LPR >= RPP) break;
         const int dim = 4 * (t % LPR);
-        float M = -INFINITY;
-        for (int i = 0; i < w.nsplit; i++) {
-            const float* ml = a.part_ml + ((rec0 + static_cast<size_t>(i) * a.Hkv) * kChunkRows + jr) * 2;
-            M = fmaxf(M, __hip_atomic_load(ml, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-        }
-        const float Ms = M == -INFINITY ? 0.0f : M;
-        float L = 0.0f, A[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int i = 0; i < w.nsplit; i++) {
-            const size_t rec = rec0 + static_cast<size_t>(i) * a.Hkv;
-            const float* ml = a.part_ml + (rec * kChunkRows + jr) * 2;
-            const float mi = __hip_atomic_load(ml, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const float li = __hip_atomic_load(ml + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const buf_rsrc rs = make_rsrc(a.part_acc + rec * kChunkRows * D, kChunkRows * D * 4u);
-            const v4i_t x = __builtin_amdgcn_raw_buffer_load_b128(rs, (jr * D + dim) * 4, 0, kChunkCoherent);
-            if (mi == -INFINITY && li == 0.0f) continue;  // no key of this split
-            const float f = fast_exp2(mi - Ms);
-            L = fmaf(li, f, L);
+        float M = -INFINITY, L = 0.0f, A[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i0 = 0; i0 < w.nsplit; i0 += kDeep) {
+            typedef int v2i_t __attribute__((ext_vector_type(2)));
+            v2i_t ml[kDeep];
+            v4i_t acc[kDeep];
 #pragma unroll
-            for (int j = 0; j < 4; j++) A[j] = fmaf(__int_as_float(x[j]), f, A[j]);
+            for (int i = 0; i < kDeep; i++) {  // (past the last split: the last one's again, left out below)
+                const int at = min(i0 + i, w.nsplit - 1);
+                ml[i] = __builtin_bit_cast(v2i_t, __builtin_amdgcn_raw_buffer_load_b64(mls, jr * 8 + at * step_ml, 0, kChunkCoherent));
+                acc[i] = __builtin_amdgcn_raw_buffer_load_b128(accs, (jr * D + dim) * 4 + at * step_acc, 0, kChunkCoherent);
+            }
+            float top = M;
+#pragma unroll
+            for (int i = 0; i < kDeep; i++) top = fmaxf(top, __int_as_float(ml[i].x));
+            const float Ms = top == -INFINITY ? 0.0f : top;
+            const float alpha = fast_exp2(M - Ms);
+            M = top;
+            L *= alpha;
+#pragma unroll
+            for (int j = 0; j < 4; j++) A[j] *= alpha;
+#pragma unroll
+            for (int i = 0; i < kDeep; i++) {
+                const float mi = __int_as_float(ml[i].x), li = __int_as_float(ml[i].y);
+                if (i0 + i >= w.nsplit || (mi == -INFINITY && li == 0.0f)) continue;  // (or no key of this split)
+                const float f = fast_exp2(mi - Ms);
+                L = fmaf(li, f, L);
+#pragma unroll
+                for (int j = 0; j < 4; j++) A[j] = fmaf(__int_as_float(acc[i][j]), f, A[j]);
+            }
         }
         const int jt = static_cast<int>(fastdiv(jr, a.group));
         const int jh = kvh * a.G + jr - jt * a.G;

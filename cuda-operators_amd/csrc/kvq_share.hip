@@ -88,41 +88,48 @@ __global__ __launch_bounds__(256) void fork_count_kernel(const ForkArgs a) {
     }
 }
 
+// Pages that have become free, kPer a thread and pass, so that a pass of 8192
+// pages costs two barriers; then the rows, in order.
 __global__ __launch_bounds__(kThreads) void fork_decide_kernel(const ForkArgs a) {
+    constexpr int kPer = 8;
     __shared__ int s_part[kWaves];
-    const int t = threadIdx.x;
+    const unsigned t = threadIdx.x;
     const int F = min(max(*a.free_count, 0), a.num_pages);
-
-    // Pages that have become free.
-    int freed = 0;
     const unsigned P = static_cast<unsigned>(a.num_pages);
-    for (unsigned p0 = 0; p0 < P; p0 += kThreads) {
-        const unsigned p = p0 + t;
-        int gone = 0;
-        if (p < P) {
-            const int delta = a.delta[p];
-            gone = delta < 0 && a.shares[p] + 1 + delta <= 0;
+    int freed = 0;
+    for (unsigned p0 = 0; p0 < P; p0 += kThreads * kPer) {
+        int delta[kPer], gone[kPer], mine = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const unsigned p = p0 + t * kPer + i;
+            delta[i] = p < P ? a.delta[p] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            gone[i] = delta[i] < 0 && a.shares[p0 + t * kPer + i] + 1 + delta[i] <= 0;
+            mine += gone[i];
         }
         int total;
-        const int at = freed + group_scan(gone, total, s_part) - gone;
-        if (gone) a.freed[at] = static_cast<int>(p);
+        int at = freed + group_scan(mine, total, s_part) - mine;
+#pragma unroll
+        for (int i = 0; i < kPer; i++)
+            if (gone[i]) a.freed[at++] = static_cast<int>(p0 + t * kPer + i);
         freed += total;
     }
     __syncthreads();
     const long long have = static_cast<long long>(F) + freed;
     auto stack_at = [&](long long i) { return i < F ? a.free_pages[i] : a.freed[i - F]; };
 
-    // Rows that need a page of their own.
     int copies = 0;
     for (int b0 = 0; b0 < a.B; b0 += kThreads) {
-        const int b = b0 + t;
+        const int b = b0 + static_cast<int>(t);
         int need = 0, page = -1, n = 0;
         if (b < a.B) {
             n = a.want[b];
+            a.want[b] = 0;
             const int whole = static_cast<int>(fastdiv(static_cast<uint32_t>(n), a.page));
             if (whole * static_cast<int>(a.page.d) < n) {
-                const int parent = a.parents[b];
-                page = a.table[static_cast<size_t>(parent) * a.max_pages + whole];
+                page = a.table[static_cast<size_t>(a.parents[b]) * a.max_pages + whole];
                 if (page >= 0 && page < a.num_pages) {
                     const int held = a.shares[page] + 1 + a.delta[page];
                     need = held > 1 && !(held <= a.writers[page] && a.first[page] == a.B - b);
@@ -136,57 +143,54 @@ __global__ __launch_bounds__(kThreads) void fork_decide_kernel(const ForkArgs a)
             int dst = -1;
             if (need) {
                 if (turn < have) dst = stack_at(have - 1 - turn);
-                else n -= n - static_cast<int>(fastdiv(static_cast<uint32_t>(n), a.page) * a.page.d);
+                else n = static_cast<int>(fastdiv(static_cast<uint32_t>(n), a.page) * a.page.d);
             }
             a.copy_src[b] = dst < 0 ? -1 : page;
             a.copy_dst[b] = dst;
-            // A row's place in `want` afterwards: its tokens, and whether it has been cut to whole pages.
-            a.want[b] = n;
+            a.new_lengths[b] = n;
         }
     }
     const long long left = have - min(static_cast<long long>(copies), have);
     __syncthreads();
-
-    // The stack, shares, and the workspace as it was.
     for (unsigned i = t; i < static_cast<unsigned>(freed); i += kThreads) {
         const long long at = static_cast<long long>(F) + i;
         if (at < left && at < a.num_pages) a.free_pages[at] = a.freed[i];
         a.freed[i] = 0;
     }
-    for (unsigned p = t; p < P; p += kThreads) {
-        const int delta = a.delta[p], writers = a.writers[p];
-        int shares = a.shares[p];
-        if (delta != 0 || writers != 0) {
-            const int held = shares + 1 + delta;
-            const int leave = held > 1 ? writers - (held <= writers ? 1 : 0) : 0;
-            shares = max(held - leave - 1, 0);
-            a.delta[p] = 0;
-            a.writers[p] = 0;
-            a.first[p] = 0;
-        }
-        a.new_shares[p] = shares;
-    }
-    __syncthreads();
-    for (int b = t; b < a.B; b += kThreads) {
-        const int dst = a.copy_dst[b];
-        if (dst >= 0 && dst < a.num_pages) a.new_shares[dst] = 0;
-    }
     if (t == 0) *a.new_free_count = static_cast<int>(min(left, static_cast<long long>(a.num_pages)));
 }
 
+// Rows (workgroups blockIdx.y of row blockIdx.x), then in the rows of the grid
+// behind them the pages' shares and the workspace as it was.
 __global__ __launch_bounds__(256) void fork_write_kernel(const ForkArgs a) {
+    if (blockIdx.x >= static_cast<unsigned>(a.B)) {
+        const unsigned groups = (gridDim.x - a.B) * gridDim.y;
+        for (unsigned p = ((blockIdx.x - a.B) * gridDim.y + blockIdx.y) * 256 + threadIdx.x; p < static_cast<unsigned>(a.num_pages);
+             p += groups * 256) {
+            const int delta = a.delta[p], writers = a.writers[p];
+            int shares = a.shares[p];
+            if (delta != 0 || writers != 0) {
+                const int held = shares + 1 + delta;
+                const int leave = held > 1 ? writers - (held <= writers ? 1 : 0) : 0;
+                shares = max(held - leave - 1, 0);
+                a.delta[p] = 0;
+                a.writers[p] = 0;
+                a.first[p] = 0;
+            }
+            a.new_shares[p] = shares;
+        }
+        return;
+    }
     const int b = blockIdx.x;
-    const int n = a.want[b];
-    const int pages = pages_of(n, a.page);
+    const int pages = pages_of(a.new_lengths[b], a.page);
     const int dst = a.copy_dst[b];
     const bool stays = a.parents[b] == b;
     const bool in_place = a.table == a.new_table;
     int32_t* row = a.new_table + static_cast<size_t>(b) * a.max_pages;
     int* stage = a.stage + static_cast<size_t>(b) * a.max_pages;
-    const int step = gridDim.y * 256;
-    // Staged entries go back to 0, those of a page that was cut off too.
+    // Staged entries go back to 0, that of a page that was cut off too.
     const int end = min(pages + 1, a.max_pages);
-    for (int j = blockIdx.y * 256 + threadIdx.x; j < end; j += step) {
+    for (int j = blockIdx.y * 256 + threadIdx.x; j < end; j += gridDim.y * 256) {
         int id = 0;
         if (!stays) {
             id = stage[j];
@@ -200,28 +204,43 @@ __global__ __launch_bounds__(256) void fork_write_kernel(const ForkArgs a) {
     }
 }
 
-// want goes back to 0 only when every row's workgroups have read it.
-__global__ __launch_bounds__(256) void fork_lengths_kernel(const ForkArgs a) {
-    const int b = blockIdx.x * 256 + threadIdx.x;
-    if (b >= a.B) return;
-    a.new_lengths[b] = a.want[b];
-    a.want[b] = 0;
-}
-
 // ---------------------------------------------------------------------------
 // Copies.
 // ---------------------------------------------------------------------------
+// A pair's arrays in one layer are laid end to end in pieces of 16 bytes (or 4, or
+// 1, where an array's place or page size is not a multiple); a workgroup takes
+// kCopyPieces of a thread's at a time, whose loads go out together.
+constexpr int kCopyLoads = 4;
+
+template <class T>
 __global__ __launch_bounds__(256) void page_copy_kernel(const CopyArgs a) {
-    const int i = blockIdx.x;
-    const int layer = blockIdx.y;
+    const unsigned unit = blockIdx.x;  // (layer, pair)
+    const unsigned layer = fastdiv(unit, a.pairs);
+    const int i = static_cast<int>(unit - layer * a.n);
     const int src = a.src[i], dst = a.dst[i];
     if (src < 0 || src >= a.num_pages || dst < 0 || dst >= a.num_pages) return;
+    const size_t first = static_cast<size_t>(layer) * a.num_pages;
+    for (size_t p0 = static_cast<size_t>(blockIdx.y) * (256 * kCopyLoads); p0 < a.pieces;
+         p0 += static_cast<size_t>(gridDim.y) * (256 * kCopyLoads)) {
+        T x[kCopyLoads];
+        char* to[kCopyLoads];
 #pragma unroll
-    for (int k = 0; k < CopyArgs::kArrays; k++) {
-        if (!a.base[k]) continue;
-        const char* x = a.base[k] + (static_cast<size_t>(layer) * a.num_pages + src) * a.bytes[k];
-        char* y = a.base[k] + (static_cast<size_t>(layer) * a.num_pages + dst) * a.bytes[k];
-        for (size_t j = threadIdx.x; j < a.bytes[k]; j += 256) y[j] = x[j];
+        for (int u = 0; u < kCopyLoads; u++) {
+            size_t p = p0 + u * 256 + threadIdx.x;
+            to[u] = nullptr;
+            if (p >= a.pieces) continue;
+            char* base = a.base[0];
+            size_t bytes = a.bytes[0], before = 0;
+#pragma unroll
+            for (int k = 1; k < CopyArgs::kArrays; k++)
+                if (p >= a.begin[k]) base = a.base[k], bytes = a.bytes[k], before = a.begin[k];
+            const size_t at = (p - before) * sizeof(T);
+            x[u] = *reinterpret_cast<const T*>(base + (first + src) * bytes + at);
+            to[u] = base + (first + dst) * bytes + at;
+        }
+#pragma unroll
+        for (int u = 0; u < kCopyLoads; u++)
+            if (to[u]) *reinterpret_cast<T*>(to[u]) = x[u];
     }
 }
 
@@ -294,6 +313,110 @@ __global__ __launch_bounds__(kThreads) void compact_plan_kernel(const CompactArg
     }
 }
 
+// The same with the free pages as bits in LDS, for pools of up to kBitPages: one
+// scan each over the words instead of one over the pages.  Both sets of free pages,
+// before and after the moves, are left in the workspace for the launch behind this.
+constexpr int kBitPages = 1 << 18;  // 32 KB of LDS
+
+__global__ __launch_bounds__(kThreads) void compact_bits_kernel(const CompactArgs a) {
+    extern __shared__ unsigned s_bits[];
+    __shared__ int s_part[kWaves];
+    const int t = threadIdx.x;
+    const int P = a.num_pages, words = (P + 31) / 32, per = (words + kThreads - 1) / kThreads;
+    const int w0 = min(t * per, words), w1 = min(w0 + per, words);
+    for (int w = t; w < words; w += kThreads) s_bits[w] = 0;
+    __syncthreads();
+    const int F = min(max(*a.free_count, 0), P);
+    for (int i = t; i < F; i += kThreads) {
+        const int p = a.free_pages[i];
+        if (p >= 0 && p < P) atomicOr(&s_bits[p >> 5], 1u << (p & 31));
+    }
+    __syncthreads();
+    auto valid = [&](int w) { return w == words - 1 && (P & 31) ? (1u << (P & 31)) - 1 : ~0u; };
+    int count = 0, total;
+    for (int w = w0; w < w1; w++) {
+        a.before[w] = s_bits[w];
+        count += __popc(s_bits[w]);
+    }
+    group_scan(count, total, s_part);
+    const int used = P - total;
+    auto below = [&](int w) {  // the word's pages before `used`
+        const int n = used - 32 * w;
+        return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1;
+    };
+    int holes = 0, highs = 0;
+    for (int w = w0; w < w1; w++) {
+        holes += __popc(s_bits[w] & below(w));
+        highs += __popc(~s_bits[w] & ~below(w) & valid(w));
+    }
+    int all_holes, all_highs;
+    int hole = group_scan(holes, all_holes, s_part) - holes;
+    int high = group_scan(highs, all_highs, s_part);  // the lowest of this thread's is the high-th from the top
+    high = all_highs - (high - highs) - 1;
+    const int moves = min(all_holes, a.max_moves);
+    for (int w = w0; w < w1; w++) {
+        unsigned x = s_bits[w] & below(w), y = ~s_bits[w] & ~below(w) & valid(w), now = s_bits[w];
+        for (; x; x &= x - 1, hole++) {
+            const int bit = __ffs(x) - 1;
+            if (hole >= moves) break;
+            a.copy_dst[hole] = 32 * w + bit;
+            now &= ~(1u << bit);
+        }
+        for (; y; y &= y - 1, high--) {
+            const int bit = __ffs(y) - 1;
+            if (high >= moves) continue;
+            a.copy_src[high] = 32 * w + bit;
+            now |= 1u << bit;
+        }
+        s_bits[w] = now;
+        a.after[w] = now;
+    }
+    if (t == 0) *a.moved = moves;
+    // The stack afterwards, descending.
+    count = 0;
+    for (int w = w0; w < w1; w++) count += __popc(s_bits[w]);
+    int at = group_scan(count, total, s_part) - count;  // free pages before this thread's
+    for (int w = w0; w < w1; w++)
+        for (unsigned x = s_bits[w]; x; x &= x - 1, at++) a.new_free_pages[total - 1 - at] = 32 * w + __ffs(x) - 1;
+}
+
+// Tables (rows of the grid), shares, and the lists' ends behind them.  A page is
+// moved if it was in use before and is free now; where to, `state` says.
+__global__ __launch_bounds__(256) void compact_bits_apply_kernel(const CompactArgs a) {
+    auto has = [](const unsigned* set, unsigned p) { return (set[p >> 5] >> (p & 31)) & 1; };
+    const int moves = *a.moved;
+    if (blockIdx.x >= static_cast<unsigned>(a.B)) {
+        const unsigned groups = (gridDim.x - a.B) * gridDim.y;
+        const unsigned me = ((blockIdx.x - a.B) * gridDim.y + blockIdx.y) * 256 + threadIdx.x;
+        for (unsigned i = me + moves; i < static_cast<unsigned>(a.max_moves); i += groups * 256) a.copy_src[i] = a.copy_dst[i] = -1;
+        if (!a.shares) return;
+        for (unsigned p = me; p < static_cast<unsigned>(a.num_pages); p += groups * 256) {
+            const bool was = has(a.before, p), is = has(a.after, p);
+            if (!was && is) {  // moved: its number goes along
+                a.new_shares[a.state[p]] = a.shares[p];
+                a.new_shares[p] = 0;
+            } else if (was == is) {  // (a page moved to gets its number from where it came)
+                a.new_shares[p] = is ? 0 : a.shares[p];
+            }
+        }
+        return;
+    }
+    const int b = blockIdx.x;
+    const int pages = pages_of(min(max(a.lengths[b], 0), a.cap), a.page);
+    const int32_t* row = a.table + static_cast<size_t>(b) * a.max_pages;
+    int32_t* out = a.new_table + static_cast<size_t>(b) * a.max_pages;
+    for (int j = blockIdx.y * 256 + threadIdx.x; j < pages; j += gridDim.y * 256) {
+        int id = row[j];
+        if (id >= 0 && id < a.num_pages && !has(a.before, id) && has(a.after, id)) id = a.state[id];
+        out[j] = id;
+    }
+}
+
+__global__ __launch_bounds__(256) void compact_bits_state_kernel(const CompactArgs a) {
+    const int moves = *a.moved;
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < moves; i += gridDim.x * 256) a.state[a.copy_src[i]] = a.copy_dst[i];
+}
+
 __global__ __launch_bounds__(256) void compact_table_kernel(const CompactArgs a) {
     const int b = blockIdx.x;
     const int pages = pages_of(min(max(a.lengths[b], 0), a.cap), a.page);
@@ -320,8 +443,6 @@ __global__ __launch_bounds__(256) void compact_shares_kernel(const CompactArgs a
                 a.new_shares[p] = s == kFree ? 0 : a.shares[p];
             }
         }
-        a.state[p] = 0;
-        a.taken[p] = 0;
     }
 }
 
@@ -345,32 +466,67 @@ void fork_place(ForkArgs& a, void* workspace) {
 }
 
 hipError_t launch_page_fork(const ForkArgs& a, hipStream_t stream) {
-    const dim3 rows(static_cast<unsigned>(a.B), blocks(a.max_pages, 256, 64));
-    hipLaunchKernelGGL(fork_count_kernel, rows, dim3(256), 0, stream, a);
+    const unsigned along = blocks(a.max_pages, 256, 64);
+    const unsigned pages = blocks(blocks(a.num_pages, 256, 4096), static_cast<int>(along), 4096);
+    hipLaunchKernelGGL(fork_count_kernel, dim3(static_cast<unsigned>(a.B), along), dim3(256), 0, stream, a);
     hipLaunchKernelGGL(fork_decide_kernel, dim3(1), dim3(kThreads), 0, stream, a);
-    hipLaunchKernelGGL(fork_write_kernel, rows, dim3(256), 0, stream, a);
-    hipLaunchKernelGGL(fork_lengths_kernel, dim3(blocks(a.B, 256, 1 << 20)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(fork_write_kernel, dim3(static_cast<unsigned>(a.B) + pages, along), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
+
+namespace {
+template <class T>
+hipError_t launch_copy(CopyArgs a, hipStream_t stream) {
+    a.pieces = 0;
+    for (int k = 0; k < CopyArgs::kArrays; k++) {
+        a.begin[k] = a.pieces;
+        if (a.base[k]) a.pieces += a.bytes[k] / sizeof(T);
+    }
+    a.pairs = make_fastdiv(static_cast<uint32_t>(a.n));
+    const dim3 grid(static_cast<unsigned>(a.n) * a.layers, blocks(static_cast<long long>(a.pieces), 256 * kCopyLoads, 1024));
+    hipLaunchKernelGGL((page_copy_kernel<T>), grid, dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
+}  // namespace
 
 hipError_t launch_page_copy(const CopyArgs& a, hipStream_t stream) {
     if (a.n == 0) return hipSuccess;
-    hipLaunchKernelGGL(page_copy_kernel, dim3(static_cast<unsigned>(a.n), static_cast<unsigned>(a.layers)), dim3(256), 0,
-                       stream, a);
-    return hipGetLastError();
+    size_t all = 0;
+    for (int k = 0; k < CopyArgs::kArrays; k++)
+        if (a.base[k]) all |= reinterpret_cast<uintptr_t>(a.base[k]) | a.bytes[k];
+    if (all % 16 == 0) return launch_copy<int4>(a, stream);
+    if (all % 4 == 0) return launch_copy<int>(a, stream);
+    return launch_copy<char>(a, stream);
 }
 
-size_t compact_workspace(const CompactArgs& a) { return sizeof(int) * 2 * static_cast<size_t>(a.num_pages); }
+// Bitmaps before and after, and where each page goes; or the larger pools' two arrays.
+size_t compact_workspace(const CompactArgs& a) {
+    const size_t P = static_cast<size_t>(a.num_pages);
+    return sizeof(int) * (a.num_pages <= kBitPages ? P + 2 * ((P + 31) / 32) : 2 * P);
+}
 void compact_place(CompactArgs& a, void* workspace) {
     a.state = static_cast<int*>(workspace);
     a.taken = a.state + a.num_pages;
+    a.before = reinterpret_cast<unsigned*>(a.taken);
+    a.after = a.before + (a.num_pages + 31) / 32;
 }
 
 hipError_t launch_page_compact(const CompactArgs& a, hipStream_t stream) {
+    const unsigned along = blocks(a.max_pages, 256, 64);
+    if (a.num_pages <= kBitPages) {
+        const unsigned pages = blocks(blocks(max(a.num_pages, a.max_moves), 256, 4096), static_cast<int>(along), 4096);
+        const size_t lds = sizeof(int) * ((a.num_pages + 31) / 32);
+        hipLaunchKernelGGL(compact_bits_kernel, dim3(1), dim3(kThreads), lds, stream, a);
+        hipLaunchKernelGGL(compact_bits_state_kernel, dim3(blocks(min(a.num_pages, a.max_moves), 256, 256)), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(compact_bits_apply_kernel, dim3(static_cast<unsigned>(a.B) + pages, along), dim3(256), 0, stream, a);
+        return hipGetLastError();
+    }
+    // (as the workspace may hold anything)
+    const hipError_t err = launch_fill_zero(a.state, compact_workspace(a), stream);
+    if (err != hipSuccess) return err;
     hipLaunchKernelGGL(compact_mark_kernel, dim3(blocks(max(a.num_pages, a.max_moves), 256, 1024)), dim3(256), 0, stream, a);
     hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(kThreads), 0, stream, a);
-    hipLaunchKernelGGL(compact_table_kernel, dim3(static_cast<unsigned>(a.B), blocks(a.max_pages, 256, 64)), dim3(256), 0,
-                       stream, a);
+    hipLaunchKernelGGL(compact_table_kernel, dim3(static_cast<unsigned>(a.B), along), dim3(256), 0, stream, a);
     hipLaunchKernelGGL(compact_shares_kernel, dim3(blocks(a.num_pages, 256, 1024)), dim3(256), 0, stream, a);
     return hipGetLastError();
 }

@@ -42,6 +42,9 @@ struct CopyArgs {
     static constexpr int kArrays = 6;
     char* base[kArrays];     // K, V, their scales, bounds and theirs (or null)
     size_t bytes[kArrays];   // of a page
+    size_t begin[kArrays];   // first piece of each, of a page's in all arrays
+    size_t pieces;
+    FastDiv pairs;           // division by n
 };
 hipError_t launch_page_copy(const CopyArgs& a, hipStream_t stream);
 
@@ -60,7 +63,11 @@ struct CompactArgs {
     int B, max_pages, num_pages, max_moves;
     int cap;
     FastDiv page;
-    // Workspace, all zero between calls.
+    // Workspace of pools of up to 2^18 pages: free pages before and after as bits,
+    // and where those go that move; nothing of it is read before it is written.
+    unsigned* before;
+    unsigned* after;
+    // Of larger ones, cleared at the start.
     int* state;  // [num_pages] -1: free, 0: in use, otherwise where the page moves to, + 1
     int* taken;  // [num_pages] 1: a free page that another moves to
 };

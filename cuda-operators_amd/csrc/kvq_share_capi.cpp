@@ -185,6 +185,7 @@ hipError_t kvq_page_copy_launch(const kvq_page_copy_params* p, hipStream_t strea
     if (!p || p->copies < 0 || p->layers < 1 || p->layers > 65535 || !heads_ok(p->num_kv_heads, p->head_dim) ||
         !slots_ok(p->page_size, p->num_pages) || (p->bounds == nullptr) != (p->bound_scale == nullptr))
         return hipErrorInvalidValue;
+    if (static_cast<long long>(p->copies) * p->layers >= 1LL << 24) return hipErrorInvalidValue;  // workgroups along x
     if (!p->src || !p->dst || !p->k_pages || !p->v_pages || !p->k_scale_pages || !p->v_scale_pages)
         return hipErrorInvalidValue;
     kvq::CopyArgs a{};

@@ -650,8 +650,8 @@ hipError_t kvq_page_fork_launch(const kvq_page_fork_params* p, void* workspace, 
                                 hipStream_t stream);
 
 typedef struct kvq_page_copy_params {
-    int copies;               /* n >= 0 pairs */
-    int layers;               /* pools of the same shape one behind the other, >= 1 */
+    int copies;               /* n >= 0 pairs; n * layers < 2^24 */
+    int layers;               /* pools of the same shape one behind the other, 1 to 65535 */
     int num_kv_heads, head_dim;
     int page_size, num_pages; /* of one layer's pool; num_pages * page_size <= INT_MAX */
     const int32_t* src;       /* device [n] */
@@ -697,8 +697,8 @@ typedef struct kvq_page_compact_params {
  * kvq_page_copy_launch before anything is written or read.  A holder that is no
  * table row learns the new numbers from copy_src and copy_dst.  Entries behind the
  * ends of rows and of the stack are left as they were.
- * Workspace: kvq_page_compact_workspace_size bytes, zero-filled once and left
- * ready.  Calls on one pool must be ordered. */
+ * Workspace: kvq_page_compact_workspace_size bytes of any contents.  Calls on one
+ * pool must be ordered. */
 size_t kvq_page_compact_workspace_size(const kvq_page_compact_params* p);
 hipError_t kvq_page_compact_launch(const kvq_page_compact_params* p, void* workspace, size_t workspace_bytes,
                                    hipStream_t stream);

@@ -113,6 +113,7 @@ hipError_t launch_mfma(const ChunkArgs& a, unsigned items, hipStream_t stream) {
 int chunk_dim(int d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : d <= 192 ? 192 : 256; }
 
 constexpr size_t kChunkCounters = 256 * 1024;
+constexpr long long kChunkMaxUnits = 1 << 22;  // workgroups of 512 threads along x (2^32 threads are not launched)
 
 }  // namespace
 
@@ -126,6 +127,8 @@ ChunkPlan chunk_plan(const ChunkArgs& a, bool vec_ok) {
     p.tile_tokens = p.rows / a.G;
     const long long tiles = std::min<long long>(a.T, a.T / p.tile_tokens + a.B);
     const long long units = tiles * a.Hkv;
+    if (units > kChunkMaxUnits) p.mfma = false;
+    if (!p.mfma) return ChunkPlan{};
     const int blocks = (a.max_len + kChunkKeys - 1) / kChunkKeys;
     p.max_tiles = static_cast<int>(tiles);
     p.slots = 256;  // a workgroup a CU

@@ -1064,13 +1064,17 @@ def page_copy(copy_src, copy_dst, k_pages, v_pages, k_scale_pages, v_scale_pages
 
     A pool is [num_pages, Hkv, page_size, d], or [layers, num_pages, ...] for all layers at once (scales and bounds
     alike)."""
-    if k_pages.dim() not in (4, 5):
+    shape = k_pages.shape
+    if len(shape) not in (4, 5):
         raise ValueError("k_pages: want [num_pages, Hkv, page_size, d] or [layers, num_pages, Hkv, page_size, d]")
-    shape = tuple(k_pages.shape)
     *lead, Hkv, page, d = shape
     scales = shape[:-1]
-    _needs((k_pages, _I8, shape, "k_pages"), (v_pages, _I8, shape, "v_pages"),
-           (k_scale_pages, _F32, scales, "k_scale_pages"), (v_scale_pages, _F32, scales, "v_scale_pages"))
+    if not (k_pages.dtype is _I8 and v_pages.dtype is _I8 and k_scale_pages.dtype is _F32 and v_scale_pages.dtype is _F32
+            and v_pages.shape == shape and k_scale_pages.shape == scales and v_scale_pages.shape == scales
+            and k_pages.is_contiguous() and v_pages.is_contiguous() and k_scale_pages.is_contiguous()
+            and v_scale_pages.is_contiguous() and k_pages.is_cuda):  # (as _check_pool)
+        _needs((k_pages, _I8, shape, "k_pages"), (v_pages, _I8, shape, "v_pages"),
+               (k_scale_pages, _F32, scales, "k_scale_pages"), (v_scale_pages, _F32, scales, "v_scale_pages"))
     if (bounds is None) != (bound_scale is None):
         raise ValueError("bounds and bound_scale must be given together")
     if bounds is not None:
@@ -1081,7 +1085,9 @@ def page_copy(copy_src, copy_dst, k_pages, v_pages, k_scale_pages, v_scale_pages
     index = _one_device(*tensors)
     if n == 0:
         return
-    p = PageCopyParams(n, lead[0] if len(lead) == 2 else 1, Hkv, d, page, lead[-1], *(_ptr(t) for t in tensors))
+    p = PageCopyParams(n, lead[0] if len(lead) == 2 else 1, Hkv, d, page, lead[-1], copy_src.data_ptr(), copy_dst.data_ptr(),
+                       k_pages.data_ptr(), v_pages.data_ptr(), k_scale_pages.data_ptr(), v_scale_pages.data_ptr(),
+                       _ptr(bounds), _ptr(bound_scale))
     _call(lib().kvq_page_copy_launch, "kvq_page_copy_launch", (ctypes.byref(p),), index, stream, tensors)
 
 

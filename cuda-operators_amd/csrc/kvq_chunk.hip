@@ -132,7 +132,7 @@ ChunkPlan chunk_plan(const ChunkArgs& a, bool vec_ok) {
     const int blocks = (a.max_len + kChunkKeys - 1) / kChunkKeys;
     p.max_tiles = static_cast<int>(tiles);
     p.slots = 256;  // a workgroup a CU
-    p.max_splits = units < p.slots && a.B <= waves * kWave ? std::min(p.slots, (blocks + 3) / 4) : 1;
+    p.max_splits = units < p.slots && a.B <= waves * kWave ? std::min(p.slots, (blocks + 1) / 2) : 1;
     p.items = static_cast<unsigned>(p.max_splits > 1 ? std::max<long long>(units, std::min<long long>(p.slots, units * p.max_splits)) : units);
     p.records = p.max_splits > 1 ? p.items : 0;
     if (p.records) p.bytes = kChunkCounters + p.records * p.rows * (p.D + 2) * sizeof(float);

@@ -434,16 +434,6 @@ chunk_mfma(const ChunkArgs a) {
         x.ks = in ? a.ks[mine] : 0.0f;
         x.vs = in ? a.vs[mine] : 0.0f;
     };
-    // The first block is on its way while q is fetched, where registers allow.
-    constexpr bool kEarly = LIMBS == 1 && D <= 192;
-    Block cur;
-    int next_id = 0;
-    auto load_first = [&]() __attribute__((always_inline)) {
-        const int id = id_of(wave);
-        next_id = id_of(wave + W);
-        load(cur, wave, id);
-    };
-    if (kEarly && narrow && wave < blocks) load_first();
 
     // q^T operands: lane has dims chunk_dim_of(n, h) + [0, 8) of its row, scaled to 2^15.
     h16x8 q[LIMBS][NS];
@@ -513,7 +503,7 @@ chunk_mfma(const ChunkArgs a) {
     // reads, 8 dims of K by one.
     auto matrix = [&](auto do_pv, auto do_qk, int pv, int qk) {
         constexpr int kPv = decltype(do_pv)::value ? 4 * NB : 0, kQk = decltype(do_qk)::value ? 2 * NS : 0;
-        constexpr int kAll = kPv + kQk, kAhead = LIMBS == 1 ? 6 : 4;
+        constexpr int kAll = kPv + kQk, kAhead = LIMBS == 1 ? 5 : 4;
         const _Float16* kp = s_k(qk) + c32 * KS;
         const _Float16* vp = s_v(pv) + (4 * h + (c16 >> 2)) * VS + 16 * ((lane >> 4) & 1) + 4 * (c16 & 3);
         auto read = [&](int n) {
@@ -749,7 +739,9 @@ chunk_mfma(const ChunkArgs a) {
         };
         __syncthreads();
         if (wave < blocks) {
-            if (!kEarly) load_first();
+            Block cur;
+            load(cur, wave, id_of(wave));
+            int next_id = id_of(wave + W);
             for (int b = wave; b < blocks; b += W) {
                 Block next;
                 load(next, b + W, next_id);  // (past the end: the last key's again)

@@ -113,7 +113,8 @@ def test_chunk_workspace_sizes():
     assert size(tokens=0) == 0
     # Many tiles, short sequences and the generic kernel split nothing.
     assert size(batch=300, tokens=300, num_q_heads=16, num_kv_heads=16) == 0
-    assert size(max_pages_per_seq=16) == 0  # 256 tokens
+    assert size(max_pages_per_seq=8) == 0   # 128 tokens: a split has two key tiles of 64 at least
+    assert size(max_pages_per_seq=16) > 0   # 256 tokens
     assert size(head_dim=20, batch=1, max_pages_per_seq=1 << 16) == 0
     # At most 256 records of 256 rows (128 from d = 256 on) and the counters.
     for d, rows, padded in ((64, 256, 64), (80, 256, 96), (128, 256, 128), (192, 128, 192), (256, 128, 256)):

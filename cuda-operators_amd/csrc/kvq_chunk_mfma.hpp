@@ -1,4 +1,31 @@
 // kvq_chunk_mfma.hpp -- chunk attention on gfx950's f16 matrix cores.
+//
+// A query row (one head of one new token) over the keys j that it sees, of int8
+// codes k_j, v_j with scales ks_j, vs_j, one of each a key and kv head:
+//   s_j = ks_j (q . k_j) scale log2(e),  p_j = 2^(s_j - m),
+//   out = sum p_j vs_j v_j / sum p_j,
+// in one pass with a running m and sum.  int8 codes are exact in f16, so both
+// products run on the f16 matrix cores (32x32x16): S^T = K q^T, O^T = V^T P^T, whose
+// results both have a row of q per lane, so m, the sum and the rescaling of O
+// need no exchange.  ks multiplies S, a key per register, by a DPP broadcast; vs goes
+// into V's f16 tile (bf16), or into p (fp32).  fp32 takes q and p as two f16 limbs.
+//
+// Rows of a kv head's G query heads and of neighbouring tokens share a tile, so
+// codes are read once per waves * 32 rows.  What bounds it then, at 2048 new tokens of
+// 32 query heads over 8 kv heads, d = 128, behind 30,720 others (1065 GFLOP, 1197 us, 890
+// TFLOP/s; a bf16 8192^3 library product runs 1208): matrix cores are busy 38 % of the
+// cycles, and the vector ALU's share (softmax, codes to f16: 309 M wave instructions)
+// takes about as long, so the two have to overlap:
+// * Four waves of 32 rows, one a SIMD, one after the other in program order: 1398 us.
+// * Eight waves in two phases, each SIMD's pair in opposite ones, a barrier after
+//   each phase: 1197 us.  The matrix phase by itself takes 556 us, softmax 390, the
+//   two without conversion and loads 882.
+// * Tiles of 64 keys: V, K and the rows' state fit two waves a SIMD (256 registers).
+// * Operands are read kAhead MFMAs early (4 and 8 for bf16: within 2 %).  Priorities
+//   (s_setprio) gain nothing; reading scales before the matrix phase 1269 against 1211 us.
+// Tiles of up to 32 rows take the narrow path, which is bound by bytes: 64 single
+// tokens over 512 to 8192 keys 158 us (3.7 TB/s; by the wide path 403), one over
+// 131,072 keys 61 us (4.5 TB/s; a copy moves 5.08).
 #pragma once
 
 #include <limits.h>
@@ -20,6 +47,8 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 // Waves of a workgroup, 32 query rows each.  Eight run in two phases a tile, which
 // takes two waves a SIMD; where the state needs a SIMD's registers, four run.
+// (64 sequences over 512 to 8192 keys, four with up to 511 new tokens, the others
+// with one, bf16, d = 128: eight 446 us, four 798.)
 constexpr int chunk_waves(int D, int limbs) { return D <= (limbs == 1 ? 128 : 96) ? 8 : 4; }
 constexpr int kChunkCoherent = 16;  // buffer cache policy sc1: device-coherent
 constexpr float kWeightTop = 15.0f;   // log2 of the largest f16 weight that is let grow,
@@ -75,6 +104,9 @@ __device__ __forceinline__ void chunk_counts(const ChunkArgs& a, const ChunkSeq&
 // are a.slots workgroups or more, each is one item.  Otherwise keys are split into
 // chunks of the fewest blocks (in steps) with which the items are at most a.slots;
 // all tiles of a sequence have the same number of splits.
+// One workgroup a CU fits (LDS), so the slots are the 256 CUs: with 512, 512 tokens
+// over 8192 keys take 168 us against 125.  A split is at least two blocks: with 4 and 8,
+// five tokens over 1001 keys take 18.2 and 20.2 us against 17.2.
 struct ChunkPlanLds {
     int part[8], best[8];
     int tiles[512], blocks[512];

@@ -38,7 +38,9 @@ __device__ __forceinline__ int group_scan(int v, int& total, int (&part)[kWaves]
 // a page of held > 1 takes a copy unless it is the first of holders that all end
 // inside it.  Three launches: entries are counted by atomics on the page (sums
 // and a max of integers: any order gives the same), one workgroup decides, in
-// page and row order by prefix sums, and the rows are written.
+// page and row order by prefix sums, and the rows are written.  Bound by latency: 16 rows
+// on pages of 64 tokens take 11.5 us a call, 256 of up to 4096 tokens on pages of 16
+// 17.6; the kernels are 2.3 to 6.1 and up to 10.5 us each.
 
 struct ForkRow {
     int parent;  // -1: none
@@ -209,7 +211,9 @@ __global__ __launch_bounds__(256) void fork_write_kernel(const ForkArgs a) {
 // ---------------------------------------------------------------------------
 // A pair's arrays in one layer are laid end to end in pieces of 16 bytes (or 4, or
 // 1, where an array's place or page size is not a multiple); a workgroup takes
-// kCopyPieces of a thread's at a time, whose loads go out together.
+// kCopyPieces of a thread's at a time, whose loads go out together.  Bound by HBM: 48
+// pages of 64 tokens in 32 layers of 8 heads, d = 128 (415 MB read and written), 74.6 us
+// a call, 67.5 the kernel; a large copy at 5.08 TB/s would take 82.
 constexpr int kCopyLoads = 4;
 
 template <class T>
@@ -247,6 +251,11 @@ __global__ __launch_bounds__(256) void page_copy_kernel(const CopyArgs a) {
 // ---------------------------------------------------------------------------
 // Compaction.
 // ---------------------------------------------------------------------------
+// Moves are decided by one workgroup: the i-th free page from below takes the i-th
+// page in use from above, as long as it lies lower, and both lists are prefix sums.
+// Bound by the latency of that workgroup's passes: 16 rows of up to 2048 tokens on pages
+// of 64 take 11.3 us a call, 256 of up to 4096 on pages of 16 (50,000 pages) 32, nearly
+// all of it this launch.
 // A page's state: kFree, 0 in use, or where it moves to, + 1.
 constexpr int kFree = -1;
 

@@ -254,8 +254,8 @@ __global__ __launch_bounds__(256) void page_copy_kernel(const CopyArgs a) {
 // Moves are decided by one workgroup: the i-th free page from below takes the i-th
 // page in use from above, as long as it lies lower, and both lists are prefix sums.
 // Bound by the latency of that workgroup's passes: 16 rows of up to 2048 tokens on pages
-// of 64 take 11.3 us a call, 256 of up to 4096 on pages of 16 (50,000 pages) 32, nearly
-// all of it this launch.
+// of 64 take 11.3 us a call, 256 of up to 4096 on pages of 16 (50,000 pages) 22.6 (32.9
+// with the stack written by that workgroup and one load at a time).
 // A page's state: kFree, 0 in use, or where it moves to, + 1.
 constexpr int kFree = -1;
 
@@ -336,9 +336,14 @@ __global__ __launch_bounds__(kThreads) void compact_bits_kernel(const CompactArg
     for (int w = t; w < words; w += kThreads) s_bits[w] = 0;
     __syncthreads();
     const int F = min(max(*a.free_count, 0), P);
-    for (int i = t; i < F; i += kThreads) {
-        const int p = a.free_pages[i];
-        if (p >= 0 && p < P) atomicOr(&s_bits[p >> 5], 1u << (p & 31));
+    constexpr int kLoads = 8;  // on their way together
+    for (int i = t; i < F; i += kLoads * kThreads) {
+        int p[kLoads];
+#pragma unroll
+        for (int j = 0; j < kLoads; j++) p[j] = i + j * kThreads < F ? a.free_pages[i + j * kThreads] : -1;
+#pragma unroll
+        for (int j = 0; j < kLoads; j++)
+            if (p[j] >= 0 && p[j] < P) atomicOr(&s_bits[p[j] >> 5], 1u << (p[j] & 31));
     }
     __syncthreads();
     auto valid = [&](int w) { return w == words - 1 && (P & 31) ? (1u << (P & 31)) - 1 : ~0u; };
@@ -381,15 +386,17 @@ __global__ __launch_bounds__(kThreads) void compact_bits_kernel(const CompactArg
         a.after[w] = now;
     }
     if (t == 0) *a.moved = moves;
-    // The stack afterwards, descending.
+    // Where the pages go in the stack afterwards, descending.
     count = 0;
     for (int w = w0; w < w1; w++) count += __popc(s_bits[w]);
     int at = group_scan(count, total, s_part) - count;  // free pages before this thread's
-    for (int w = w0; w < w1; w++)
-        for (unsigned x = s_bits[w]; x; x &= x - 1, at++) a.new_free_pages[total - 1 - at] = 32 * w + __ffs(x) - 1;
+    for (int w = w0; w < w1; w++) {
+        a.place[w] = total - 1 - at;
+        at += __popc(s_bits[w]);
+    }
 }
 
-// Tables (rows of the grid), shares, and the lists' ends behind them.  A page is
+// Tables (rows of the grid), shares, the stack, and the lists' ends behind them.  A page is
 // moved if it was in use before and is free now; where to, `state` says.
 __global__ __launch_bounds__(256) void compact_bits_apply_kernel(const CompactArgs a) {
     auto has = [](const unsigned* set, unsigned p) { return (set[p >> 5] >> (p & 31)) & 1; };
@@ -398,9 +405,10 @@ __global__ __launch_bounds__(256) void compact_bits_apply_kernel(const CompactAr
         const unsigned groups = (gridDim.x - a.B) * gridDim.y;
         const unsigned me = ((blockIdx.x - a.B) * gridDim.y + blockIdx.y) * 256 + threadIdx.x;
         for (unsigned i = me + moves; i < static_cast<unsigned>(a.max_moves); i += groups * 256) a.copy_src[i] = a.copy_dst[i] = -1;
-        if (!a.shares) return;
         for (unsigned p = me; p < static_cast<unsigned>(a.num_pages); p += groups * 256) {
             const bool was = has(a.before, p), is = has(a.after, p);
+            if (is) a.new_free_pages[a.place[p >> 5] - __popc(a.after[p >> 5] & ((1u << (p & 31)) - 1))] = static_cast<int>(p);
+            if (!a.shares) continue;
             if (!was && is) {  // moved: its number goes along
                 a.new_shares[a.state[p]] = a.shares[p];
                 a.new_shares[p] = 0;
@@ -511,13 +519,14 @@ hipError_t launch_page_copy(const CopyArgs& a, hipStream_t stream) {
 // Bitmaps before and after, and where each page goes; or the larger pools' two arrays.
 size_t compact_workspace(const CompactArgs& a) {
     const size_t P = static_cast<size_t>(a.num_pages);
-    return sizeof(int) * (a.num_pages <= kBitPages ? P + 2 * ((P + 31) / 32) : 2 * P);
+    return sizeof(int) * (a.num_pages <= kBitPages ? P + 3 * ((P + 31) / 32) : 2 * P);
 }
 void compact_place(CompactArgs& a, void* workspace) {
     a.state = static_cast<int*>(workspace);
     a.taken = a.state + a.num_pages;
     a.before = reinterpret_cast<unsigned*>(a.taken);
     a.after = a.before + (a.num_pages + 31) / 32;
+    a.place = reinterpret_cast<int*>(a.after + (a.num_pages + 31) / 32);
 }
 
 hipError_t launch_page_compact(const CompactArgs& a, hipStream_t stream) {

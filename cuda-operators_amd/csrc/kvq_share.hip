@@ -253,9 +253,9 @@ __global__ __launch_bounds__(256) void page_copy_kernel(const CopyArgs a) {
 // ---------------------------------------------------------------------------
 // Moves are decided by one workgroup: the i-th free page from below takes the i-th
 // page in use from above, as long as it lies lower, and both lists are prefix sums.
-// Bound by the latency of that workgroup's passes: 16 rows of up to 2048 tokens on pages
-// of 64 take 11.3 us a call, 256 of up to 4096 on pages of 16 (50,000 pages) 22.6 (32.9
-// with the stack written by that workgroup and one load at a time).
+// Bound by launches and latency: 16 rows of up to 2048 tokens on pages of 64 take 9.7 us a
+// call, 256 of up to 4096 on pages of 16 (50,000 pages) 12.4.  With all lists written by
+// the one workgroup that scans, and one load at a time, the latter took 32.9.
 // A page's state: kFree, 0 in use, or where it moves to, + 1.
 constexpr int kFree = -1;
 
@@ -324,7 +324,8 @@ __global__ __launch_bounds__(kThreads) void compact_plan_kernel(const CompactArg
 
 // The same with the free pages as bits in LDS, for pools of up to kBitPages: one
 // scan each over the words instead of one over the pages.  Both sets of free pages,
-// before and after the moves, are left in the workspace for the launch behind this.
+// before and after the moves, are left in the workspace with counts for each word, from
+// which the launches behind this one write the lists, a page a thread.
 constexpr int kBitPages = 1 << 18;  // 32 KB of LDS
 
 __global__ __launch_bounds__(kThreads) void compact_bits_kernel(const CompactArgs a) {
@@ -365,25 +366,22 @@ __global__ __launch_bounds__(kThreads) void compact_bits_kernel(const CompactArg
     }
     int all_holes, all_highs;
     int hole = group_scan(holes, all_holes, s_part) - holes;
-    int high = group_scan(highs, all_highs, s_part);  // the lowest of this thread's is the high-th from the top
-    high = all_highs - (high - highs) - 1;
+    int high = group_scan(highs, all_highs, s_part);
+    high = all_highs - (high - highs);  // pages that could move, from this thread's first word on
     const int moves = min(all_holes, a.max_moves);
     for (int w = w0; w < w1; w++) {
-        unsigned x = s_bits[w] & below(w), y = ~s_bits[w] & ~below(w) & valid(w), now = s_bits[w];
-        for (; x; x &= x - 1, hole++) {
-            const int bit = __ffs(x) - 1;
-            if (hole >= moves) break;
-            a.copy_dst[hole] = 32 * w + bit;
-            now &= ~(1u << bit);
-        }
-        for (; y; y &= y - 1, high--) {
-            const int bit = __ffs(y) - 1;
-            if (high >= moves) continue;
-            a.copy_src[high] = 32 * w + bit;
-            now |= 1u << bit;
-        }
-        s_bits[w] = now;
-        a.after[w] = now;
+        // The lowest of the free pages are moved to, the highest of those in use moved;
+        // in one word each some may stay.
+        unsigned x = s_bits[w] & below(w), y = ~s_bits[w] & ~below(w) & valid(w);
+        const int nx = static_cast<int>(__popc(x)), ny = static_cast<int>(__popc(y));  // (__popc is unsigned)
+        a.hole[w] = hole;
+        hole += nx;
+        for (int i = min(hole - moves, nx); i > 0; i--) x &= ~(1u << (31 - __clz(x)));
+        high -= ny;
+        a.high[w] = high;
+        for (int i = min(high + ny - moves, ny); i > 0; i--) y &= y - 1;
+        s_bits[w] = (s_bits[w] & ~x) | y;
+        a.after[w] = s_bits[w];
     }
     if (t == 0) *a.moved = moves;
     // Where the pages go in the stack afterwards, descending.
@@ -397,9 +395,14 @@ __global__ __launch_bounds__(kThreads) void compact_bits_kernel(const CompactArg
 }
 
 // Tables (rows of the grid), shares, the stack, and the lists' ends behind them.  A page is
-// moved if it was in use before and is free now; where to, `state` says.
+// moved if it was in use before and is free now, to the page of the same rank among
+// those that were free and are in use now.
+__device__ __forceinline__ bool has(const unsigned* set, unsigned p) { return (set[p >> 5] >> (p & 31)) & 1; }
+__device__ __forceinline__ int move_of(const CompactArgs& a, unsigned p) {  // of a page that moves, from the highest
+    const unsigned w = p >> 5;
+    return a.high[w] + __popc(~a.before[w] & a.after[w] & ~((2u << (p & 31)) - 1));
+}
 __global__ __launch_bounds__(256) void compact_bits_apply_kernel(const CompactArgs a) {
-    auto has = [](const unsigned* set, unsigned p) { return (set[p >> 5] >> (p & 31)) & 1; };
     const int moves = *a.moved;
     if (blockIdx.x >= static_cast<unsigned>(a.B)) {
         const unsigned groups = (gridDim.x - a.B) * gridDim.y;
@@ -410,7 +413,7 @@ __global__ __launch_bounds__(256) void compact_bits_apply_kernel(const CompactAr
             if (is) a.new_free_pages[a.place[p >> 5] - __popc(a.after[p >> 5] & ((1u << (p & 31)) - 1))] = static_cast<int>(p);
             if (!a.shares) continue;
             if (!was && is) {  // moved: its number goes along
-                a.new_shares[a.state[p]] = a.shares[p];
+                a.new_shares[a.copy_dst[move_of(a, p)]] = a.shares[p];
                 a.new_shares[p] = 0;
             } else if (was == is) {  // (a page moved to gets its number from where it came)
                 a.new_shares[p] = is ? 0 : a.shares[p];
@@ -424,14 +427,18 @@ __global__ __launch_bounds__(256) void compact_bits_apply_kernel(const CompactAr
     int32_t* out = a.new_table + static_cast<size_t>(b) * a.max_pages;
     for (int j = blockIdx.y * 256 + threadIdx.x; j < pages; j += gridDim.y * 256) {
         int id = row[j];
-        if (id >= 0 && id < a.num_pages && !has(a.before, id) && has(a.after, id)) id = a.state[id];
+        if (id >= 0 && id < a.num_pages && !has(a.before, id) && has(a.after, id)) id = a.copy_dst[move_of(a, id)];
         out[j] = id;
     }
 }
 
-__global__ __launch_bounds__(256) void compact_bits_state_kernel(const CompactArgs a) {
-    const int moves = *a.moved;
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < moves; i += gridDim.x * 256) a.state[a.copy_src[i]] = a.copy_dst[i];
+__global__ __launch_bounds__(256) void compact_bits_moves_kernel(const CompactArgs a) {
+    for (unsigned p = blockIdx.x * 256 + threadIdx.x; p < static_cast<unsigned>(a.num_pages); p += gridDim.x * 256) {
+        const bool was = has(a.before, p), is = has(a.after, p);
+        if (!was && is) a.copy_src[move_of(a, p)] = static_cast<int>(p);
+        const unsigned w = p >> 5;
+        if (was && !is) a.copy_dst[a.hole[w] + __popc(a.before[w] & ~a.after[w] & ((1u << (p & 31)) - 1))] = static_cast<int>(p);
+    }
 }
 
 __global__ __launch_bounds__(256) void compact_table_kernel(const CompactArgs a) {
@@ -516,17 +523,19 @@ hipError_t launch_page_copy(const CopyArgs& a, hipStream_t stream) {
     return launch_copy<char>(a, stream);
 }
 
-// Bitmaps before and after, and where each page goes; or the larger pools' two arrays.
+// Bitmaps before and after and three counts a word; or the larger pools' two arrays.
 size_t compact_workspace(const CompactArgs& a) {
     const size_t P = static_cast<size_t>(a.num_pages);
-    return sizeof(int) * (a.num_pages <= kBitPages ? P + 3 * ((P + 31) / 32) : 2 * P);
+    return sizeof(int) * (a.num_pages <= kBitPages ? 5 * ((P + 31) / 32) : 2 * P);
 }
 void compact_place(CompactArgs& a, void* workspace) {
     a.state = static_cast<int*>(workspace);
     a.taken = a.state + a.num_pages;
-    a.before = reinterpret_cast<unsigned*>(a.taken);
+    a.before = static_cast<unsigned*>(workspace);
     a.after = a.before + (a.num_pages + 31) / 32;
     a.place = reinterpret_cast<int*>(a.after + (a.num_pages + 31) / 32);
+    a.hole = a.place + (a.num_pages + 31) / 32;
+    a.high = a.hole + (a.num_pages + 31) / 32;
 }
 
 hipError_t launch_page_compact(const CompactArgs& a, hipStream_t stream) {
@@ -535,7 +544,7 @@ hipError_t launch_page_compact(const CompactArgs& a, hipStream_t stream) {
         const unsigned pages = blocks(blocks(max(a.num_pages, a.max_moves), 256, 4096), static_cast<int>(along), 4096);
         const size_t lds = sizeof(int) * ((a.num_pages + 31) / 32);
         hipLaunchKernelGGL(compact_bits_kernel, dim3(1), dim3(kThreads), lds, stream, a);
-        hipLaunchKernelGGL(compact_bits_state_kernel, dim3(blocks(min(a.num_pages, a.max_moves), 256, 256)), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(compact_bits_moves_kernel, dim3(blocks(a.num_pages, 256, 1024)), dim3(256), 0, stream, a);
         hipLaunchKernelGGL(compact_bits_apply_kernel, dim3(static_cast<unsigned>(a.B) + pages, along), dim3(256), 0, stream, a);
         return hipGetLastError();
     }

@@ -64,10 +64,12 @@ struct CompactArgs {
     int cap;
     FastDiv page;
     // Workspace of pools of up to 2^18 pages: free pages before and after as bits,
-    // their places in the stack, and where those go that move; nothing of it is read before it is written.
+    // and counts a word; nothing of it is read before it is written.
     unsigned* before;
     unsigned* after;
     int* place;  // [words] where a word's first free page goes in the stack
+    int* hole;   // [words] pages below the word that could be moved to
+    int* high;   // [words] pages above the word that could move
     // Of larger ones, cleared at the start.
     int* state;  // [num_pages] -1: free, 0: in use, otherwise where the page moves to, + 1
     int* taken;  // [num_pages] 1: a free page that another moves to

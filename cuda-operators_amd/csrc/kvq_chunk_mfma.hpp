@@ -209,6 +209,13 @@ __device__ inline bool chunk_locate(const ChunkArgs& a, ChunkPlanLds& s, int r, 
     return true;
 }
 
+// e with |vs| <= 2^e for all of a tile's V scales, the largest of which is top.  Of a tile
+// whose values are all zero the lowest there is: its scores shall not raise a row's m,
+// under which the weights of tokens with small scales would leave f16's range.
+__device__ __forceinline__ int scale_exponent(float top) {
+    return top > 0.0f ? min(max(__builtin_amdgcn_frexp_expf(top), -60), 60) : -60;
+}
+
 // LDS exchange within a wave.
 __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -410,7 +417,7 @@ chunk_mfma(const ChunkArgs a) {
         if (v > 0.0f) vmin = fminf(vmin, v);
         // (bits of a float >= 0 order as integers)
         const float top = __int_as_float(__builtin_amdgcn_readlane(wave_inclusive_max_nonneg(__float_as_int(v)), kWave - 1));
-        const int e = min(max(__builtin_amdgcn_frexp_expf(top), -60), 60);
+        const int e = scale_exponent(top);
         x.ks[lane] = ksr;
         const _Float16 h = static_cast<_Float16>(ldexpf(vsr, -e));
         x.vs[lane] = LIMBS == 1 ? __builtin_bit_cast(float, h16x2{h, h}) : vsr;
@@ -714,7 +721,7 @@ chunk_mfma(const ChunkArgs a) {
             vmax = fmaxf(vmax, v);
             if (v > 0.0f) vmin = fminf(vmin, v);
             const float vtop = __int_as_float(__builtin_amdgcn_readlane(wave_inclusive_max_nonneg(__float_as_int(v)), kWave - 1));
-            const float lv = static_cast<float>(min(max(__builtin_amdgcn_frexp_expf(vtop), -60), 60));
+            const float lv = static_cast<float>(scale_exponent(vtop));
             times_lanes(p, __shfl(x.ks, scale_key));
             const int t0 = k0 + blk * 32;
             if (t0 + 32 > keys_all) {

@@ -8,7 +8,7 @@
 // products run on the f16 matrix cores (32x32x16): S^T = K q^T, O^T = V^T P^T, whose
 // results both have a row of q per lane, so m, the sum and the rescaling of O
 // need no exchange.  ks multiplies S, a key per register, by a DPP broadcast; vs goes
-// into V's f16 tile (bf16), or into p (fp32).  fp32 takes q and p as two f16 limbs.
+// into V's f16 tile (bf16, but where a tile's differ too much for f16), or into p.  fp32 takes q and p as two f16 limbs.
 //
 // Rows of a kv head's G query heads and of neighbouring tokens share a tile, so
 // codes are read once per waves * 32 rows.  What bounds it then, at 2048 new tokens of
@@ -57,6 +57,9 @@ constexpr float kKsMax = 0x1p80f;     // |k scale|s above overflow as scores of 
 constexpr float kVsMax = 0x1p40f, kVsMin = 0x1p-40f;  // |v scale|s outside take fp32 weights, as does a
 template <int LIMBS>                                  // tile set whose scales differ by more than this
 constexpr float kVsRatio = LIMBS == 1 ? 0x1p18f : 0x1p14f;
+// bf16: V's scales of a tile lie within 2^14 (vs / 2^e >= 2^-14 is normal in f16), or go into
+// its weights in fp32 before those are rounded.
+constexpr int kVfBits = 14;
 
 // Dims that lane half h contracts in step n: steps 2 j and 2 j + 1 take the halves
 // of one 16-byte piece, so that a row's codes can come straight from memory.
@@ -286,8 +289,11 @@ chunk_mfma(const ChunkArgs a) {
     struct Scales {
         long long at[kChunkKeys];   // byte offsets of the pool rows
         float ks[kChunkKeys];
-        float vs[kChunkKeys];       // LIMBS == 1: two f16 of vs / 2^lv
-        float lv, unit;             // |vs| <= 2^lv; 2^-lv
+        float vs[kChunkKeys];
+        unsigned vf[LIMBS == 1 ? kChunkKeys : 1];  // V's factor in the f16 tile, twice
+        // x: |vs| <= 2^x; y: log2 of the factor that the f16 tile's V lacks, z: its inverse
+        // (0 and 1 where vs goes into the weights: w)
+        float4 v;
     };
     constexpr int kKTile = kChunkKeys * KS, kVTile = kChunkKeys * VS;
     __shared__ __align__(16) _Float16 s_buf[2 * (kKTile + kVTile)];
@@ -379,7 +385,7 @@ chunk_mfma(const ChunkArgs a) {
         for (int i = 0; i < NP; i++) {
             const int piece = i * 256 + t256;
             const int kr = piece / PPR, c = (piece - kr * PPR) * 8;
-            const h16x2 f = LIMBS == 1 ? __builtin_bit_cast(h16x2, s_scale[tile & (kSlots - 1)].vs[kr]) : bias;
+            const h16x2 f = LIMBS == 1 ? __builtin_bit_cast(h16x2, s_scale[tile & (kSlots - 1)].vf[LIMBS == 1 ? kr : 0]) : bias;
             *reinterpret_cast<h16x8*>(s_v(tile) + kr * VS + c) =
                 codes_to_f16(raw[i], [&](h16x2 x) { return LIMBS == 1 ? (x - bias) * f : x - bias; });
         }
@@ -419,12 +425,15 @@ chunk_mfma(const ChunkArgs a) {
         const float top = __int_as_float(__builtin_amdgcn_readlane(wave_inclusive_max_nonneg(__float_as_int(v)), kWave - 1));
         const int e = scale_exponent(top);
         x.ks[lane] = ksr;
-        const _Float16 h = static_cast<_Float16>(ldexpf(vsr, -e));
-        x.vs[lane] = LIMBS == 1 ? __builtin_bit_cast(float, h16x2{h, h}) : vsr;
-        if (lane == 0) {
-            x.lv = static_cast<float>(e);
-            x.unit = ldexpf(1.0f, -e);
+        x.vs[lane] = vsr;
+        // bf16: vs / 2^e goes into V's f16 tile, unless some token's would be subnormal there.
+        const bool in_weights = LIMBS == 2 || __builtin_amdgcn_ballot_w64(v > 0.0f && v < ldexpf(1.0f, e - kVfBits)) != 0;
+        if (LIMBS == 1) {
+            const _Float16 h = in_weights ? static_cast<_Float16>(1.0f) : static_cast<_Float16>(ldexpf(vsr, -e));
+            x.vf[LIMBS == 1 ? lane : 0] = __builtin_bit_cast(unsigned, h16x2{h, h});
         }
+        const float lv = static_cast<float>(e);
+        if (lane == 0) x.v = in_weights ? make_float4(lv, 0.0f, 1.0f, 1.0f) : make_float4(lv, lv, ldexpf(1.0f, -e), 0.0f);
     };
     int far_id = 0;
     if (tiles > 0 && wave == 0 && !narrow) {
@@ -599,7 +608,8 @@ chunk_mfma(const ChunkArgs a) {
         for (int i = 1; i < 32; i++) top = fmaxf(top, p[i / 16][i % 16]);
         // m is a reference that weights pass by up to 2^kWeightTop: it moves, with the
         // state, only when some row's could pass by more.
-        const float u = fmaf(top, c_row, sc.lv);
+        const float4 sv = sc.v;
+        const float u = fmaf(top, c_row, sv.x);
         if (__builtin_amdgcn_ballot_w64(u > m + kWeightTop) != 0) {
             const float un = fmaxf(u, __shfl_xor(u, 32)) - kWeightReset;
             const float mn = un > m ? un : m;
@@ -611,29 +621,33 @@ chunk_mfma(const ChunkArgs a) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[c][i] *= alpha;
         }
-        const float ms = (m == -INFINITY ? 0.0f : m) - (LIMBS == 1 ? sc.lv : 0.0f);
-        // Summed by themselves, so l rounds once a tile (2000 keys in fp32: error 2.0e-6 with a sum key by key).
-        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float ms = (m == -INFINITY ? 0.0f : m) - (LIMBS == 1 ? sv.y : 0.0f);
+        auto weights = [&](auto vs_in_weights) __attribute__((always_inline)) {
+            // Summed by themselves, so l rounds once a tile (2000 keys in fp32: error 2.0e-6 with a sum key by key).
+            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int kb = 0; kb < 2; kb++) {
+            for (int kb = 0; kb < 2; kb++) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                p[kb][i] = fast_exp2(fmaf(p[kb][i], c_row, -ms));
-                part[i % 4] += p[kb][i];
+                for (int i = 0; i < 16; i++) {
+                    p[kb][i] = fast_exp2(fmaf(p[kb][i], c_row, -ms));
+                    part[i % 4] += p[kb][i];
+                }
+                if (decltype(vs_in_weights)::value) times_lanes(p[kb], sc.vs[32 * kb + scale_at]);
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float y = p[kb][i];
+                    // One value for both limbs: contracted into one of them, the product would be
+                    // rounded once there and twice here, 2^-10 apart in one weight of some thousand.
+                    if (LIMBS == 2) asm("" : "+v"(y));
+                    const _Float16 hi = static_cast<_Float16>(y);
+                    wt[0][2 * kb + i / 8][i % 8] = hi;
+                    if (LIMBS == 2) wt[LIMBS - 1][2 * kb + i / 8][i % 8] = static_cast<_Float16>(y - static_cast<float>(hi));
+                }
             }
-            if (LIMBS == 2) times_lanes(p[kb], sc.vs[32 * kb + scale_at]);
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                float y = p[kb][i];
-                // One value for both limbs: contracted into one of them, the product would be
-                // rounded once there and twice here, 2^-10 apart in one weight of some thousand.
-                if (LIMBS == 2) asm("" : "+v"(y));
-                const _Float16 hi = static_cast<_Float16>(y);
-                wt[0][2 * kb + i / 8][i % 8] = hi;
-                if (LIMBS == 2) wt[LIMBS - 1][2 * kb + i / 8][i % 8] = static_cast<_Float16>(y - static_cast<float>(hi));
-            }
-        }
-        l = fmaf((part[0] + part[1]) + (part[2] + part[3]), LIMBS == 1 ? sc.unit : 1.0f, l);
+            l = fmaf((part[0] + part[1]) + (part[2] + part[3]), LIMBS == 1 ? sv.z : 1.0f, l);
+        };
+        if (LIMBS == 2 || __builtin_amdgcn_readfirstlane(__float_as_int(sv.w)) != 0) weights(yes);
+        else weights(no);
     };
     // Rows and scales ahead of tile i's: scales of tile i + 2 are stored, rows and
     // scales of tile i + 3 fetched into the slot of tile i - 1.

@@ -7,7 +7,7 @@ import torch
 
 import _share_ref as ref
 from _gpu import kvq
-from test_gpu_chunk import BF16, F32, attention
+from test_gpu_chunk import BF16, F32, attention, pool_at
 
 pytestmark = pytest.mark.gpu
 
@@ -60,6 +60,30 @@ def check(i, **kw):
             worst = max(worst, off.max().item())
             assert worst <= 1.0, (b, h, worst, torch.nonzero(off > 1)[0].tolist())
     return worst
+
+
+def sink(i, b, at, ratio):
+    """Token `at` of sequence b takes nearly all the weight of every row, with a V scale `ratio` of what it was."""
+    p, at = pool_at(i, b, at)
+    q = i["q"].float()
+    q[:, :, 0] = 30.0
+    i["q"] = q.to(i["q"].dtype)
+    i["k"][:, :, :, 0] = 0
+    i["k"][p, :, at] = 0
+    i["k"][p, :, at, 0] = 127
+    i["ks"][p, :, at] = 0.1
+    i["vs"][p, :, at] *= ratio
+
+
+# ---- ratios of scales -----------------------------------------------------------
+@pytest.mark.parametrize("half_steps", range(-36, -25))
+@pytest.mark.parametrize("n", [30, 3])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_the_token_with_the_weight_has_a_tiny_scale(half_steps, n, dtype):
+    for seed, d in ((0, 64), (1, 128), (2, 96)):
+        i = ref.batch(seed, [(200, n)], 4, 1, d, 16, dtype)
+        sink(i, 0, 5 + seed, 2.0 ** (half_steps / 2))
+        check(i)
 
 
 # ---- scales of zero -------------------------------------------------------------

@@ -54,12 +54,22 @@ constexpr int kChunkCoherent = 16;  // buffer cache policy sc1: device-coherent
 constexpr float kWeightTop = 15.0f;   // log2 of the largest f16 weight that is let grow,
 constexpr float kWeightReset = 12.0f; // and of what a row's weights are set to when they pass it
 constexpr float kKsMax = 0x1p80f;     // |k scale|s above overflow as scores of q scaled to 2^15
-constexpr float kVsMax = 0x1p40f, kVsMin = 0x1p-40f;  // |v scale|s outside take fp32 weights, as does a
-template <int LIMBS>                                  // tile set whose scales differ by more than this
-constexpr float kVsRatio = LIMBS == 1 ? 0x1p18f : 0x1p14f;
-// bf16: V's scales of a tile lie within 2^14 (vs / 2^e >= 2^-14 is normal in f16), or go into
-// its weights in fp32 before those are rounded.
-constexpr int kVfBits = 14;
+// |vs|s that are computed in fp32 throughout (chunk_row_f32); within them ratios do not
+// matter.  Above: the weights of other tokens would leave fp32.  Below, 2^-10 (fp32: 2^-6)
+// under the lowest exponent that m counts, f16 weights would lose bits.
+constexpr float kVsMax = 0x1p60f;
+template <int LIMBS>
+constexpr float kVsMin = LIMBS == 1 ? 0x1p-90f : 0x1p-86f;
+constexpr int kVsHigh = 60, kVsLow = -80;
+// A row's m is set so that weights times |vs| are at most 2^15 and some of them 2^12, by
+// s + (an exponent of vs): a tile's largest, unless some token's scale is 2^kSpreadBits below
+// it.  Then each token counts its own, as a weight that m overrates has fewer bits: from
+// 2^12 / 2^13 on they are enough for one f16 (off by 2^-25), from 2^12 / 2^6 for two.  In bf16's V
+// tiles vs / 2^e is normal in f16 then, with e within +-kVfRange: 2^e in a weight's sum is
+// within fp32 beside kVsHigh.
+template <int LIMBS>
+constexpr int kSpreadBits = LIMBS == 1 ? 12 : 5;
+constexpr int kVfRange = 48;
 
 // Dims that lane half h contracts in step n: steps 2 j and 2 j + 1 take the halves
 // of one 16-byte piece, so that a row's codes can come straight from memory.
@@ -87,6 +97,16 @@ __device__ __forceinline__ void times_lanes(f32x16& x, float y) {
         x[I] = times_lane<I>(x[I], y);
         times_lanes<I + 1>(x, y);
     }
+}
+
+// The largest of x[i] c + (lane i's y) and u.
+template <int I = 0>
+__device__ __forceinline__ float max_with_lanes(const f32x16& x, float c, float y, float u) {
+    if constexpr (I < 16) {
+        const float lane = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(y), 0x150 + I, 0xF, 0xF, true));
+        return max_with_lanes<I + 1>(x, c, y, fmaxf(u, fmaf(x[I], c, lane)));
+    }
+    return u;
 }
 
 // What a workgroup computes: query tile `tile` of sequence b and one kv head,
@@ -212,11 +232,14 @@ __device__ inline bool chunk_locate(const ChunkArgs& a, ChunkPlanLds& s, int r, 
     return true;
 }
 
-// e with |vs| <= 2^e for all of a tile's V scales, the largest of which is top.  Of a tile
-// whose values are all zero the lowest there is: its scores shall not raise a row's m,
-// under which the weights of tokens with small scales would leave f16's range.
-__device__ __forceinline__ int scale_exponent(float top) {
-    return top > 0.0f ? min(max(__builtin_amdgcn_frexp_expf(top), -60), 60) : -60;
+// Moving sums from reference m to mn >= m: 2^(m - mn) twice halved, as small V scales can put
+// more than fp32's range between two references; l comes back into it.
+__device__ __forceinline__ float half_step(float m, float mn) { return fast_exp2(0.5f * (m - mn)); }
+
+// e with |vs| < 2^e, within [kVsLow, kVsHigh].  A token of value zero has the lowest there is:
+// its score shall not raise m, under which the weights of others would lose bits.
+__device__ __forceinline__ int scale_exponent(float v) {
+    return v > 0.0f ? min(max(__builtin_amdgcn_frexp_expf(v), kVsLow), kVsHigh) : kVsLow;
 }
 
 // LDS exchange within a wave.
@@ -291,8 +314,8 @@ chunk_mfma(const ChunkArgs a) {
         float ks[kChunkKeys];
         float vs[kChunkKeys];
         unsigned vf[LIMBS == 1 ? kChunkKeys : 1];  // V's factor in the f16 tile, twice
-        // x: |vs| <= 2^x; y: log2 of the factor that the f16 tile's V lacks, z: its inverse
-        // (0 and 1 where vs goes into the weights: w)
+        // x: |vs| <= 2^x; w: the tile's scales are far apart; y: log2 of the factor that the f16
+        // tile's V lacks, z: its inverse (0 and 1 where vs goes into the weights)
         float4 v;
     };
     constexpr int kKTile = kChunkKeys * KS, kVTile = kChunkKeys * VS;
@@ -421,19 +444,20 @@ chunk_mfma(const ChunkArgs a) {
         vbad |= !(v < INFINITY);
         vmax = fmaxf(vmax, v);
         if (v > 0.0f) vmin = fminf(vmin, v);
-        // (bits of a float >= 0 order as integers)
-        const float top = __int_as_float(__builtin_amdgcn_readlane(wave_inclusive_max_nonneg(__float_as_int(v)), kWave - 1));
-        const int e = scale_exponent(top);
+        // (bits of a float >= 0 order as integers; their top ones are the exponent)
+        const int top = __builtin_amdgcn_readlane(wave_inclusive_max_nonneg(__float_as_int(v)), kWave - 1);
+        const int e = (top >> 23) - 126;
+        const bool in = k0 + tile * kChunkKeys + lane < k1;
+        const bool spread = __builtin_amdgcn_ballot_w64(in && __float_as_int(v) < top - (kSpreadBits<LIMBS> << 23)) != 0 || e < -kVfRange || e > kVfRange;
+        const float unit = spread ? 1.0f : __int_as_float((127 - e) << 23);  // 2^-e
         x.ks[lane] = ksr;
         x.vs[lane] = vsr;
-        // bf16: vs / 2^e goes into V's f16 tile, unless some token's would be subnormal there.
-        const bool in_weights = LIMBS == 2 || __builtin_amdgcn_ballot_w64(v > 0.0f && v < ldexpf(1.0f, e - kVfBits)) != 0;
         if (LIMBS == 1) {
-            const _Float16 h = in_weights ? static_cast<_Float16>(1.0f) : static_cast<_Float16>(ldexpf(vsr, -e));
+            const _Float16 h = static_cast<_Float16>(spread ? 1.0f : vsr * unit);
             x.vf[LIMBS == 1 ? lane : 0] = __builtin_bit_cast(unsigned, h16x2{h, h});
         }
-        const float lv = static_cast<float>(e);
-        if (lane == 0) x.v = in_weights ? make_float4(lv, 0.0f, 1.0f, 1.0f) : make_float4(lv, lv, ldexpf(1.0f, -e), 0.0f);
+        const float lv = static_cast<float>(min(max(e, kVsLow), kVsHigh));
+        if (lane == 0) x.v = make_float4(lv, spread ? 0.0f : lv, unit, spread ? 1.0f : 0.0f);
     };
     int far_id = 0;
     if (tiles > 0 && wave == 0 && !narrow) {
@@ -606,16 +630,24 @@ chunk_mfma(const ChunkArgs a) {
         float top = p[0][0];
 #pragma unroll
         for (int i = 1; i < 32; i++) top = fmaxf(top, p[i / 16][i % 16]);
+        const float4 sv = sc.v;
+        const bool spread = __builtin_amdgcn_readfirstlane(__float_as_int(sv.w)) != 0;
         // m is a reference that weights pass by up to 2^kWeightTop: it moves, with the
         // state, only when some row's could pass by more.
-        const float4 sv = sc.v;
-        const float u = fmaf(top, c_row, sv.x);
+        float u = fmaf(top, c_row, sv.x);
         if (__builtin_amdgcn_ballot_w64(u > m + kWeightTop) != 0) {
+            if (spread) {
+                u = -INFINITY;
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++)
+                    u = max_with_lanes(p[kb], c_row, static_cast<float>(scale_exponent(fabsf(sc.vs[32 * kb + scale_at]))), u);
+            }
             const float un = fmaxf(u, __shfl_xor(u, 32)) - kWeightReset;
             const float mn = un > m ? un : m;
-            const float alpha = mn == -INFINITY ? 1.0f : fast_exp2(m - mn);
+            const float half = mn == -INFINITY ? 1.0f : half_step(m, mn);
+            const float alpha = half * half;
             m = mn;
-            l *= alpha;
+            l = l * half * half;
 #pragma unroll
             for (int c = 0; c < NB; c++)
 #pragma unroll
@@ -646,7 +678,7 @@ chunk_mfma(const ChunkArgs a) {
             }
             l = fmaf((part[0] + part[1]) + (part[2] + part[3]), LIMBS == 1 ? sv.z : 1.0f, l);
         };
-        if (LIMBS == 2 || __builtin_amdgcn_readfirstlane(__float_as_int(sv.w)) != 0) weights(yes);
+        if (LIMBS == 2 || spread) weights(yes);
         else weights(no);
     };
     // Rows and scales ahead of tile i's: scales of tile i + 2 are stored, rows and
@@ -692,11 +724,12 @@ chunk_mfma(const ChunkArgs a) {
         __builtin_amdgcn_raw_buffer_store_b64(v2i_t{__float_as_int(m_row), __float_as_int(l_row)}, ml_rs, row * 8, 0, kChunkCoherent);
     };
 
-    // Whether the scales that this wave knows of are beyond f16 weights, or q scaled to 2^15.
+    // Whether the scales that this wave knows of are not finite, or beyond what m and q scaled
+    // to 2^15 cover.
     auto out_of_range = [&]() {
         const float top = wave_max(vmax), low = -wave_max(-vmin);
         return __builtin_amdgcn_ballot_w64(vbad || kmax > kKsMax) != 0 ||
-               (top > 0.0f && (top > kVsMax || low < kVsMin || top > low * kVsRatio<LIMBS>));
+               top > kVsMax || low < kVsMin<LIMBS>;
     };
     if (narrow) {
         // Each wave takes every W-th block of 32 keys, with nothing to wait for but its
@@ -734,8 +767,8 @@ chunk_mfma(const ChunkArgs a) {
             vbad |= !(v < INFINITY);
             vmax = fmaxf(vmax, v);
             if (v > 0.0f) vmin = fminf(vmin, v);
-            const float vtop = __int_as_float(__builtin_amdgcn_readlane(wave_inclusive_max_nonneg(__float_as_int(v)), kWave - 1));
-            const float lv = static_cast<float>(scale_exponent(vtop));
+            const int vtop = __builtin_amdgcn_readlane(wave_inclusive_max_nonneg(__float_as_int(v)), kWave - 1);
+            const int e = min(max((vtop >> 23) - 126, kVsLow), kVsHigh);
             times_lanes(p, __shfl(x.ks, scale_key));
             const int t0 = k0 + blk * 32;
             if (t0 + 32 > keys_all) {
@@ -746,13 +779,17 @@ chunk_mfma(const ChunkArgs a) {
             float top = p[0];
 #pragma unroll
             for (int i = 1; i < 16; i++) top = fmaxf(top, p[i]);
-            const float u = fmaf(top, c_row, lv);
+            float u = fmaf(top, c_row, static_cast<float>(e));
             if (__builtin_amdgcn_ballot_w64(u > m + kWeightTop) != 0) {
+                // (tokens' scales too far apart)
+                if (__builtin_amdgcn_ballot_w64(k0 + blk * 32 + c32 < k1 && __float_as_int(v) < vtop - (kSpreadBits<LIMBS> << 23)) != 0 || e == kVsLow)
+                    u = max_with_lanes(p, c_row, __shfl(static_cast<float>(scale_exponent(v)), scale_key), -INFINITY);
                 const float un = fmaxf(u, __shfl_xor(u, 32)) - kWeightReset;
                 const float mn = un > m ? un : m;
-                const float alpha = mn == -INFINITY ? 1.0f : fast_exp2(m - mn);
+                const float half = mn == -INFINITY ? 1.0f : half_step(m, mn);
+                const float alpha = half * half;
                 m = mn;
-                l *= alpha;
+                l = l * half * half;
 #pragma unroll
                 for (int c = 0; c < NB; c++)
 #pragma unroll
@@ -828,8 +865,12 @@ chunk_mfma(const ChunkArgs a) {
         for (int i = 0; i < W; i++) M = fmaxf(M, s_ml[i][c32][0]);
         const float Ms = M == -INFINITY ? 0.0f : M;
 #pragma unroll
-        for (int i = 0; i < W; i++) L = fmaf(s_ml[i][c32][1], fast_exp2(s_ml[i][c32][0] - Ms), L);
-        const float f = fast_exp2(m - Ms);
+        for (int i = 0; i < W; i++) {
+            const float half = half_step(s_ml[i][c32][0], Ms);
+            L = fmaf(s_ml[i][c32][1] * half, half, L);
+        }
+        const float own = half_step(m, Ms);
+        const float f = own * own;
 #pragma unroll
         for (int c = 0; c < NB; c++)
 #pragma unroll
@@ -941,7 +982,7 @@ chunk_mfma(const ChunkArgs a) {
         __syncthreads();
     }
 
-    // Scales that f16 weights, or q scaled to 2^15, do not cover.
+    // Those rows are computed in fp32, hundreds of times slower.
     if (wave == 0) {
         const bool bad = out_of_range();
         if (lane == 0) s_flag = bad;
@@ -1021,17 +1062,19 @@ chunk_mfma(const ChunkArgs a) {
 #pragma unroll
             for (int i = 0; i < kDeep; i++) top = fmaxf(top, __int_as_float(ml[i].x));
             const float Ms = top == -INFINITY ? 0.0f : top;
-            const float alpha = fast_exp2(M - Ms);
+            const float moved = half_step(M, Ms);
+            const float alpha = moved * moved;
             M = top;
-            L *= alpha;
+            L = L * moved * moved;
 #pragma unroll
             for (int j = 0; j < 4; j++) A[j] *= alpha;
 #pragma unroll
             for (int i = 0; i < kDeep; i++) {
                 const float mi = __int_as_float(ml[i].x), li = __int_as_float(ml[i].y);
                 if (i0 + i >= w.nsplit || (mi == -INFINITY && li == 0.0f)) continue;  // (or no key of this split)
-                const float f = fast_exp2(mi - Ms);
-                L = fmaf(li, f, L);
+                const float half = half_step(mi, Ms);
+                const float f = half * half;
+                L = fmaf(li * half, half, L);
 #pragma unroll
                 for (int j = 0; j < 4; j++) A[j] = fmaf(__int_as_float(acc[i][j]), f, A[j]);
             }

@@ -86,6 +86,72 @@ def test_the_token_with_the_weight_has_a_tiny_scale(half_steps, n, dtype):
         check(i)
 
 
+@pytest.mark.parametrize("bits", [-19, -23, -30, -41, -57, -70])
+@pytest.mark.parametrize("n", [30, 3])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_the_token_with_the_weight_has_a_scale_far_below(bits, n, dtype):
+    for seed, d in ((0, 64), (1, 192)):
+        i = ref.batch(seed, [(200, n), (900, n)], 4, 1, d, 16, dtype)
+        sink(i, 0, 5 + seed, 2.0**bits)
+        check(i)
+
+
+@pytest.mark.parametrize("gap", [4.0, 12.0, 20.0, 26.0, 40.0])
+@pytest.mark.parametrize("n", [30, 3])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_the_token_with_the_weight_has_the_value_zero(gap, n, dtype):
+    """Its score is about `gap` (log2) above the others', of whose weights the output then consists."""
+    for seed, d in ((0, 64), (1, 128)):
+        i = ref.batch(seed, [(200, n)], 4, 1, d, 16, dtype)
+        sink(i, 0, 5, 0.0)
+        p, at = pool_at(i, 0, 5)
+        i["v"][p, :, at] = 0
+        i["ks"][p, :, at] = gap * 0.6931 * d**0.5 / (30.0 * 127)
+        check(i)
+
+
+@pytest.mark.parametrize("low,high", [(-80, 58), (-85, -30), (-20, 59), (-70, 10)])
+@pytest.mark.parametrize("pairs", [[(2000, 1)], [(2000, 70)], [(700, 1)] * 130, [(700, 40)] * 130])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_scales_of_two_sizes(low, high, pairs, dtype):
+    """The first and the second half of the tokens far apart: the weights' sum keeps both."""
+    for first, second in ((low, high), (high, low)):
+        i = ref.batch(21, pairs, 4, 2, 64, 16, dtype)
+        g = torch.Generator(device="cuda")
+        g.manual_seed(5)
+        r = torch.rand(i["vs"].shape, generator=g, device="cuda")
+        x = torch.exp2(r + second)
+        page = i["k"].shape[2]
+        for b, (length, _) in enumerate(pairs):
+            ids = i["block_table"][b, :length // 2 // page].long()
+            x[ids] = torch.exp2(r[ids] + first)
+        i["vs"] = torch.where(torch.isnan(i["vs"]), i["vs"], x)
+        check(i)
+
+
+@pytest.mark.parametrize("tiny", [1e-7, 1e-20, 0.0])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_token_of_tiny_value_does_not_slow_its_sequence(tiny, dtype):
+    """A padding token's V row next to nothing; 512 tokens over 4096 stay on the matrix cores (in fp32, a row at a time,
+    they take hundreds of times as long)."""
+    i = ref.batch(22, [(4096, 512)], 8, 2, 128, 16, dtype)
+    ms = []
+    for value in (0.01, tiny):
+        p, at = pool_at(i, 0, 3)
+        i["vs"][p, :, at] = value
+        h = attention(i)
+        begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        times = []
+        for _ in range(5):
+            begin.record()
+            h()
+            end.record()
+            torch.cuda.synchronize()
+            times.append(begin.elapsed_time(end))
+        ms.append(min(times))
+    assert ms[1] < 5 * ms[0], ms
+
+
 # ---- scales of zero -------------------------------------------------------------
 def values_of_zero(i, tokens, low):
     """V scales of 2^low to 2^(low + 1), but zero for `tokens` of every sequence."""

@@ -168,6 +168,24 @@ hipError_t kvq_chunk_attention_launch(const kvq_chunk_attention_params* p, void*
     return checked_call(stream, [&] { return kvq::launch_chunk(a, plan, workspace, stream); });
 }
 
+hipError_t kvq_chunk_attention_plan(const kvq_chunk_attention_params* p, kvq_plan_info* info) {
+    if (!info || !chunk_params_ok(p)) return hipErrorInvalidValue;
+    const kvq::ChunkArgs a = chunk_args(p);
+    const kvq::ChunkPlan plan = kvq::chunk_plan(a, chunk_vec_ok(p, a));
+    kvq_plan_info r{};
+    r.kernel = plan.mfma ? KVQ_KERNEL_CHUNK_MFMA : KVQ_KERNEL_CHUNK_GENERIC;
+    r.heads_per_group = plan.mfma ? a.G : 1;
+    const bool split = plan.records > 0;
+    r.splits = split ? 0 : 1;
+    r.chunk = split ? 0 : a.max_len;
+    r.split_plan = split ? KVQ_SPLITS_IN_KERNEL : KVQ_SPLITS_STATIC;
+    r.query_block = plan.mfma ? plan.rows : 1;
+    r.workspace_bytes = plan.bytes;
+    r.tile_tokens = plan.mfma ? kvq::kChunkKeys : 0;
+    *info = r;
+    return hipSuccess;
+}
+
 size_t kvq_page_fork_workspace_size(const kvq_page_fork_params* p) {
     return fork_params_ok(p) ? kvq::fork_workspace(fork_args(p)) : 0;
 }

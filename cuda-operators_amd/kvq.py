@@ -208,6 +208,7 @@ class PlanInfo(ctypes.Structure):
 
 KERNEL_DECODE_GENERIC, KERNEL_DECODE_VALU, KERNEL_DECODE_MFMA = 0, 1, 2
 KERNEL_ATTENTION_MFMA, KERNEL_ATTENTION_ROWS, KERNEL_ATTENTION_GENERIC, KERNEL_ATTENTION_DIRECT = 3, 4, 5, 6
+KERNEL_CHUNK_MFMA, KERNEL_CHUNK_GENERIC = 7, 8
 SPLITS_STATIC, SPLITS_IN_KERNEL, SPLITS_SCHEDULE, SPLITS_TILES = 0, 1, 2, 3
 
 EXPORTS = ("solve", "kv_int8_split_launch", "kv_int8_simple_launch", "kvq_decode_workspace_size",
@@ -220,7 +221,7 @@ EXPORTS = ("solve", "kv_int8_split_launch", "kv_int8_simple_launch", "kvq_decode
            "kvq_page_bounds_launch", "kvq_sparse_decode_workspace_size", "kvq_sparse_decode_launch",
            "kvq_sparse_decode_plan", "kvq_chunk_attention_workspace_size", "kvq_chunk_attention_launch",
            "kvq_page_fork_workspace_size", "kvq_page_fork_launch", "kvq_page_copy_launch",
-           "kvq_page_compact_workspace_size", "kvq_page_compact_launch")
+           "kvq_page_compact_workspace_size", "kvq_page_compact_launch", "kvq_chunk_attention_plan")
 
 
 class KvqError(RuntimeError):
@@ -299,6 +300,8 @@ def lib() -> ctypes.CDLL:
             size, launch = getattr(L, fn + "_workspace_size"), getattr(L, fn + "_launch")
             size.argtypes, size.restype = [ctypes.POINTER(cls)], ctypes.c_size_t
             launch.argtypes, launch.restype = [ctypes.POINTER(cls), _vp, ctypes.c_size_t, _vp], _int
+        L.kvq_chunk_attention_plan.argtypes = [ctypes.POINTER(ChunkAttentionParams), ctypes.POINTER(PlanInfo)]
+        L.kvq_chunk_attention_plan.restype = _int
         L.kvq_page_copy_launch.argtypes = [ctypes.POINTER(PageCopyParams), _vp]
         L.kvq_page_copy_launch.restype = _int
         _lib = L
@@ -993,6 +996,13 @@ class ChunkAttention(_Planned):
         self._plan("kvq_chunk_attention", p, tensors, stream, workspace)
 
 
+def chunk_attention_plan(p: ChunkAttentionParams) -> PlanInfo:
+    """Plan of kvq_chunk_attention_launch for p (host-only): KERNEL_CHUNK_MFMA, or the far slower KERNEL_CHUNK_GENERIC."""
+    info = PlanInfo()
+    _check("kvq_chunk_attention_plan", lib().kvq_chunk_attention_plan(ctypes.byref(p), ctypes.byref(info)))
+    return info
+
+
 def _pad_ptr(t):
     """A tensor's address; of an empty one some address that is not null (nothing there is read or written)."""
     return t.data_ptr() or 4096
@@ -1247,4 +1257,4 @@ __all__ = ["lib", "version", "solve", "kv_int8_split_launch", "DecodeParams", "A
            "page_map", "slot_write", "slot_read", "new_bounds", "page_bounds", "SparseDecoder", "sparse_decode_plan",
            "CHUNK_MAX_BATCH", "FORK_MAX_BATCH", "ChunkAttentionParams", "PageForkParams", "PageCopyParams",
            "PageCompactParams", "ChunkAttention", "chunk_attention", "PageForker", "page_fork", "new_shares", "page_copy",
-           "PageCompactor", "page_compact"]
+           "PageCompactor", "page_compact", "chunk_attention_plan"]

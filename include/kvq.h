@@ -337,6 +337,8 @@ const char* kvq_version(void);
 #define KVQ_KERNEL_ATTENTION_ROWS 4   /* attention_rows: up to 8 queries per workgroup */
 #define KVQ_KERNEL_ATTENTION_GENERIC 5 /* attention_generic: any head dim or alignment */
 #define KVQ_KERNEL_ATTENTION_DIRECT 6  /* attention_direct: 9-64 queries, 16 per wave, no LDS tiles */
+#define KVQ_KERNEL_CHUNK_MFMA 7        /* chunk_mfma: new tokens over pages on matrix cores */
+#define KVQ_KERNEL_CHUNK_GENERIC 8     /* chunk_generic: a wave a row in fp32, any shape or alignment */
 
 #define KVQ_SPLITS_STATIC 0     /* splits and chunk fixed on the host */
 #define KVQ_SPLITS_IN_KERNEL 1  /* ragged batch planned inside the decode kernel */
@@ -350,10 +352,11 @@ typedef struct kvq_plan_info {
     int splits;             /* static plans: splits per sequence (1 = unsplit); 0 otherwise */
     int chunk;              /* static plans: tokens (keys) per split */
     int split_plan;         /* KVQ_SPLITS_* */
-    int query_block;        /* attention: queries per workgroup; decode: 0 */
+    int query_block;        /* attention: queries per workgroup (chunk attention: rows, one of a head of a
+                               new token each); decode: 0 */
     size_t workspace_bytes; /* workspace (or scratch S) bytes the launch uses */
-    int tile_tokens;        /* decode: tokens one workgroup iteration of the tuned kernel covers
-                               (0: generic kernel); attention: 0 */
+    int tile_tokens;        /* decode and chunk attention: tokens one workgroup iteration of the tuned
+                               kernel covers (0: generic kernel); attention: 0 */
 } kvq_plan_info;
 
 /* The plan of kv_int8_split_launch / kv_int8_simple_launch for these
@@ -602,6 +605,12 @@ typedef struct kvq_chunk_attention_params {
 size_t kvq_chunk_attention_workspace_size(const kvq_chunk_attention_params* p);
 hipError_t kvq_chunk_attention_launch(const kvq_chunk_attention_params* p, void* workspace, size_t workspace_bytes,
                                       hipStream_t stream);
+/* The plan of kvq_chunk_attention_launch for p (part 6).  KVQ_KERNEL_CHUNK_GENERIC, which takes hundreds
+ * of times as long, runs where q or out do not begin on 16 bytes or a token's stride is no multiple of 16
+ * bytes, k_pages or v_pages do not begin on 8, head_dim is above 256 or no multiple of 8, there are
+ * more than 128 query heads a kv head, or more than 2^22 query tiles.  With KVQ_SPLITS_IN_KERNEL the keys
+ * of the sequences are split by their lengths (splits 0), with KVQ_SPLITS_STATIC nothing is (splits 1). */
+hipError_t kvq_chunk_attention_plan(const kvq_chunk_attention_params* p, kvq_plan_info* info);
 
 typedef struct kvq_page_fork_params {
     int batch;               /* B in [1, KVQ_FORK_MAX_BATCH] */

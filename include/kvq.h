@@ -596,7 +596,11 @@ typedef struct kvq_chunk_attention_params {
  * position lengths[b] - n_b + i; with `causal` it attends the tokens up to that
  * position, without (the states of an encoder, say) all lengths[b] of them.  A row
  * with no token to attend is zero; rows at or behind token_offsets[B] are left as
- * they are.  The math is part 1's for each row; bf16 outputs are rounded once.
+ * they are.  The math is part 1's for each row, with scores, sums and the softmax's
+ * statistics in fp32.  fp32 rows' weights are two f16 halves, as in part 1.  bf16 rows' are
+ * one f16, and V codes times their scale another, so a token's term is off by up to 3 * 2^-11
+ * of itself before the sum is rounded to bf16 (2^-8): outputs may be the neighbouring bf16 value
+ * of what fp32 arithmetic would give.
  * A contiguous cache [B, Hkv, capacity, d] is a pool of B pages of `capacity`
  * tokens with the block table 0, 1, .., B - 1.
  * Workspace: kvq_chunk_attention_workspace_size bytes, zero-filled once

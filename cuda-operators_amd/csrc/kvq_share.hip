@@ -211,18 +211,18 @@ __global__ __launch_bounds__(256) void fork_write_kernel(const ForkArgs a) {
 // ---------------------------------------------------------------------------
 // A pair's arrays in one layer are laid end to end in pieces of 16 bytes (or 4, or
 // 1, where an array's place or page size is not a multiple); a workgroup takes
-// kCopyPieces of a thread's at a time, whose loads go out together.  Bound by HBM: 48
+// kCopyLoads of a thread's at a time, whose loads go out together.  Bound by HBM: 48
 // pages of 64 tokens in 32 layers of 8 heads, d = 128 (415 MB read and written), 74.6 us
 // a call, 67.5 the kernel; a large copy at 5.08 TB/s would take 82.
 constexpr int kCopyLoads = 4;
+// Pairs of all layers up to which each has workgroups of its own; more go to this many, 16 for
+// each that fits the chip.  50,000 pairs of 4.4 KB in 32 layers, none, 1000 or 12,000 of them to
+// copy: 32, 59 and 375 us, with a workgroup a pair 518, 560 and 837; but 48 of 135 KB in 32 layers
+// 73, with workgroups of their own 67.
+constexpr unsigned kCopyGroups = 1 << 15;
 
 template <class T>
-__global__ __launch_bounds__(256) void page_copy_kernel(const CopyArgs a) {
-    const unsigned unit = blockIdx.x;  // (layer, pair)
-    const unsigned layer = fastdiv(unit, a.pairs);
-    const int i = static_cast<int>(unit - layer * a.n);
-    const int src = a.src[i], dst = a.dst[i];
-    if (src < 0 || src >= a.num_pages || dst < 0 || dst >= a.num_pages) return;
+__device__ __forceinline__ void copy_page(const CopyArgs& a, unsigned layer, int src, int dst) {
     const size_t first = static_cast<size_t>(layer) * a.num_pages;
     for (size_t p0 = static_cast<size_t>(blockIdx.y) * (256 * kCopyLoads); p0 < a.pieces;
          p0 += static_cast<size_t>(gridDim.y) * (256 * kCopyLoads)) {
@@ -245,6 +245,40 @@ __global__ __launch_bounds__(256) void page_copy_kernel(const CopyArgs a) {
 #pragma unroll
         for (int u = 0; u < kCopyLoads; u++)
             if (to[u]) *reinterpret_cast<T*>(to[u]) = x[u];
+    }
+}
+
+// A workgroup (or some, along y) for each (layer, pair).
+template <class T>
+__global__ __launch_bounds__(256) void page_copy_kernel(const CopyArgs a) {
+    const unsigned unit = blockIdx.x;
+    const unsigned layer = fastdiv(unit, a.pairs);
+    const int i = static_cast<int>(unit - layer * a.n);
+    const int src = a.src[i], dst = a.dst[i];
+    if (src < 0 || src >= a.num_pages || dst < 0 || dst >= a.num_pages) return;
+    copy_page<T>(a, layer, src, dst);
+}
+
+// Long lists, which may be mostly -1 (a compaction's): workgroups take every so many a pair,
+// and read 64 of theirs at once.
+template <class T>
+__global__ __launch_bounds__(256) void page_copy_list_kernel(const CopyArgs a) {
+    const unsigned lane = threadIdx.x & (kWave - 1);
+    const unsigned units = static_cast<unsigned>(a.n) * a.layers;
+    for (unsigned u0 = blockIdx.x; u0 < units; u0 += gridDim.x * kWave) {
+        const unsigned unit = u0 + lane * gridDim.x;
+        unsigned layer = 0;
+        int src = -1, dst = -1;
+        if (unit < units) {
+            layer = fastdiv(unit, a.pairs);
+            src = a.src[unit - layer * a.n];
+            dst = a.dst[unit - layer * a.n];
+        }
+        unsigned long long live = __builtin_amdgcn_ballot_w64(src >= 0 && src < a.num_pages && dst >= 0 && dst < a.num_pages);
+        for (; live; live &= live - 1) {
+            const int l = __builtin_ctzll(live);
+            copy_page<T>(a, __builtin_amdgcn_readlane(layer, l), __builtin_amdgcn_readlane(src, l), __builtin_amdgcn_readlane(dst, l));
+        }
     }
 }
 
@@ -507,8 +541,13 @@ hipError_t launch_copy(CopyArgs a, hipStream_t stream) {
         if (a.base[k]) a.pieces += a.bytes[k] / sizeof(T);
     }
     a.pairs = make_fastdiv(static_cast<uint32_t>(a.n));
-    const dim3 grid(static_cast<unsigned>(a.n) * a.layers, blocks(static_cast<long long>(a.pieces), 256 * kCopyLoads, 1024));
-    hipLaunchKernelGGL((page_copy_kernel<T>), grid, dim3(256), 0, stream, a);
+    const unsigned units = static_cast<unsigned>(a.n) * a.layers;
+    if (units <= kCopyGroups) {
+        const dim3 grid(units, blocks(static_cast<long long>(a.pieces), 256 * kCopyLoads, 1024));
+        hipLaunchKernelGGL((page_copy_kernel<T>), grid, dim3(256), 0, stream, a);
+    } else {
+        hipLaunchKernelGGL((page_copy_list_kernel<T>), dim3(kCopyGroups), dim3(256), 0, stream, a);
+    }
     return hipGetLastError();
 }
 }  // namespace

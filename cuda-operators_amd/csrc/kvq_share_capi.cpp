@@ -203,7 +203,9 @@ hipError_t kvq_page_copy_launch(const kvq_page_copy_params* p, hipStream_t strea
     if (!p || p->copies < 0 || p->layers < 1 || p->layers > 65535 || !heads_ok(p->num_kv_heads, p->head_dim) ||
         !slots_ok(p->page_size, p->num_pages) || (p->bounds == nullptr) != (p->bound_scale == nullptr))
         return hipErrorInvalidValue;
-    if (static_cast<long long>(p->copies) * p->layers >= 1LL << 24) return hipErrorInvalidValue;  // workgroups along x
+    // Pairs of all layers are numbered in 32 bits; a list longer than the pool has mostly nothing to copy.
+    const long long units = static_cast<long long>(p->copies) * p->layers;
+    if (p->copies >= 1 << 24 || units > INT_MAX || (units >= 1 << 24 && p->copies > p->num_pages)) return hipErrorInvalidValue;
     if (!p->src || !p->dst || !p->k_pages || !p->v_pages || !p->k_scale_pages || !p->v_scale_pages)
         return hipErrorInvalidValue;
     kvq::CopyArgs a{};

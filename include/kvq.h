@@ -663,7 +663,7 @@ hipError_t kvq_page_fork_launch(const kvq_page_fork_params* p, void* workspace, 
                                 hipStream_t stream);
 
 typedef struct kvq_page_copy_params {
-    int copies;               /* n >= 0 pairs; n * layers < 2^24 */
+    int copies;               /* 0 <= n < 2^24 pairs; n * layers < 2^31, and < 2^24 where n > num_pages */
     int layers;               /* pools of the same shape one behind the other, 1 to 65535 */
     int num_kv_heads, head_dim;
     int page_size, num_pages; /* of one layer's pool; num_pages * page_size <= INT_MAX */

@@ -8,24 +8,26 @@
 // products run on the f16 matrix cores (32x32x16): S^T = K q^T, O^T = V^T P^T, whose
 // results both have a row of q per lane, so m, the sum and the rescaling of O
 // need no exchange.  ks multiplies S, a key per register, by a DPP broadcast; vs goes
-// into V's f16 tile (bf16, but where a tile's differ too much for f16), or into p.  fp32 takes q and p as two f16 limbs.
+// into V's f16 tile (bf16, unless a tile's are too far apart for f16), or into p.  fp32
+// takes q and p as two f16 limbs.
 //
 // Rows of a kv head's G query heads and of neighbouring tokens share a tile, so
 // codes are read once per waves * 32 rows.  What bounds it then, at 2048 new tokens of
-// 32 query heads over 8 kv heads, d = 128, behind 30,720 others (1065 GFLOP, 1197 us, 890
-// TFLOP/s; a bf16 8192^3 library product runs 1208): matrix cores are busy 38 % of the
-// cycles, and the vector ALU's share (softmax, codes to f16: 309 M wave instructions)
-// takes about as long, so the two have to overlap:
-// * Four waves of 32 rows, one a SIMD, one after the other in program order: 1398 us.
+// 32 query heads over 8 kv heads, d = 128, behind 30,720 others (1065 GFLOP; 1234 to 1256 us on
+// three boxes, 848 to 863 TFLOP/s; a bf16 8192^3 library product runs 1208 to 1246): matrix
+// cores are busy 38 % of the cycles, and the vector ALU's share (softmax, codes to f16: 312 M
+// wave instructions) takes about as long, so the two have to overlap:
+// * Four waves of 32 rows, one a SIMD, one after the other in program order: 1398 us, when
+//   eight took 1197.
 // * Eight waves in two phases, each SIMD's pair in opposite ones, a barrier after
-//   each phase: 1197 us.  The matrix phase by itself takes 556 us, softmax 390, the
-//   two without conversion and loads 882.
+//   each phase.  The matrix phase by itself takes 556 us, softmax 390, the two without
+//   conversion and loads 882.
 // * Tiles of 64 keys: V, K and the rows' state fit two waves a SIMD (256 registers).
 // * Operands are read kAhead MFMAs early (4 and 8 for bf16: within 2 %).  Priorities
 //   (s_setprio) gain nothing; reading scales before the matrix phase 1269 against 1211 us.
 // Tiles of up to 32 rows take the narrow path, which is bound by bytes: 64 single
-// tokens over 512 to 8192 keys 158 us (3.7 TB/s; by the wide path 403), one over
-// 131,072 keys 61 us (4.5 TB/s; a copy moves 5.08).
+// tokens over 512 to 8192 keys 160 us (3.7 TB/s; by the wide path 403), one over
+// 131,072 keys 62 us (4.5 TB/s; a copy moves 5.08 to 5.14).
 #pragma once
 
 #include <limits.h>
@@ -232,8 +234,9 @@ __device__ inline bool chunk_locate(const ChunkArgs& a, ChunkPlanLds& s, int r, 
     return true;
 }
 
-// Moving sums from reference m to mn >= m: 2^(m - mn) twice halved, as small V scales can put
-// more than fp32's range between two references; l comes back into it.
+// The root of what sums are multiplied by when their reference moves from m to mn: applied
+// twice, as V scales of 2^-80 and 2^60 put more than fp32's range between two references,
+// and l, which they are not in, has to come through.
 __device__ __forceinline__ float half_step(float m, float mn) { return fast_exp2(0.5f * (m - mn)); }
 
 // e with |vs| < 2^e, within [kVsLow, kVsHigh].  A token of value zero has the lowest there is:
@@ -982,7 +985,8 @@ chunk_mfma(const ChunkArgs a) {
         __syncthreads();
     }
 
-    // Those rows are computed in fp32, hundreds of times slower.
+    // Then all its rows are computed in fp32, one after the other (one V scale of 1e-30 before 512
+    // tokens over 8192 keys: 41 ms, not 0.12).
     if (wave == 0) {
         const bool bad = out_of_range();
         if (lane == 0) s_flag = bad;

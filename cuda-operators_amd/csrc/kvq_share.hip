@@ -39,8 +39,8 @@ __device__ __forceinline__ int group_scan(int v, int& total, int (&part)[kWaves]
 // inside it.  Three launches: entries are counted by atomics on the page (sums
 // and a max of integers: any order gives the same), one workgroup decides, in
 // page and row order by prefix sums, and the rows are written.  Bound by latency: 16 rows
-// on pages of 64 tokens take 11.5 us a call, 256 of up to 4096 tokens on pages of 16
-// 17.6; the kernels are 2.3 to 6.1 and up to 10.5 us each.
+// on pages of 64 tokens take 11.5 to 13.7 us a call, 256 of up to 4096 tokens on pages of 16
+// 17.7; count, decide and write are 3.6, 4.7 and 2.8 us, and 6.7, 8.8 and 3.0.
 
 struct ForkRow {
     int parent;  // -1: none
@@ -212,8 +212,9 @@ __global__ __launch_bounds__(256) void fork_write_kernel(const ForkArgs a) {
 // A pair's arrays in one layer are laid end to end in pieces of 16 bytes (or 4, or
 // 1, where an array's place or page size is not a multiple); a workgroup takes
 // kCopyLoads of a thread's at a time, whose loads go out together.  Bound by HBM: 48
-// pages of 64 tokens in 32 layers of 8 heads, d = 128 (415 MB read and written), 74.6 us
-// a call, 67.5 the kernel; a large copy at 5.08 TB/s would take 82.
+// pairs of pages of 64 tokens in 32 layers of 8 heads, d = 128, 42 of them to copy, from 23
+// pages (281 MB read and written): 75 us a call, 65 to 69 the kernel (4.1 TB/s or more); a
+// large copy of as much at 5.08 TB/s would take 55.
 constexpr int kCopyLoads = 4;
 // Pairs of all layers up to which each has workgroups of its own; more go to this many, 16 for
 // each that fits the chip.  50,000 pairs of 4.4 KB in 32 layers, none, 1000 or 12,000 of them to
@@ -287,9 +288,10 @@ __global__ __launch_bounds__(256) void page_copy_list_kernel(const CopyArgs a) {
 // ---------------------------------------------------------------------------
 // Moves are decided by one workgroup: the i-th free page from below takes the i-th
 // page in use from above, as long as it lies lower, and both lists are prefix sums.
-// Bound by launches and latency: 16 rows of up to 2048 tokens on pages of 64 take 9.7 us a
-// call, 256 of up to 4096 on pages of 16 (50,000 pages) 12.4.  With all lists written by
-// the one workgroup that scans, and one load at a time, the latter took 32.9.
+// Bound by launches and latency: 16 rows of up to 2048 tokens on pages of 64 take 9.7 to 12.7
+// us a call, 256 of up to 4096 on pages of 16 (50,000 pages) 11.7 to 12.4 (32.9
+// with all lists written by the one workgroup that scans, and one load at a time), 64 on 261,000
+// pages 36.  Above 2^18 pages the one workgroup does all: 264,000 take 523 us, 524,000 1075.
 // A page's state: kFree, 0 in use, or where it moves to, + 1.
 constexpr int kFree = -1;
 

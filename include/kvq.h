@@ -600,7 +600,9 @@ typedef struct kvq_chunk_attention_params {
  * statistics in fp32.  fp32 rows' weights are two f16 halves, as in part 1.  bf16 rows' are
  * one f16, and V codes times their scale another, so a token's term is off by up to 3 * 2^-11
  * of itself before the sum is rounded to bf16 (2^-8): outputs may be the neighbouring bf16 value
- * of what fp32 arithmetic would give.
+ * of what fp32 arithmetic would give.  Scales that are not finite, of K above 2^80 or of V
+ * above 2^60 or (not zero) below 2^-90 (fp32: 2^-86) send the rows of the workgroups that see
+ * them, up to 256 each, through fp32 arithmetic, hundreds of times slower.
  * A contiguous cache [B, Hkv, capacity, d] is a pool of B pages of `capacity`
  * tokens with the block table 0, 1, .., B - 1.
  * Workspace: kvq_chunk_attention_workspace_size bytes, zero-filled once

@@ -90,7 +90,7 @@ def test_the_token_with_the_weight_has_a_tiny_scale(half_steps, n, dtype):
 @pytest.mark.parametrize("n", [30, 3])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_the_token_with_the_weight_has_a_scale_far_below(bits, n, dtype):
-    for seed, d in ((0, 64), (1, 192)):
+    for seed, d in ((0, 64), (1, 192), (2, 256)):
         i = ref.batch(seed, [(200, n), (900, n)], 4, 1, d, 16, dtype)
         sink(i, 0, 5 + seed, 2.0**bits)
         check(i)

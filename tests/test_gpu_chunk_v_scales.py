@@ -129,6 +129,20 @@ def test_scales_of_two_sizes(low, high, pairs, dtype):
         check(i)
 
 
+@pytest.mark.parametrize("step", [0.25, -0.25, 0.07, -0.07])
+@pytest.mark.parametrize("pairs", [[(230, 230)], [(230, 9)], [(200, 200), (230, 64), (7, 7)] * 20])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_scales_that_grow_from_token_to_token(step, pairs, dtype):
+    """The largest scales of a tile belong to tokens that its first rows do not see, or the smallest."""
+    for d in (64, 128, 256):
+        i = ref.batch(d, pairs, 4, 2, d, 16, dtype)
+        page = i["k"].shape[2]
+        for b, (length, _) in enumerate(pairs):
+            t = torch.arange(length, device="cuda")
+            i["vs"][i["block_table"][b, t // page].long(), :, t % page] = torch.exp2(step * t - 20.0)[:, None]
+        check(i)
+
+
 @pytest.mark.parametrize("tiny", [1e-7, 1e-20, 0.0])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_a_token_of_tiny_value_does_not_slow_its_sequence(tiny, dtype):

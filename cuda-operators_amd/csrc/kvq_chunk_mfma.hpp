@@ -14,7 +14,7 @@
 // Rows of a kv head's G query heads and of neighbouring tokens share a tile, so
 // codes are read once per waves * 32 rows.  What bounds it then, at 2048 new tokens of
 // 32 query heads over 8 kv heads, d = 128, behind 30,720 others (1065 GFLOP; 1234 to 1256 us on
-// three boxes, 848 to 863 TFLOP/s; a bf16 8192^3 library product runs 1208 to 1246): matrix
+// three GPUs, 848 to 863 TFLOP/s; a bf16 8192^3 library product runs 1208 to 1246): matrix
 // cores are busy 38 % of the cycles, and the vector ALU's share (softmax, codes to f16: 312 M
 // wave instructions) takes about as long, so the two have to overlap:
 // * Four waves of 32 rows, one a SIMD, one after the other in program order: 1398 us, when
